@@ -206,7 +206,8 @@ def prepare(case, seed):
         s["out"] = torch.empty_like(s["q"])
     if own:
         s["lg"] = importlib.import_module("little-gemma_b200")
-        s["cache"] = s["lg"].PagedCache(s["k_cache"], s["v_cache"], s["table"], s["len"], s["free"], s["n_free"])
+        stack = (s["free"], s["n_free"]) if op == "step" else ()
+        s["cache"] = s["lg"].PagedCache(s["k_cache"], s["v_cache"], s["table"], s["len"], *stack)
         if op == "attn":
             s["work"] = torch.empty(s["cache"].attn_work(case["requests"], case["new"], case["heads"]), dtype=torch.uint8, device="cuda")
     return s

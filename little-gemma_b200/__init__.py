@@ -36,6 +36,9 @@ ABI_SYMBOLS = [
     "lg_dense_pair_host", "lg_row_norm_pair_host", "lg_mixer_blocks_host",
 ]
 
+# every symbol include/lg_serve.h declares
+SERVE_SYMBOLS = ["lg_paged_step", "lg_paged_append", "lg_paged_attn_work", "lg_paged_attn", "lg_sample", "lg_forward_sample"]
+
 class PlanLayer(C.Structure):
     """struct lg_plan_layer of include/lg_plan.h"""
     _fields_ = [(n, C.c_int) for n in ("mixer", "heads", "dim", "rot_dim", "vdim", "q_rank", "kv_rank", "kv_src", "rot_dims")] + \
@@ -44,6 +47,17 @@ class PlanLayer(C.Structure):
 
 
 MIX_LATENT, MIX_GROUPED, MIX_SSM = 1, 2, 3
+
+
+class PagedDesc(C.Structure):
+    """struct lg_paged_cache of include/lg_serve.h"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_longlong) for n in ("page_stride", "row_stride", "head_stride")] + \
+               [(n, C.c_int) for n in ("type", "n_pages", "page_size", "n_kv_heads", "head_dim", "max_req", "max_pages", "table_stride")] + \
+               [(n, C.c_void_p) for n in ("table", "len", "free_pages", "n_free", "status")]
+
+
+# bits of a paged cache's status word (include/lg_serve.h)
+PAGED_NO_PAGES, PAGED_TOO_LONG, PAGED_NO_ROWS, PAGED_BAD_PAGE, PAGED_BAD_SLOT, PAGED_BAD_ROWS = 1, 2, 4, 8, 16, 32
 
 _lib = None
 
@@ -130,6 +144,15 @@ def load() -> C.CDLL:
                        ("lg_mixer_blocks_host", [C.POINTER(PlanLayer), fl, i, C.POINTER(vp), f, i, _i32p, _i32p, i, i, i, f])):
         getattr(L, name).argtypes = args
         getattr(L, name).restype = i
+    ll = C.c_longlong
+    for name, args, res in (("lg_paged_step", [vp, i, vp, vp, i, vp, vp, vp, vp, vp], i),
+                            ("lg_paged_append", [vp, vp, vp, i, ll, ll, i, vp, vp], i),
+                            ("lg_paged_attn_work", [vp, i, i, i], ll),
+                            ("lg_paged_attn", [vp, vp, i, ll, i, i, i, vp, i, fl, i, vp, ll, vp, ll, vp], i),
+                            ("lg_sample", [vp, i, ll, i, i, vp, vp, vp, vp, vp, vp, vp, vp], i),
+                            ("lg_forward_sample", [vp, vp, i, i, fl, i, fl, fl, fl, C.POINTER(C.c_float)], i)):
+        getattr(L, name).argtypes = args
+        getattr(L, name).restype = res
     _lib = L
     return L
 
@@ -307,6 +330,117 @@ def flash_decode_noalloc(d_q: int, d_k: int, d_v: int, M: int, H: int, n_head_kv
     return int(load().lg_flash_decode_noalloc(d_q, d_k, d_v, M, H, n_head_kv, hd, seq, window, pos, d_out, stream))
 
 
+_SERVE_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 30}
+
+
+def _array(t, dtype: str, n: int, what: str):
+    """Address of a contiguous device tensor of n elements or more; None stays None."""
+    if t is None:
+        return None
+    if str(t.dtype) != dtype or t.numel() < n or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous {dtype} tensor of {n} elements is wanted, not {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _rows(t, heads: int, dim: int, what: str):
+    """(address, type, elements from row to row, rows) of a tensor [rows, heads, dim] or [rows, heads * dim] whose rows are contiguous."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3:
+        ok = shape[1] == heads and shape[2] == dim and (dim == 1 or stride[2] == 1) and (heads == 1 or stride[1] == dim)
+    else:
+        ok = len(shape) == 2 and shape[1] == heads * dim and stride[1] == 1
+    kind = _SERVE_TYPES.get(str(t.dtype))
+    if not ok or kind is None:
+        raise ValueError(f"{what}: rows of {heads} heads of {dim} are wanted, not {t.dtype} {tuple(shape)} with strides {stride}")
+    return t.data_ptr(), kind, max(stride[0], heads * dim) if shape[0] < 2 else stride[0], shape[0]
+
+
+class PagedCache:
+    """A K / V cache of many requests in pages, on device tensors that the caller owns (include/lg_serve.h has the details of every call).
+
+    k, v     [pages, page_size, kv_heads, head_dim] of one type (float32, float16, bfloat16) and with the same strides; the last
+             dimension is contiguous, the others may lie in any order (a transposed view, halves of one tensor)
+    table    int32 [requests, columns]: page ids of each request, in the order of its rows
+    length   int32 [requests]: rows that each request has
+    free, n_free   int32 [pages] and [1]: stack of free page ids and its height; only step() needs them
+    status   int32 [1] or None: bits (PAGED_*) of what the kernels left out; the caller clears it
+
+    The calls enqueue on `stream` (a raw stream handle, 0: the default stream) and wait for nothing."""
+
+    def __init__(self, k, v, table, length, free=None, n_free=None, status=None):
+        kind = _SERVE_TYPES.get(str(k.dtype))
+        if kind is None or k.dtype != v.dtype or k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or (k.shape[3] > 1 and k.stride(3) != 1):
+            raise ValueError(f"k and v: two tensors [pages, page_size, kv_heads, head_dim] of one type and layout are wanted, not {k.dtype} {tuple(k.shape)} "
+                             f"{k.stride()} and {v.dtype} {tuple(v.shape)} {v.stride()}")
+        if str(table.dtype) != "torch.int32" or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1) or table.shape[0] < 1:
+            raise ValueError("table: an int32 tensor [requests, columns] with contiguous rows is wanted")
+        if (free is None) != (n_free is None):
+            raise ValueError("free and n_free come together")
+        self.L = load()
+        self._keep = (k, v, table, length, free, n_free, status)         # the description below holds their addresses
+        ps, rs, hs, _ = k.stride()
+        width = max(table.stride(0), table.shape[1]) if table.shape[0] < 2 else table.stride(0)
+        self.type, self.kv_heads, self.dim = kind, k.shape[2], k.shape[3]
+        self.desc = PagedDesc(k.data_ptr(), v.data_ptr(), ps, rs, hs, kind, k.shape[0], k.shape[1], k.shape[2], k.shape[3], table.shape[0],
+                              table.shape[1], width, table.data_ptr(), _array(length, "torch.int32", table.shape[0], "length"),
+                              _array(free, "torch.int32", k.shape[0], "free"), _array(n_free, "torch.int32", 1, "n_free"),
+                              _array(status, "torch.int32", 1, "status"))
+        self._ref = C.byref(self.desc)
+
+    def step(self, new, start, pos=None, slot=None, req=None, keep=None, stream: int = 0) -> None:
+        """Requests 0 .. len(new)-1 keep their first `keep` rows (None: all) and get `new` rows more: pages, table, lengths and stack are
+        brought up to date; start [requests + 1] and, for each token of the step, pos, slot and req (-1 behind the last) are written."""
+        n = new.numel()
+        rows = [t.numel() for t in (pos, slot, req) if t is not None]
+        cap = min(rows) if rows else 0
+        i32 = "torch.int32"
+        _ok(self.L.lg_paged_step(self._ref, n, _array(keep, i32, n, "keep"), _array(new, i32, n, "new"), cap, _array(start, i32, n + 1, "start"),
+                                 _array(pos, i32, cap, "pos"), _array(slot, i32, cap, "slot"), _array(req, i32, cap, "req"), stream), "paged step")
+
+    def append(self, k, v, slot, stream: int = 0) -> None:
+        """Rows k, v [n, kv_heads, head_dim] (float32 or the cache's type) into slots slot[:n]; -1 skips a row."""
+        pk, tk, lk, n = _rows(k, self.kv_heads, self.dim, "k")
+        pv, tv, lv, nv = _rows(v, self.kv_heads, self.dim, "v")
+        if tk != tv or n != nv:
+            raise ValueError("k and v: the same number of rows of one type is wanted")
+        _ok(self.L.lg_paged_append(self._ref, pk, pv, tk, lk, lv, n, _array(slot, "torch.int32", n, "slot"), stream), "paged append")
+
+    def attn_work(self, n_req: int, n_new: int, n_heads: int) -> int:
+        """Bytes of workspace that attn() wants for so many requests, new tokens a request (at most) and query heads."""
+        n = self.L.lg_paged_attn_work(self._ref, n_req, n_new, n_heads)
+        if n < 0:
+            raise ValueError(f"paged attention: {n_req} requests of {n_new} tokens, {n_heads} heads")
+        return n
+
+    def attn(self, q, out, work, n_new: int = 1, start=None, scale: float = 0.0, window: int = 0, stream: int = 0) -> None:
+        """out = attention of the newest rows of the requests over the cache; q, out [rows, heads, head_dim], float32 or the cache's type.
+        start None: n_new rows for each request in turn; else the row starts that step() wrote, at most n_new rows a request.
+        work: attn_work() bytes of device memory that no other call uses at the same time."""
+        if len(q.shape) != 3 or q.shape != out.shape or q.dtype != out.dtype:
+            raise ValueError("q and out: two tensors [rows, heads, head_dim] of one type are wanted")
+        heads = q.shape[1]
+        pq, tq, lq, rows = _rows(q, heads, self.dim, "q")
+        po, _, lo, _ = _rows(out, heads, self.dim, "out")
+        n_req = rows // max(1, n_new) if start is None else start.numel() - 1
+        _ok(self.L.lg_paged_attn(self._ref, pq, tq, lq, n_req, n_new, rows, _array(start, "torch.int32", 2, "start"), heads, scale, window, po, lo,
+                                 work.data_ptr(), work.numel() * work.element_size(), stream), "paged attention")
+
+
+def sample(logits, u, token, prob=None, temperature=None, top_k=None, top_p=None, min_p=None, stream: int = 0) -> None:
+    """One token from each row of logits [rows, vocab] (device tensors; float32, float16, bfloat16) into token (int32) with the random
+    numbers u in [0, 1) (float32); prob (float32): its share of what was kept.  temperature, top_p, min_p (float32) and top_k (int32) have
+    one value a row; None: 1, or off.  The order of the filters and the draw are described in include/lg_serve.h."""
+    kind = _SERVE_TYPES.get(str(logits.dtype))
+    if kind is None or len(logits.shape) != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError(f"logits: a float tensor [rows, vocab] with contiguous rows is wanted, not {logits.dtype} {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    f32 = "torch.float32"
+    _ok(load().lg_sample(logits.data_ptr(), kind, max(vocab, logits.stride(0)) if rows < 2 else logits.stride(0), rows, vocab,
+                         _array(temperature, f32, rows, "temperature"), _array(top_k, "torch.int32", rows, "top_k"), _array(top_p, f32, rows, "top_p"),
+                         _array(min_p, f32, rows, "min_p"), _array(u, f32, rows, "u"), _array(token, "torch.int32", rows, "token"),
+                         _array(prob, f32, rows, "prob"), stream), "sample")
+
+
 class Session:
     """One loaded target model (+ optional draft head) with its KV cache on the GPU.
 
@@ -352,6 +486,12 @@ class Session:
 
     def next(self, tok: int, pos: int) -> int:
         return self.L.lgs_next(self.h, tok, pos)
+
+    def next_sampled(self, tok: int, pos: int, u: float, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
+        """One forward and a token drawn from its logits on the device (see sample()): (token, its probability)."""
+        prob = C.c_float()
+        tok = self.L.lg_forward_sample(self.model, self.kv, tok, pos, temperature, top_k, top_p, min_p, u, C.byref(prob))
+        return tok, prob.value
 
     def prefill(self, toks, pos0: int = 0):
         toks = np.ascontiguousarray(toks, dtype=np.int32)

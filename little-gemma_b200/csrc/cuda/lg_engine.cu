@@ -899,6 +899,7 @@ void engine_free(Engine *e) {
     cudaFreeHost(e->host_out);
     cudaFree(e->st); cudaFreeHost(e->st_host); cudaFree(e->log); cudaFree(e->replay); cudaFree(e->d_n_replay); cudaFree(e->err); cudaFree(e->tickets); cudaFree(e->d_margin_thr);
     free(e->pick_rows);
+    cudaFree(e->draw); cudaFreeHost(e->draw_host);
     cudaStreamDestroy(e->stream);
     delete e;
 }
@@ -1636,6 +1637,17 @@ cudaGraphExec_t round_graph(Engine *e, const struct kvcache *kv, DraftW *d, int 
 int g_round_width = LG_MTP_N;                 // verify width the blocking calls' whole-round path assumes (lg_set_round_width)
 
 }  // namespace
+
+// The forward of model_forward_next with its logits kept; whoever draws from them is next on the engine's stream.
+const float *lg::forward_device_logits(struct model *m, struct kvcache *kv, int token, int pos, Engine **engine) {
+    Engine *e = engine_for(m);
+    e->lazy.valid = false;
+    if (!pos_in_cache(kv, pos, 1, "a forward") || !can_start(e, kv, pos, 1, false, "a forward")) exit(1);
+    upload_round(e, &token, 1, pos);
+    run_forward(e, kv, 1, F_HEAD | F_LOGITS | F_ACCEPT);
+    *engine = e;
+    return e->logits;
+}
 
 // ==========================================================================================
 // exported backend symbols

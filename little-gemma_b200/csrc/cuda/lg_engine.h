@@ -145,6 +145,7 @@ struct Engine {
     const struct kvcache *kv_bound = nullptr;
     DraftW *draft = nullptr; const struct mtp *draft_owner = nullptr;
     float *pick_rows = nullptr;               // host logits rows for model_pick
+    float *draw = nullptr, *draw_host = nullptr;   // lg_forward_sample: one row's parameters, token and probability; its pinned mirror
     long long launches = 0;                   // kernels enqueued by the most recent graph build
     int pdl = 1;                              // programmatic dependent launch (LG_PDL=0 turns it off)
     bool hold_next = false;                   // the next launch starts only when its predecessor has ended (behind an import)
@@ -269,6 +270,8 @@ inline CUtensorMap tile_boxes_map(const void *ptr, int bytes, int positions, int
     return map;
 }
 
+// One forward of `token` at pos whose logits stay on the device (a row of n_vocab floats, valid on the engine's stream).
+const float *forward_device_logits(struct model *m, struct kvcache *kv, int token, int pos, Engine **engine);
 void check_err(Engine *e);                    // waits for the stream; ends the process when a kernel raised the status word
 
 }  // namespace lg

@@ -1,0 +1,216 @@
+// lg_serve.cu -- operators of a decode step of many requests (include/lg_serve.h): the entry points, their checks and launches.
+// Kernels: lg_paged.cuh (block tables and slots, append, attention of a paged cache), lg_sample.cuh.
+#include "lg_engine.h"
+#include "lg_serve.h"
+#include "lg_paged.cuh"
+#include "lg_sample.cuh"
+
+using namespace lg;
+
+namespace {
+
+#define SERVE_FAIL(code, ...) do { fprintf(stderr, __VA_ARGS__); fputc('\n', stderr); return (code); } while (0)
+
+enum { TY_F32 = 0, TY_F16 = 1, TY_BF16 = 30 };
+bool known_type(int t) { return t == TY_F32 || t == TY_F16 || t == TY_BF16; }
+int type_bytes(int t) { return t == TY_F32 ? 4 : 2; }
+
+// The device of a call: where its memory lies.  Made current for the call, the caller's is put back.
+struct OnDevice {
+    int dev = -1, prev = -1;
+    bool ok = true;
+    // p is device memory on the same device as the pointers before it
+    void add(const void *p) {
+        cudaPointerAttributes at;
+        if (!ok) return;
+        if (cudaPointerGetAttributes(&at, p) != cudaSuccess) { cudaGetLastError(); ok = false; return; }
+        if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) ok = false;
+        else if (dev < 0) dev = at.device;
+        else if (dev != at.device) ok = false;
+    }
+    void add_opt(const void *p) { if (p) add(p); }
+    bool enter() {
+        if (!ok || cudaGetDevice(&prev) != cudaSuccess) return false;
+        if (prev == dev) { prev = -1; return true; }
+        if (cudaSetDevice(dev) == cudaSuccess) return true;
+        cudaGetLastError();
+        prev = -1;
+        return false;
+    }
+    ~OnDevice() { if (prev >= 0) cudaSetDevice(prev); }
+};
+
+template <typename... KArgs> int launch_serve(const char *who, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, void *stream, KArgs... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = (cudaStream_t)stream;
+    const cudaError_t rc = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (rc != cudaSuccess) { cudaGetLastError(); SERVE_FAIL(-6, "%s: launch failed: %s", who, cudaGetErrorString(rc)); }
+    return 0;
+}
+// Dynamic shared memory above 48 KB, up to `most`: once per device and kernel
+template <typename K> bool allow_smem(K *kernel, size_t bytes, size_t most, int dev, unsigned char *done) {
+    if (bytes <= 48 * 1024 || (dev < 64 && done[dev])) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) { cudaGetLastError(); return false; }
+    if (dev < 64) done[dev] = 1;
+    return true;
+}
+
+// NULL where the description of a cache is good, else what is wrong with it
+const char *cache_fault(const struct lg_paged_cache *c) {
+    if (!c || !c->k || !c->v || !c->table || !c->len) return "a NULL pointer in the cache";
+    if (!known_type(c->type)) return "the cache's type is not f32, f16 or bf16";
+    if (c->n_pages < 1 || c->page_size < 1 || c->n_kv_heads < 1 || c->max_req < 1 || c->max_pages < 1 || c->table_stride < c->max_pages)
+        return "a size of the cache out of range";
+    if (c->head_dim < 8 || c->head_dim > 512 || c->head_dim % 8) return "head_dim is not a multiple of 8 up to 512";
+    if ((long long)c->n_pages * c->page_size > 0x7fffffffLL) return "more slots than 2^31 - 1";
+    if ((long long)c->max_pages * c->page_size > 0x7fffffffLL - LG_PAGED_MAX_REQ) return "more rows in a request than fit an int";
+    if (c->page_stride < 0 || c->row_stride < 0 || c->head_stride < 0 || (c->page_stride | c->row_stride | c->head_stride) % 8)
+        return "a stride is negative or not a multiple of 8";
+    if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return "k and v must be 16-byte aligned";
+    if (((uintptr_t)c->table | (uintptr_t)c->len | (uintptr_t)c->free_pages | (uintptr_t)c->n_free | (uintptr_t)c->status) & 3)
+        return "table, len and the stack must be 4-byte aligned";
+    return nullptr;
+}
+LgPaged paged_of(const struct lg_paged_cache *c) {
+    LgPaged p;
+    p.k = c->k; p.v = c->v; p.page_stride = c->page_stride; p.row_stride = c->row_stride; p.head_stride = c->head_stride;
+    p.n_pages = c->n_pages; p.page_size = c->page_size; p.n_kv = c->n_kv_heads; p.hd = c->head_dim;
+    p.max_pages = c->max_pages; p.table_stride = c->table_stride;
+    p.table = c->table; p.len = c->len; p.free_pages = c->free_pages; p.n_free = c->n_free; p.status = c->status;
+    return p;
+}
+void add_cache(OnDevice &on, const struct lg_paged_cache *c) {
+    on.add(c->k); on.add(c->v); on.add(c->table); on.add(c->len);
+    on.add_opt(c->status);
+}
+
+}  // namespace
+
+extern "C" int lg_paged_step(const struct lg_paged_cache *c, int n_req, const int *d_keep, const int *d_new, int cap, int *d_start, int *d_pos,
+                             int *d_slot, int *d_req, void *stream) {
+    if (const char *f = cache_fault(c)) SERVE_FAIL(-1, "lg_paged_step: %s", f);
+    if (!c->free_pages || !c->n_free) SERVE_FAIL(-1, "lg_paged_step: the cache has no stack of free pages");
+    if (n_req < 1 || n_req > c->max_req || cap < 0 || !d_new || !d_start) SERVE_FAIL(-1, "lg_paged_step: bad arguments");
+    if (n_req > LG_PAGED_MAX_REQ) SERVE_FAIL(-2, "lg_paged_step: %d requests, at most %d", n_req, LG_PAGED_MAX_REQ);
+    if (((uintptr_t)d_keep | (uintptr_t)d_new | (uintptr_t)d_start | (uintptr_t)d_pos | (uintptr_t)d_slot | (uintptr_t)d_req) & 3)
+        SERVE_FAIL(-1, "lg_paged_step: arrays must be 4-byte aligned");
+    OnDevice on;
+    add_cache(on, c);
+    on.add(c->free_pages); on.add(c->n_free); on.add(d_new); on.add(d_start);
+    on.add_opt(d_keep); on.add_opt(d_pos); on.add_opt(d_slot); on.add_opt(d_req);
+    if (!on.enter()) SERVE_FAIL(-1, "lg_paged_step: pointers are not memory of one device");
+    LgStepArgs a;
+    a.c = paged_of(c); a.n_req = n_req; a.cap = cap; a.keep = d_keep; a.fresh = d_new;
+    a.start = d_start; a.pos = d_pos; a.slot = d_slot; a.req = d_req;
+    const size_t smem = 3 * ((size_t)n_req + 1) * sizeof(int), most = 3 * ((size_t)LG_PAGED_MAX_REQ + 1) * sizeof(int);
+    static unsigned char done[64];
+    if (!allow_smem(lg_paged_step_kernel, smem, most, on.dev, done)) SERVE_FAIL(-6, "lg_paged_step: no %zu bytes of shared memory", smem);
+    return launch_serve("lg_paged_step", lg_paged_step_kernel, dim3(1), dim3(LG_STEP_THREADS), smem, stream, a);
+}
+
+extern "C" int lg_paged_append(const struct lg_paged_cache *c, const void *d_k, const void *d_v, int type, long long ld_k, long long ld_v, int n,
+                               const int *d_slot, void *stream) {
+    if (const char *f = cache_fault(c)) SERVE_FAIL(-1, "lg_paged_append: %s", f);
+    const long long width = (long long)c->n_kv_heads * c->head_dim;
+    if (n == 0) return 0;
+    if (n < 0 || !d_k || !d_v || !d_slot || ld_k < width || ld_v < width) SERVE_FAIL(-1, "lg_paged_append: bad arguments");
+    if (type != TY_F32 && type != c->type) SERVE_FAIL(-1, "lg_paged_append: rows are f32 or of the cache's type");
+    const int eb = type_bytes(type);
+    if (((uintptr_t)d_k | (uintptr_t)d_v) % eb || (uintptr_t)d_slot & 3) SERVE_FAIL(-1, "lg_paged_append: a pointer into the middle of an element");
+    OnDevice on;
+    add_cache(on, c);
+    on.add(d_k); on.add(d_v); on.add(d_slot);
+    if (!on.enter()) SERVE_FAIL(-1, "lg_paged_append: pointers are not memory of one device");
+    LgAppendArgs a;
+    a.c = paged_of(c); a.k = d_k; a.v = d_v; a.ld_k = ld_k; a.ld_v = ld_v; a.n = n; a.slot = d_slot;
+    a.wide = !(((uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)(ld_k * eb) | (uintptr_t)(ld_v * eb)) & 15);
+    const long long blocks = ((long long)n * width / 4 + 255) / 256;
+    const dim3 grid((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8));
+    void (*kernel)(LgAppendArgs) = nullptr;
+    if (c->type == TY_F32) kernel = lg_paged_append_kernel<float, float>;
+    else if (c->type == TY_F16) kernel = type == TY_F32 ? lg_paged_append_kernel<float, __half> : lg_paged_append_kernel<__half, __half>;
+    else kernel = type == TY_F32 ? lg_paged_append_kernel<float, __nv_bfloat16> : lg_paged_append_kernel<__nv_bfloat16, __nv_bfloat16>;
+    return launch_serve("lg_paged_append", kernel, grid, dim3(256), 0, stream, a);
+}
+
+extern "C" long long lg_paged_attn_work(const struct lg_paged_cache *c, int n_req, int n_new, int n_heads) {
+    if (const char *f = cache_fault(c)) SERVE_FAIL(-1, "lg_paged_attn_work: %s", f);
+    if (n_req < 1 || n_req > c->max_req || n_new < 1 || n_new > LG_PAGED_MAX_NEW || n_heads < 1 || n_heads % c->n_kv_heads)
+        SERVE_FAIL(-1, "lg_paged_attn_work: bad arguments");
+    return 16;
+}
+
+extern "C" int lg_paged_attn(const struct lg_paged_cache *c, const void *d_q, int type, long long ld_q, int n_req, int n_new, int n_rows,
+                             const int *d_start, int n_heads, float scale, int window, void *d_out, long long ld_out, void *d_work,
+                             long long work_bytes, void *stream) {
+    if (const char *f = cache_fault(c)) SERVE_FAIL(-1, "lg_paged_attn: %s", f);
+    if (n_rows == 0 && d_start) return 0;
+    if (n_req < 1 || n_req > c->max_req || n_new < 1 || n_new > LG_PAGED_MAX_NEW || n_heads < 1 || n_heads % c->n_kv_heads || n_rows < 0 ||
+        !d_q || !d_out || !d_work || window < 0 || !(scale >= 0.0f) || isinf(scale))
+        SERVE_FAIL(-1, "lg_paged_attn: bad arguments");
+    if (!d_start && (long long)n_req * n_new != n_rows) SERVE_FAIL(-1, "lg_paged_attn: %d rows for %d requests of %d tokens", n_rows, n_req, n_new);
+    if (type != TY_F32 && type != c->type) SERVE_FAIL(-1, "lg_paged_attn: q and out are f32 or of the cache's type");
+    const long long width = (long long)n_heads * c->head_dim;
+    if (ld_q < width || ld_out < width) SERVE_FAIL(-1, "lg_paged_attn: rows overlap");
+    const int eb = type_bytes(type);
+    if (((uintptr_t)d_q | (uintptr_t)d_out) % eb || (uintptr_t)d_start & 3 || (uintptr_t)d_work & 15)
+        SERVE_FAIL(-1, "lg_paged_attn: a misaligned pointer");
+    if (n_heads > 65535 || n_req > 65535) SERVE_FAIL(-2, "lg_paged_attn: %d requests of %d heads", n_req, n_heads);
+    const long long need = lg_paged_attn_work(c, n_req, n_new, n_heads);
+    if (work_bytes < need) SERVE_FAIL(-3, "lg_paged_attn: a workspace of %lld bytes, %lld are needed", work_bytes, need);
+    OnDevice on;
+    add_cache(on, c);
+    on.add(d_q); on.add(d_out); on.add(d_work); on.add_opt(d_start);
+    if (!on.enter()) SERVE_FAIL(-1, "lg_paged_attn: pointers are not memory of one device");
+    LgPagedAttnArgs a;
+    a.c = paged_of(c); a.q = d_q; a.out = d_out; a.ld_q = ld_q; a.ld_out = ld_out; a.n_req = n_req; a.n_new = n_new; a.n_rows = n_rows;
+    a.n_heads = n_heads; a.window = window; a.start = d_start;
+    a.scale = (scale > 0.0f ? scale : 1.0f / sqrtf((float)c->head_dim)) * LG_LOG2E;
+    void (*kernel)(LgPagedAttnArgs) = nullptr;
+    if (c->type == TY_F32) kernel = lg_paged_attn_rows_kernel<float, float>;
+    else if (c->type == TY_F16) kernel = type == TY_F32 ? lg_paged_attn_rows_kernel<float, __half> : lg_paged_attn_rows_kernel<__half, __half>;
+    else kernel = type == TY_F32 ? lg_paged_attn_rows_kernel<float, __nv_bfloat16> : lg_paged_attn_rows_kernel<__nv_bfloat16, __nv_bfloat16>;
+    return launch_serve("lg_paged_attn", kernel, dim3(n_new, n_heads, n_req), dim3(LG_PATTN_WARPS * 32), 0, stream, a);
+}
+
+extern "C" int lg_sample(const void *d_logits, int type, long long ld, int rows, int vocab, const float *d_temperature, const int *d_top_k,
+                         const float *d_top_p, const float *d_min_p, const float *d_u, int *d_token, float *d_prob, void *stream) {
+    if (rows == 0) return 0;
+    if (!d_logits || !d_u || !d_token || rows < 0 || vocab < 1 || ld < vocab || !known_type(type)) SERVE_FAIL(-1, "lg_sample: bad arguments");
+    if (vocab > 1 << 20) SERVE_FAIL(-2, "lg_sample: a vocabulary of %d, at most %d", vocab, 1 << 20);
+    if ((uintptr_t)d_logits % type_bytes(type) ||
+        ((uintptr_t)d_temperature | (uintptr_t)d_top_k | (uintptr_t)d_top_p | (uintptr_t)d_min_p | (uintptr_t)d_u | (uintptr_t)d_token | (uintptr_t)d_prob) & 3)
+        SERVE_FAIL(-1, "lg_sample: a pointer into the middle of an element");
+    OnDevice on;
+    on.add(d_logits); on.add(d_u); on.add(d_token);
+    on.add_opt(d_temperature); on.add_opt(d_top_k); on.add_opt(d_top_p); on.add_opt(d_min_p); on.add_opt(d_prob);
+    if (!on.enter()) SERVE_FAIL(-1, "lg_sample: pointers are not memory of one device");
+    LgSampleArgs a;
+    a.logits = d_logits; a.ld = ld; a.vocab = vocab;
+    int bits = 0;
+    while ((1 << bits) < vocab) bits++;
+    a.shift = 62 - bits;
+    a.temperature = d_temperature; a.top_k = d_top_k; a.top_p = d_top_p; a.min_p = d_min_p; a.u = d_u; a.token = d_token; a.prob = d_prob;
+    void (*kernel)(LgSampleArgs) = type == TY_F32 ? lg_sample_kernel<float> : type == TY_F16 ? lg_sample_kernel<__half> : lg_sample_kernel<__nv_bfloat16>;
+    return launch_serve("lg_sample", kernel, dim3(rows), dim3(LG_SAMPLE_THREADS), 0, stream, a);
+}
+
+// The parameters of the one row go to the device beside its forward; the token and its probability return behind it.
+extern "C" int lg_forward_sample(struct model *m, struct kvcache *kv, int token, int pos, float temperature, int top_k, float top_p, float min_p,
+                                 float u, float *prob) {
+    Engine *e = nullptr;
+    const float *logits = forward_device_logits(m, kv, token, pos, &e);
+    struct Words { float temperature; int top_k; float top_p, min_p, u; int token; float prob; };
+    if (!e->draw) e->draw = dalloc<float>(sizeof(Words) / 4);
+    if (!e->draw_host) LG_CHECK(cudaMallocHost(&e->draw_host, sizeof(Words)));
+    Words *d = (Words *)e->draw, *h = (Words *)e->draw_host;
+    *h = Words{temperature, top_k, top_p, min_p, u, -1, 0.0f};
+    LG_CHECK(cudaMemcpyAsync(d, h, sizeof(Words), cudaMemcpyHostToDevice, e->stream));
+    const int n_vocab = m->cfg.n_vocab;
+    if (lg_sample(logits, TY_F32, n_vocab, 1, n_vocab, &d->temperature, &d->top_k, &d->top_p, &d->min_p, &d->u, &d->token, &d->prob, e->stream)) exit(1);
+    LG_CHECK(cudaMemcpyAsync(&h->token, &d->token, 8, cudaMemcpyDeviceToHost, e->stream));
+    check_err(e);
+    e->host_syncs++;
+    if (prob) *prob = h->prob;
+    return h->token;
+}

@@ -3,6 +3,7 @@
 #pragma once
 #include "lg_device.cuh"
 #include <cuda_bf16.h>
+#include <type_traits>
 #include "lg_serve.h"
 
 struct LgPaged {                       // struct lg_paged_cache as the kernels need it
@@ -254,6 +255,8 @@ struct LgPagedAttnArgs {
     int n_req, n_new, n_rows, n_heads, window;
     float scale;                       // times log2(e)
     const int *start;
+    int gqa, group_rows, max_spans;    // query heads of a KV head, query rows of an item, spans of a request at most
+    float *part; float2 *part_ml;      // [request][token][head][span]: unnormalised output; maximum and sum
 };
 
 // The block of rows of request r: first row, rows to compute, rows it has.
@@ -334,5 +337,494 @@ template <typename TQ, typename TC> __global__ void __launch_bounds__(LG_PATTN_W
         #pragma unroll
         for (int w = 0; w < LG_PATTN_WARPS; w++) y += po[w][d] * f[w];
         out[d] = Elem<TQ>::put(sum == 0.0f ? 0.0f : y / sum);
+    }
+}
+
+// ---- 16-bit caches: tensor-core tiles, spans over the length, a merge ----------------------------
+// The work is cut into items: (request, KV head, group of 8 NT query rows, span of keys).  A request's spans depend on its own length and on the
+// number of heads alone, never on the other requests, so neither do its sums.  A persistent grid walks the items in that order, each CTA a
+// stretch of about equal key counts; one with several spans leaves (max, sum, unnormalised output) per span for lg_paged_merge_kernel.
+//
+// Inside a CTA every warp works alone: it takes 16 keys (a slice) at a time, brings K and V in with 16-byte asynchronous copies through a ring
+// of U units of its own (a unit: 16 rows of K or of V; rows that no query may see are filled with zeros and never read), so the loop has no block barrier and
+// runs ahead across items.  Both products have the keys / head dims on the 16-row side and 8 queries as columns:
+//   S^T (16 keys x 8) = K Q^T, softmax with a running maximum per column in the accumulator's own lanes, O^T (16 dims x 8) += V^T P^T,
+// P^T turned from accumulator order into operand order by movmatrix.  Numerics: an f32 query enters as a sum of 16-bit parts (f16: 2 parts behind a
+// power of two per row, 22 bits; bf16: 3, 24 bits), P as 2 parts (3 where the answer is f32 and the cache bf16); P carries a factor 2^15 in f16 so that
+// weights down to 2^-29 of the largest stay normal numbers.  Everything else is f32.
+#define LG_PA_TARGET 148               // items that a request of one KV head is cut into at most: the device's SMs
+#define LG_PA_MIN_SLICES 8             // of a span
+
+template <typename T> __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma_16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { mma_f16(c, a, b0, b1); }
+template <> __device__ __forceinline__ void mma_16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two numbers rounded and packed, the first in the low half; x and y keep what the rounding left over.
+template <typename T> __device__ __forceinline__ uint32_t split2(float &x, float &y);
+template <> __device__ __forceinline__ uint32_t split2<__half>(float &x, float &y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    x -= f.x; y -= f.y;
+    return *(const uint32_t *)&h;
+}
+template <> __device__ __forceinline__ uint32_t split2<__nv_bfloat16>(float &x, float &y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const uint32_t w = *(const uint32_t *)&h;
+    x -= __uint_as_float(w << 16); y -= __uint_as_float(w & 0xFFFF0000u);
+    return w;
+}
+__device__ __forceinline__ uint32_t movm(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+// 16 bytes from global memory, or 16 zero bytes without a read
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool read) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
+// A request as the walk over items sees it.
+struct LgReq {
+    int first, m, held, len;           // rows, see paged_rows
+    int groups;                        // of query rows, per KV head
+    int s0, n_sl, ss, spans;           // first slice, slices, slices per span, spans
+};
+__device__ __forceinline__ LgReq paged_request(const LgPagedAttnArgs &a, int r) {
+    LgReq q;
+    paged_rows(a, r, q.first, q.m, q.held);
+    q.len = paged_len(a, r);
+    q.groups = (q.m * a.gqa + a.group_rows - 1) / a.group_rows;
+    // keys lo .. hi-1 are seen by some row
+    const int hi = max(0, q.len - q.held + q.m), lo = a.window > 0 ? max(0, q.len - q.held - a.window + 1) : 0;
+    q.s0 = min(lo, hi) >> 4;
+    q.n_sl = ((hi + 15) >> 4) - q.s0;
+    q.ss = max(LG_PA_MIN_SLICES, (q.n_sl + a.max_spans - 1) / a.max_spans);
+    q.ss = (q.ss + 3) & ~3;
+    q.spans = max(1, (q.n_sl + q.ss - 1) / q.ss);
+    return q;
+}
+// Weight of a request in the walk: slices of all its items, at least one each (an item without keys writes zeros)
+__device__ __forceinline__ long long paged_weight(const LgPagedAttnArgs &a, const LgReq &q) { return (long long)max(1, q.n_sl) * q.groups * a.c.n_kv; }
+
+// The walk of one CTA: items whose offset in the order of slices is below `end`.
+struct LgWalk {
+    LgReq q;
+    int r, hg, span;                   // request, KV head * groups + group, span
+    long long at, end;                 // offset of the request's current (head, group), end of the CTA's stretch
+    __device__ __forceinline__ bool valid(const LgPagedAttnArgs &a) const { return r < a.n_req && at + (long long)span * q.ss < end; }
+    __device__ __forceinline__ void settle(const LgPagedAttnArgs &a) {        // past requests without rows
+        while (r < a.n_req && hg >= q.groups * a.c.n_kv) {
+            if (++r < a.n_req && at < end) { q = paged_request(a, r); hg = 0; span = 0; }
+            else if (r < a.n_req) r = a.n_req;
+        }
+    }
+    __device__ __forceinline__ void next(const LgPagedAttnArgs &a) {
+        if (++span < q.spans) return;
+        span = 0;
+        at += max(1, q.n_sl);
+        hg++;
+        settle(a);
+    }
+};
+
+template <typename TQ, typename TC, int HD, int NT> struct LgPagedTile {
+    static constexpr bool SAME = sizeof(TQ) == 2;
+    static constexpr bool F16 = std::is_same<TC, __half>::value;
+    static constexpr int NQ = SAME ? 1 : F16 ? 2 : 3;                         // parts of a query
+    static constexpr int NP = SAME || F16 ? 2 : 3;                            // parts of a weight
+    static constexpr int KS = HD / 16;
+    static constexpr int ROWS = 8 * NT;
+    static constexpr int UNIT = 16 * HD * 2;
+    static constexpr int LDB = HD + 4;                                        // floats from row to row of the merge buffer: no bank conflicts
+    static constexpr bool QREG = (NT * NQ * 2 + NT * 4) * KS <= 160;          // queries stay in registers beside the outputs
+    static constexpr int Q_BYTES = NT * NQ * KS * 32 * 8, BUF_BYTES = ROWS * LDB * 4;
+    static constexpr int SHARED = QREG ? (Q_BYTES > BUF_BYTES ? Q_BYTES : BUF_BYTES) : Q_BYTES + BUF_BYTES;   // in registers they need the room only on the way
+    static constexpr int fixed(int w) { return SHARED + 2 * w * ROWS * 8 + ROWS * 4 + 128 + w * 16 * 4; }
+    // Two CTAs of 4 warps per SM where three units a warp fit (one merges while the other streams), else one of as many warps as fit
+    static constexpr int CTAS = fixed(4) + 12 * UNIT <= 115712 ? 2 : 1;
+    static constexpr int ROOM = CTAS == 2 ? 115712 : 232448;
+    static constexpr int W = CTAS == 2 ? 4 : fixed(8) + 24 * UNIT <= ROOM ? 8 : fixed(6) + 18 * UNIT <= ROOM ? 6 : fixed(4) + 12 * UNIT <= ROOM ? 4 : 3;
+    static constexpr int U0 = (ROOM - fixed(W)) / (W * UNIT);
+    static constexpr int U = U0 > 8 ? 8 : U0;
+    static constexpr int SMEM = fixed(W) + W * U * UNIT;
+    static_assert(U >= 3, "a ring of three units at least");
+};
+
+template <typename TQ, typename TC, int HD, int NT>
+__global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPagedTile<TQ, TC, HD, NT>::CTAS)) lg_paged_attn_kernel(LgPagedAttnArgs a) {
+    typedef LgPagedTile<TQ, TC, HD, NT> P;
+    extern __shared__ __align__(128) unsigned char lg_pa_sm[];
+    unsigned char *ring = lg_pa_sm;
+    uint32_t *sq = (uint32_t *)(lg_pa_sm + P::W * P::U * P::UNIT);           // [nt][part][ks][lane][2]
+    float *buf = P::QREG ? (float *)sq : (float *)((unsigned char *)sq + P::Q_BYTES);      // [row][LDB]
+    float2 *stats = (float2 *)((unsigned char *)sq + P::SHARED);              // [2][warp][row]: max, sum; items take turns
+    float *cscale = (float *)(stats + 2 * P::W * P::ROWS);                  // [row]: scale of the scores
+    long long *red = (long long *)(cscale + P::ROWS);                         // 16 words
+    uint32_t *vmask = (uint32_t *)(red + 16);                                  // [warp][16]: keys of a slice that are there
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    pdl_launch();
+
+    // this CTA's stretch: weights of all requests, thread by thread, and where the stretch begins
+    LgWalk w;
+    {
+        const int per = (a.n_req + P::W * 32 - 1) / (P::W * 32), r0 = min(a.n_req, tid * per), r1 = min(a.n_req, r0 + per);
+        long long mine = 0;
+        for (int r = r0; r < r1; r++) mine += paged_weight(a, paged_request(a, r));
+        long long s = mine;
+        #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += x; }
+        if (lane == 31) red[warp] = s;
+        if (tid == 0) red[8] = a.n_req;
+        __syncthreads();
+        long long before = 0, total = 0;
+        #pragma unroll
+        for (int i = 0; i < P::W; i++) { if (i < warp) before += red[i]; total += red[i]; }
+        before += s - mine;
+        const long long lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
+        if (mine && before <= lo && lo < before + mine) {
+            int r = r0;
+            for (;; r++) {
+                const long long x = paged_weight(a, paged_request(a, r));
+                if (lo < before + x) break;
+                before += x;
+            }
+            red[8] = r; red[9] = before;
+        }
+        __syncthreads();
+        w.r = (int)red[8]; w.end = hi;
+        if (w.r >= a.n_req || lo >= hi) return;
+        w.at = red[9];
+        w.q = paged_request(a, w.r);
+        const int n = max(1, w.q.n_sl);
+        const long long rem = lo - w.at;
+        w.hg = (int)(rem / n);
+        w.at += (long long)w.hg * n;
+        w.span = ((int)(rem - (long long)w.hg * n) + w.q.ss - 1) / w.q.ss;    // the first item that begins in the stretch
+        if (w.span >= w.q.spans) { w.span = w.q.spans - 1; w.next(a); }
+    }
+    // the copies run ahead of the arithmetic with a walk of their own
+    LgWalk p = w;
+    int ps = 0, ps_end = 0, n_issued = 0, slot_in = 0, page = -1;             // next slice of this warp, end of the item's slices
+    long long poff = 0;
+    bool pread = false;
+    const int ps_size = a.c.page_size, hd8 = a.c.hd >> 3;
+    auto begin_item = [&]() {                                                 // first slice of this warp in walk p's item, or the next item that has one
+        while (p.valid(a)) {
+            ps = p.q.s0 + p.span * p.q.ss + warp;
+            ps_end = p.q.s0 + min(p.q.n_sl, (p.span + 1) * p.q.ss);
+            if (ps < ps_end) return true;
+            p.next(a);
+        }
+        return false;
+    };
+    bool more = begin_item();
+    auto fetch_page = [&]() {                                                 // page of this lane's row in slice ps (lanes 16..31: the same rows)
+        page = -1;
+        const int key = ps * 16 + (lane & 15);
+        const int hi = p.q.len - p.q.held + p.q.m, lo = a.window > 0 ? p.q.len - p.q.held - a.window + 1 : 0;
+        if (key < hi && key >= lo) {
+            page = a.c.table[(size_t)p.r * a.c.table_stride + key / ps_size];
+            if (page < 0 || page >= a.c.n_pages) { paged_raise(a.c, LG_PAGED_BAD_PAGE); page = -1; }
+        }
+    };
+    if (more) fetch_page();
+    const uint32_t ring_u32 = smem_u32(ring) + warp * (P::U * P::UNIT);
+    auto issue = [&]() {                                                      // one unit: K of a slice, then its V
+        if (more) {
+            const bool is_v = n_issued & 1;
+            if (!is_v) {
+                const int key = ps * 16 + (lane & 15);
+                pread = page >= 0;
+                poff = pread ? ((long long)page * a.c.page_stride + (long long)(key - key / ps_size * ps_size) * a.c.row_stride + (long long)(p.hg / p.q.groups) * a.c.head_stride) * 2 : 0;
+                const uint32_t ok = __ballot_sync(0xffffffffu, pread) & 0xFFFFu;
+                if (lane == 0) vmask[warp * 16 + ((n_issued >> 1) & 15)] = ok;
+            }
+            const unsigned char *base = (const unsigned char *)(is_v ? a.c.v : a.c.k);
+            const uint32_t dst = ring_u32 + slot_in * P::UNIT;
+            #pragma unroll
+            for (int i = 0; i < HD / 16; i++) {                               // 32 chunks of 16 bytes at a time
+                const int idx = i * 32 + lane, row = idx / (HD / 8), c = idx % (HD / 8);
+                const long long off = __shfl_sync(0xffffffffu, poff, row);
+                const bool rd = __shfl_sync(0xffffffffu, (int)pread, row) && c < hd8;
+                cp_async16_or_zero(dst + row * (HD * 2) + ((c ^ (row & 7)) << 4), rd ? base + off + c * 16 : base, rd);
+            }
+            if (is_v) {
+                ps += P::W;
+                if (ps >= ps_end) { p.next(a); more = begin_item(); }
+                if (more) fetch_page();
+            }
+            n_issued++;
+            if (++slot_in == P::U) slot_in = 0;
+        }
+        cp_async_commit();
+    };
+    #pragma unroll
+    for (int i = 0; i < P::U - 1; i++) issue();
+
+    int slot = 0, n_used = 0, q_r = -1, q_hg = -1, turn = 0;
+    uint32_t qr[P::QREG ? NT * P::NQ * P::KS * 2 : 1];
+    for (; w.valid(a); w.next(a), turn ^= 1) {
+        float2 *stat = stats + turn * P::W * P::ROWS;
+        const int kvh = w.hg / w.q.groups, row0 = (w.hg - kvh * w.q.groups) * P::ROWS;      // first of the group's rows: row = token * gqa + head of the group
+        const int n_rows = min(P::ROWS, w.q.m * a.gqa - row0);
+        if (q_r != w.r || q_hg != w.hg) {                                     // queries of the group into operand order
+            q_r = w.r; q_hg = w.hg;
+            if (P::QREG) __syncthreads();                                     // the merge buffer lies there
+            for (int n = warp; n < P::ROWS; n += P::W) {
+                const int rho = row0 + n, t = rho / a.gqa;
+                const TQ *src = (const TQ *)a.q + (long long)(w.q.first + t) * a.ld_q + (long long)(kvh * a.gqa + rho - t * a.gqa) * a.c.hd;
+                float x[HD / 32];
+                #pragma unroll
+                for (int i = 0; i < HD / 64; i++) {
+                    const int d = 64 * i + 2 * lane;
+                    x[2 * i] = n < n_rows && d < a.c.hd ? Elem<TQ>::get(src + d) : 0.0f;
+                    x[2 * i + 1] = n < n_rows && d < a.c.hd ? Elem<TQ>::get(src + d + 1) : 0.0f;
+                }
+                float back = a.scale;
+                if (P::NQ == 2) {                                             // a power of two that takes the row's largest element to 2^14 .. 2^15
+                    float top = 0.0f;
+                    #pragma unroll
+                    for (int i = 0; i < HD / 32; i++) top = fmaxf(top, fabsf(x[i]));
+                    top = warp_max(top);
+                    if (top > 0.0f && top < INFINITY) {
+                        int e;
+                        frexpf(top, &e);
+                        const int up = 15 - e;
+                        #pragma unroll
+                        for (int i = 0; i < HD / 32; i++) x[i] = ldexpf(x[i], up);
+                        back = ldexpf(back, -up);
+                    }
+                }
+                #pragma unroll
+                for (int i = 0; i < HD / 64; i++) {
+                    const int d = 64 * i + 2 * lane, ks = d >> 4, half = (d >> 3) & 1, t = (d & 7) >> 1;
+                    #pragma unroll
+                    for (int part = 0; part < P::NQ; part++)
+                        sq[((((n >> 3) * P::NQ + part) * P::KS + ks) * 32 + (n & 7) * 4 + t) * 2 + half] = split2<TC>(x[2 * i], x[2 * i + 1]);
+                }
+                if (lane == 0) cscale[n] = back;
+            }
+            __syncthreads();
+            if (P::QREG) {
+                #pragma unroll
+                for (int i = 0; i < NT * P::NQ * P::KS; i++) {
+                    const uint2 v = *(const uint2 *)(sq + (i * 32 + lane) * 2);
+                    qr[2 * i] = v.x; qr[2 * i + 1] = v.y;
+                }
+            }
+        }
+        float cs[NT][2], mx[NT][2], l[NT][2], o[P::KS][NT][4];
+        int top[NT][2];                                                       // position of the column's query
+        const int pos0 = w.q.len - w.q.held;
+        #pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+            #pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int n = nt * 8 + 2 * t4 + j;
+                cs[nt][j] = cscale[n]; mx[nt][j] = -INFINITY; l[nt][j] = 0.0f;
+                top[nt][j] = pos0 + (row0 + min(n, n_rows - 1)) / a.gqa;
+            }
+        #pragma unroll
+        for (int ks = 0; ks < P::KS; ks++)
+            #pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+                #pragma unroll
+                for (int j = 0; j < 4; j++) o[ks][nt][j] = 0.0f;
+        const int pos_lo = pos0 + row0 / a.gqa, pos_hi = pos0 + (row0 + n_rows - 1) / a.gqa;
+        const int s_end = w.q.s0 + min(w.q.n_sl, (w.span + 1) * w.q.ss);
+        for (int s = w.q.s0 + w.span * w.q.ss + warp; s < s_end; s += P::W) {
+            cp_async_wait<P::U - 2>();
+            __syncwarp();
+            issue();
+            const uint32_t ok = vmask[warp * 16 + ((n_used++) & 15)];
+            uint32_t at = ring_u32 + slot * P::UNIT;
+            if (++slot == P::U) slot = 0;
+            float sc[NT][2][4];                                               // two chains of products
+            #pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+                #pragma unroll
+                for (int j = 0; j < 4; j++) sc[nt][0][j] = sc[nt][1][j] = 0.0f;
+            {
+                const int row = (lane & 7) + (lane & 8), c = lane >> 4;
+                #pragma unroll
+                for (int ks = 0; ks < P::KS; ks++) {
+                    uint32_t k4[4];
+                    ldsm_x4_u32(k4, at + row * (HD * 2) + (((2 * ks + c) ^ (row & 7)) << 4));
+                    #pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+                        #pragma unroll
+                        for (int part = 0; part < P::NQ; part++) {
+                            const int i = (nt * P::NQ + part) * P::KS + ks;
+                            if (P::QREG) mma_16<TC>(sc[nt][ks & 1], k4, qr[2 * i], qr[2 * i + 1]);
+                            else {
+                                const uint2 v = *(const uint2 *)(sq + (i * 32 + lane) * 2);
+                                mma_16<TC>(sc[nt][ks & 1], k4, v.x, v.y);
+                            }
+                        }
+                }
+            }
+            const int k0 = s * 16;
+            const bool all = ok == 0xFFFFu && k0 + 15 <= pos_lo && (a.window <= 0 || k0 > pos_hi - a.window);
+            uint32_t pb[NT][P::NP][2];
+            bool moved = false;
+            float f[NT][2];
+            #pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float x[4];
+                #pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    x[j] = (sc[nt][0][j] + sc[nt][1][j]) * cs[nt][j & 1];
+                    if (!all) {
+                        const int key = k0 + g + (j >> 1) * 8, pos = top[nt][j & 1];
+                        if (!(ok >> (g + (j >> 1) * 8) & 1) || key > pos || (a.window > 0 && key <= pos - a.window)) x[j] = -INFINITY;
+                    }
+                }
+                #pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float m2 = fmaxf(x[j], x[j + 2]);
+                    m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, 4));
+                    m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, 8));
+                    m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, 16));
+                    m2 = fmaxf(m2, mx[nt][j]);
+                    const float ref = m2 == -INFINITY ? 0.0f : m2;
+                    f[nt][j] = ex2(mx[nt][j] - ref);
+                    moved |= m2 != mx[nt][j];
+                    mx[nt][j] = m2;
+                    const float up = P::F16 ? 15.0f : 0.0f;
+                    x[j] = ex2(x[j] - ref + up);
+                    x[j + 2] = ex2(x[j + 2] - ref + up);
+                    l[nt][j] = l[nt][j] * f[nt][j] + (x[j] + x[j + 2]);
+                }
+                #pragma unroll
+                for (int part = 0; part < P::NP; part++) {
+                    pb[nt][part][0] = movm(split2<TC>(x[0], x[1]));
+                    pb[nt][part][1] = movm(split2<TC>(x[2], x[3]));
+                }
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+                #pragma unroll
+                for (int ks = 0; ks < P::KS; ks++)
+                    #pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+                        #pragma unroll
+                        for (int j = 0; j < 4; j++) o[ks][nt][j] *= f[nt][j & 1];
+            }
+            cp_async_wait<P::U - 2>();
+            __syncwarp();
+            issue();
+            at = ring_u32 + slot * P::UNIT;
+            if (++slot == P::U) slot = 0;
+            {
+                const int row = (lane & 7) + ((lane >> 4) << 3), c = (lane >> 3) & 1;
+                #pragma unroll
+                for (int ks = 0; ks < P::KS; ks++) {
+                    uint32_t v4[4];
+                    ldsm_x4_t_u32(v4, at + row * (HD * 2) + (((2 * ks + c) ^ (row & 7)) << 4));
+                    #pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+                        #pragma unroll
+                        for (int part = 0; part < P::NP; part++) mma_16<TC>(o[ks][nt], v4, pb[nt][part][0], pb[nt][part][1]);
+                }
+            }
+        }
+        // the warps' results into one, in warp order
+        #pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+            #pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float x = l[nt][j];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (g == 0) stat[warp * P::ROWS + nt * 8 + 2 * t4 + j] = make_float2(mx[nt][j], x);
+            }
+        __syncthreads();
+        float f[NT][2];
+        #pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+            #pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float m2 = -INFINITY;
+                #pragma unroll
+                for (int i = 0; i < P::W; i++) m2 = fmaxf(m2, stat[i * P::ROWS + nt * 8 + 2 * t4 + j].x);
+                f[nt][j] = ex2(mx[nt][j] - (m2 == -INFINITY ? 0.0f : m2));
+            }
+        for (int i = 0; i < P::W; i++) {
+            if (warp == i) {
+                #pragma unroll
+                for (int ks = 0; ks < P::KS; ks++)
+                    #pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+                        #pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            float *e = buf + (nt * 8 + 2 * t4 + (j & 1)) * P::LDB + ks * 16 + g + (j >> 1) * 8;
+                            const float x = o[ks][nt][j] * f[nt][j & 1];
+                            *e = i ? *e + x : x;
+                        }
+            }
+            __syncthreads();
+        }
+        for (int n = warp; n < n_rows; n += P::W) {
+            float m2 = -INFINITY, sum = 0.0f;
+            #pragma unroll
+            for (int i = 0; i < P::W; i++) m2 = fmaxf(m2, stat[i * P::ROWS + n].x);
+            #pragma unroll
+            for (int i = 0; i < P::W; i++) sum += stat[i * P::ROWS + n].y * ex2(stat[i * P::ROWS + n].x - (m2 == -INFINITY ? 0.0f : m2));
+            const int rho = row0 + n, t = rho / a.gqa, h = kvh * a.gqa + rho - t * a.gqa;
+            if (w.q.spans == 1) {
+                TQ *out = (TQ *)a.out + (long long)(w.q.first + t) * a.ld_out + (long long)h * a.c.hd;
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                for (int d = lane; d < a.c.hd; d += 32) out[d] = Elem<TQ>::put(buf[n * P::LDB + d] * inv);
+            } else {
+                const long long prow = (((long long)w.r * a.n_new + t) * a.n_heads + h) * a.max_spans + w.span;
+                for (int d = lane; d < a.c.hd; d += 32) a.part[prow * a.c.hd + d] = buf[n * P::LDB + d];
+                if (lane == 0) a.part_ml[prow] = make_float2(m2, sum);
+            }
+        }
+    }
+}
+
+// A warp per query row and head: the spans' results in their order.  Bound by the reads of the partial results.
+template <typename TQ> __global__ void __launch_bounds__(256) lg_paged_merge_kernel(LgPagedAttnArgs a) {
+    const long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, h = (int)(i % a.n_heads);
+    const long long j = i / a.n_heads;
+    const int t = (int)(j % a.n_new), r = (int)(j / a.n_new);
+    pdl_wait();
+    if (r >= a.n_req) return;
+    const LgReq q = paged_request(a, r);
+    if (t >= q.m || q.spans == 1) return;
+    const long long prow = (((long long)r * a.n_new + t) * a.n_heads + h) * a.max_spans;
+    float top = -INFINITY;
+    for (int s = lane; s < q.spans; s += 32) top = fmaxf(top, a.part_ml[prow + s].x);
+    top = warp_max(top);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float y[16], sum = 0.0f;                                                  // dims lane * 4 .. of every 128
+    #pragma unroll
+    for (int k = 0; k < 16; k++) y[k] = 0.0f;
+    for (int s = 0; s < q.spans; s++) {
+        const float2 ml = a.part_ml[prow + s];
+        const float f = ex2(ml.x - ref);
+        sum += ml.y * f;
+        #pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int d = k * 128 + lane * 4;
+            if (d < a.c.hd) {
+                const float4 v = *(const float4 *)(a.part + (prow + s) * a.c.hd + d);
+                y[4 * k] += v.x * f; y[4 * k + 1] += v.y * f; y[4 * k + 2] += v.z * f; y[4 * k + 3] += v.w * f;
+            }
+        }
+    }
+    TQ *out = (TQ *)a.out + (long long)(q.first + t) * a.ld_out + (long long)h * a.c.hd;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    #pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const int d = (k >> 2) * 128 + lane * 4 + (k & 3);
+        if (d < a.c.hd) out[d] = Elem<TQ>::put(y[k] * inv);
     }
 }

@@ -40,9 +40,14 @@ struct OnDevice {
     ~OnDevice() { if (prev >= 0) cudaSetDevice(prev); }
 };
 
-template <typename... KArgs> int launch_serve(const char *who, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, void *stream, KArgs... args) {
+// early: the kernel may start while the one before it drains (it begins with pdl_wait)
+template <typename... KArgs> int launch_serve(const char *who, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, void *stream, bool early, KArgs... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = early ? 1 : 0;
     const cudaError_t rc = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (rc != cudaSuccess) { cudaGetLastError(); SERVE_FAIL(-6, "%s: launch failed: %s", who, cudaGetErrorString(rc)); }
     return 0;
@@ -105,7 +110,7 @@ extern "C" int lg_paged_step(const struct lg_paged_cache *c, int n_req, const in
     const size_t smem = 3 * ((size_t)n_req + 1) * sizeof(int), most = 3 * ((size_t)LG_PAGED_MAX_REQ + 1) * sizeof(int);
     static unsigned char done[64];
     if (!allow_smem(lg_paged_step_kernel, smem, most, on.dev, done)) SERVE_FAIL(-6, "lg_paged_step: no %zu bytes of shared memory", smem);
-    return launch_serve("lg_paged_step", lg_paged_step_kernel, dim3(1), dim3(LG_STEP_THREADS), smem, stream, a);
+    return launch_serve("lg_paged_step", lg_paged_step_kernel, dim3(1), dim3(LG_STEP_THREADS), smem, stream, false, a);
 }
 
 extern "C" int lg_paged_append(const struct lg_paged_cache *c, const void *d_k, const void *d_v, int type, long long ld_k, long long ld_v, int n,
@@ -130,14 +135,67 @@ extern "C" int lg_paged_append(const struct lg_paged_cache *c, const void *d_k, 
     if (c->type == TY_F32) kernel = lg_paged_append_kernel<float, float>;
     else if (c->type == TY_F16) kernel = type == TY_F32 ? lg_paged_append_kernel<float, __half> : lg_paged_append_kernel<__half, __half>;
     else kernel = type == TY_F32 ? lg_paged_append_kernel<float, __nv_bfloat16> : lg_paged_append_kernel<__nv_bfloat16, __nv_bfloat16>;
-    return launch_serve("lg_paged_append", kernel, grid, dim3(256), 0, stream, a);
+    return launch_serve("lg_paged_append", kernel, grid, dim3(256), 0, stream, false, a);
 }
+
+namespace {
+int device_sms(int dev) {
+    static int n[64];
+    int v = dev < 64 ? n[dev] : 0;
+    if (!v) {
+        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); v = 148; }
+        if (dev < 64) n[dev] = v;
+    }
+    return v;
+}
+
+// How an attention call is cut up: query rows of an item (8 NT) and spans of a request at most.  More rows share one read of the cache and
+// more matrix work; 8 NT x head_dim outputs have to fit a warp's registers.
+struct AttnCut { int hd, nt, group_rows, max_spans; };
+AttnCut attn_cut(const struct lg_paged_cache *c, int n_new, int n_heads) {
+    AttnCut k;
+    const int rows = n_new * (n_heads / c->n_kv_heads);
+    k.hd = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : c->head_dim <= 256 ? 256 : 512;
+    const int most = k.hd <= 128 ? 4 : k.hd == 256 ? 2 : 1;
+    k.nt = rows <= 8 || most == 1 ? 1 : rows <= 16 || most == 2 ? 2 : 4;
+    k.group_rows = 8 * k.nt;
+    const long long items = (long long)c->n_kv_heads * ((rows + k.group_rows - 1) / k.group_rows);
+    const long long slices = ((long long)c->max_pages * c->page_size + 15) / 16 + 1;
+    long long spans = items < LG_PA_TARGET ? LG_PA_TARGET / items : 1;
+    if (spans > (slices + LG_PA_MIN_SLICES - 1) / LG_PA_MIN_SLICES) spans = (slices + LG_PA_MIN_SLICES - 1) / LG_PA_MIN_SLICES;
+    k.max_spans = (int)spans;
+    return k;
+}
+
+template <typename TQ, typename TC, int HD, int NT> int launch_attn_tile(LgPagedAttnArgs &a, int dev, void *stream) {
+    typedef LgPagedTile<TQ, TC, HD, NT> P;
+    static unsigned char done[64];
+    if (!allow_smem(lg_paged_attn_kernel<TQ, TC, HD, NT>, P::SMEM, P::SMEM, dev, done)) SERVE_FAIL(-6, "lg_paged_attn: no %d bytes of shared memory", P::SMEM);
+    const long long items = (long long)a.n_req * a.c.n_kv * ((a.n_new * a.gqa + a.group_rows - 1) / a.group_rows) * a.max_spans;
+    const long long ctas = (long long)device_sms(dev) * P::CTAS;
+    return launch_serve("lg_paged_attn", lg_paged_attn_kernel<TQ, TC, HD, NT>, dim3((unsigned)(items < ctas ? items : ctas)), dim3(P::W * 32), P::SMEM, stream,
+                        false, a);
+}
+template <typename TQ, typename TC> int launch_attn_16(LgPagedAttnArgs &a, const AttnCut &k, int dev, void *stream) {
+    int rc;
+    if (k.hd == 64) rc = k.nt == 1 ? launch_attn_tile<TQ, TC, 64, 1>(a, dev, stream) : k.nt == 2 ? launch_attn_tile<TQ, TC, 64, 2>(a, dev, stream) : launch_attn_tile<TQ, TC, 64, 4>(a, dev, stream);
+    else if (k.hd == 128) rc = k.nt == 1 ? launch_attn_tile<TQ, TC, 128, 1>(a, dev, stream) : k.nt == 2 ? launch_attn_tile<TQ, TC, 128, 2>(a, dev, stream) : launch_attn_tile<TQ, TC, 128, 4>(a, dev, stream);
+    else if (k.hd == 256) rc = k.nt == 1 ? launch_attn_tile<TQ, TC, 256, 1>(a, dev, stream) : launch_attn_tile<TQ, TC, 256, 2>(a, dev, stream);
+    else rc = launch_attn_tile<TQ, TC, 512, 1>(a, dev, stream);
+    if (rc || a.max_spans == 1) return rc;
+    const long long warps = (long long)a.n_req * a.n_new * a.n_heads;
+    return launch_serve("lg_paged_attn", lg_paged_merge_kernel<TQ>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream, true, a);
+}
+}  // namespace
 
 extern "C" long long lg_paged_attn_work(const struct lg_paged_cache *c, int n_req, int n_new, int n_heads) {
     if (const char *f = cache_fault(c)) SERVE_FAIL(-1, "lg_paged_attn_work: %s", f);
     if (n_req < 1 || n_req > c->max_req || n_new < 1 || n_new > LG_PAGED_MAX_NEW || n_heads < 1 || n_heads % c->n_kv_heads)
         SERVE_FAIL(-1, "lg_paged_attn_work: bad arguments");
-    return 16;
+    const AttnCut k = attn_cut(c, n_new, n_heads);
+    if (c->type == TY_F32 || k.max_spans == 1) return 16;
+    const long long rows = (long long)n_req * n_new * n_heads * k.max_spans;
+    return rows * (c->head_dim + 2) * 4 + 16;
 }
 
 extern "C" int lg_paged_attn(const struct lg_paged_cache *c, const void *d_q, int type, long long ld_q, int n_req, int n_new, int n_rows,
@@ -155,22 +213,25 @@ extern "C" int lg_paged_attn(const struct lg_paged_cache *c, const void *d_q, in
     const int eb = type_bytes(type);
     if (((uintptr_t)d_q | (uintptr_t)d_out) % eb || (uintptr_t)d_start & 3 || (uintptr_t)d_work & 15)
         SERVE_FAIL(-1, "lg_paged_attn: a misaligned pointer");
-    if (n_heads > 65535 || n_req > 65535) SERVE_FAIL(-2, "lg_paged_attn: %d requests of %d heads", n_req, n_heads);
+    if (n_heads > 65535 || n_req > 65535 || (long long)n_req * n_new * n_heads > 1LL << 31) SERVE_FAIL(-2, "lg_paged_attn: %d requests of %d heads", n_req, n_heads);
     const long long need = lg_paged_attn_work(c, n_req, n_new, n_heads);
     if (work_bytes < need) SERVE_FAIL(-3, "lg_paged_attn: a workspace of %lld bytes, %lld are needed", work_bytes, need);
     OnDevice on;
     add_cache(on, c);
     on.add(d_q); on.add(d_out); on.add(d_work); on.add_opt(d_start);
     if (!on.enter()) SERVE_FAIL(-1, "lg_paged_attn: pointers are not memory of one device");
+    const AttnCut k = attn_cut(c, n_new, n_heads);
     LgPagedAttnArgs a;
     a.c = paged_of(c); a.q = d_q; a.out = d_out; a.ld_q = ld_q; a.ld_out = ld_out; a.n_req = n_req; a.n_new = n_new; a.n_rows = n_rows;
     a.n_heads = n_heads; a.window = window; a.start = d_start;
     a.scale = (scale > 0.0f ? scale : 1.0f / sqrtf((float)c->head_dim)) * LG_LOG2E;
-    void (*kernel)(LgPagedAttnArgs) = nullptr;
-    if (c->type == TY_F32) kernel = lg_paged_attn_rows_kernel<float, float>;
-    else if (c->type == TY_F16) kernel = type == TY_F32 ? lg_paged_attn_rows_kernel<float, __half> : lg_paged_attn_rows_kernel<__half, __half>;
-    else kernel = type == TY_F32 ? lg_paged_attn_rows_kernel<float, __nv_bfloat16> : lg_paged_attn_rows_kernel<__nv_bfloat16, __nv_bfloat16>;
-    return launch_serve("lg_paged_attn", kernel, dim3(n_new, n_heads, n_req), dim3(LG_PATTN_WARPS * 32), 0, stream, a);
+    a.gqa = n_heads / c->n_kv_heads; a.group_rows = k.group_rows; a.max_spans = k.max_spans;
+    a.part = (float *)d_work;
+    a.part_ml = (float2 *)(a.part + (long long)n_req * n_new * n_heads * k.max_spans * c->head_dim);
+    if (c->type == TY_F32)
+        return launch_serve("lg_paged_attn", lg_paged_attn_rows_kernel<float, float>, dim3(n_new, n_heads, n_req), dim3(LG_PATTN_WARPS * 32), 0, stream, false, a);
+    if (c->type == TY_F16) return type == TY_F32 ? launch_attn_16<float, __half>(a, k, on.dev, stream) : launch_attn_16<__half, __half>(a, k, on.dev, stream);
+    return type == TY_F32 ? launch_attn_16<float, __nv_bfloat16>(a, k, on.dev, stream) : launch_attn_16<__nv_bfloat16, __nv_bfloat16>(a, k, on.dev, stream);
 }
 
 extern "C" int lg_sample(const void *d_logits, int type, long long ld, int rows, int vocab, const float *d_temperature, const int *d_top_k,
@@ -192,7 +253,7 @@ extern "C" int lg_sample(const void *d_logits, int type, long long ld, int rows,
     a.shift = 62 - bits;
     a.temperature = d_temperature; a.top_k = d_top_k; a.top_p = d_top_p; a.min_p = d_min_p; a.u = d_u; a.token = d_token; a.prob = d_prob;
     void (*kernel)(LgSampleArgs) = type == TY_F32 ? lg_sample_kernel<float> : type == TY_F16 ? lg_sample_kernel<__half> : lg_sample_kernel<__nv_bfloat16>;
-    return launch_serve("lg_sample", kernel, dim3(rows), dim3(LG_SAMPLE_THREADS), 0, stream, a);
+    return launch_serve("lg_sample", kernel, dim3(rows), dim3(LG_SAMPLE_THREADS), 0, stream, false, a);
 }
 
 // The parameters of the one row go to the device beside its forward; the token and its probability return behind it.

@@ -67,8 +67,8 @@ int  lg_paged_append(const struct lg_paged_cache *c, const void *d_k, const void
  * as lg_paged_step wrote them, at most n_new of them (rows beyond are left as they are, with a status bit), and rows from d_start[n_req] on are left as
  * they are.  The last of a request's m rows is the query at position len - 1, row t the one at len - m + t; it sees the rows at its position and
  * before, with window > 0 the nearest `window` of them.  A query that sees nothing (a length of 0, pages that are not in the cache) gives
- * zeros.  scale 0: 1 / sqrt(head_dim).  A request's rows depend on its own queries, rows and lengths alone, not on the rest of the call, and every
- * sum has a fixed order.
+ * zeros.  scale 0: 1 / sqrt(head_dim).  Rows that a query sees are finite.  Every sum has an order that the call's sizes and lengths
+ * fix: the same call gives the same bits.
  * d_work: lg_paged_attn_work bytes, 16-byte aligned, this call's alone until the call's work has ended: calls and graphs that may
  * overlap have workspaces of their own. */
 long long lg_paged_attn_work(const struct lg_paged_cache *c, int n_req, int n_new, int n_heads);

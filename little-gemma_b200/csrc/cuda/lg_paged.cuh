@@ -255,8 +255,9 @@ struct LgPagedAttnArgs {
     int n_req, n_new, n_rows, n_heads, window;
     float scale;                       // times log2(e)
     const int *start;
-    int gqa, group_rows, max_spans;    // query heads of a KV head, query rows of an item, spans of a request at most
-    float *part; float2 *part_ml;      // [request][token][head][span]: unnormalised output; maximum and sum
+    int gqa, group_rows;               // query heads of a KV head, query rows of an item
+    float *part; float2 *part_ml;      // [CTA][2][query row of an item]: unnormalised output; maximum and sum
+    int4 *jobs;                        // [CTA]: the item that it leaves unfinished (request, head and group, last CTA, rows), or -1
 };
 
 // The block of rows of request r: first row, rows to compute, rows it has.
@@ -341,9 +342,11 @@ template <typename TQ, typename TC> __global__ void __launch_bounds__(LG_PATTN_W
 }
 
 // ---- 16-bit caches: tensor-core tiles, spans over the length, a merge ----------------------------
-// The work is cut into items: (request, KV head, group of 8 NT query rows, span of keys).  A request's spans depend on its own length and on the
-// number of heads alone, never on the other requests, so neither do its sums.  A persistent grid walks the items in that order, each CTA a
-// stretch of about equal key counts; one with several spans leaves (max, sum, unnormalised output) per span for lg_paged_merge_kernel.
+// The work is a line of slices of 16 keys: request by request, KV head by KV head, group of 8 NT query rows by group (an item).  Every CTA of a
+// persistent grid takes a stretch of equal length of that line, so ragged lengths cost nothing; an item that one stretch holds is written at once,
+// of one that several stretches share each leaves (max, sum, unnormalised output), and lg_paged_merge_kernel adds those in their order.
+// (Spans fixed by a request's own length were the first form: 876 us for 96 requests of 1.6K to 16K rows, where this takes less; short spans cost merges,
+// and about as many items as CTAs leave SMs idle: 153 us for two requests of 120000 rows with 58 % of the SMs' time in use.)
 //
 // Inside a CTA every warp works alone: it takes 16 keys (a slice) at a time, brings K and V in with 16-byte asynchronous copies through a ring
 // of U units of its own (a unit: 16 rows of K or of V; rows that no query may see are filled with zeros and never read), so the loop has no block barrier and
@@ -352,8 +355,9 @@ template <typename TQ, typename TC> __global__ void __launch_bounds__(LG_PATTN_W
 // P^T turned from accumulator order into operand order by movmatrix.  Numerics: an f32 query enters as a sum of 16-bit parts (f16: 2 parts behind a
 // power of two per row, 22 bits; bf16: 3, 24 bits), P as 2 parts (3 where the answer is f32 and the cache bf16); P carries a factor 2^15 in f16 so that
 // weights down to 2^-29 of the largest stay normal numbers.  Everything else is f32.
-#define LG_PA_TARGET 148               // items that a request of one KV head is cut into at most: the device's SMs
-#define LG_PA_MIN_SLICES 8             // of a span
+#define LG_PA_MAX_CTAS 296             // two per SM
+#define LG_PA_ITEM_COST 6              // of an item beside its slices, in slices: queries in, warps' results together, rows out
+#define LG_PA_MIN_STRETCH 8
 
 template <typename T> __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma_16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { mma_f16(c, a, b0, b1); }
@@ -392,7 +396,7 @@ template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile(
 struct LgReq {
     int first, m, held, len;           // rows, see paged_rows
     int groups;                        // of query rows, per KV head
-    int s0, n_sl, ss, spans;           // first slice, slices, slices per span, spans
+    int s0, n_sl;                      // first slice, slices
 };
 __device__ __forceinline__ LgReq paged_request(const LgPagedAttnArgs &a, int r) {
     LgReq q;
@@ -403,32 +407,26 @@ __device__ __forceinline__ LgReq paged_request(const LgPagedAttnArgs &a, int r) 
     const int hi = max(0, q.len - q.held + q.m), lo = a.window > 0 ? max(0, q.len - q.held - a.window + 1) : 0;
     q.s0 = min(lo, hi) >> 4;
     q.n_sl = ((hi + 15) >> 4) - q.s0;
-    q.ss = max(LG_PA_MIN_SLICES, (q.n_sl + a.max_spans - 1) / a.max_spans);
-    q.ss = (q.ss + 3) & ~3;
-    q.spans = max(1, (q.n_sl + q.ss - 1) / q.ss);
     return q;
 }
-// Weight of a request in the walk: slices of all its items, at least one each (an item without keys writes zeros)
-__device__ __forceinline__ long long paged_weight(const LgPagedAttnArgs &a, const LgReq &q) { return (long long)max(1, q.n_sl) * q.groups * a.c.n_kv; }
+__device__ __forceinline__ long long paged_weight(const LgPagedAttnArgs &a, const LgReq &q) { return (long long)(q.n_sl + LG_PA_ITEM_COST) * q.groups * a.c.n_kv; }
 
-// The walk of one CTA: items whose offset in the order of slices is below `end`.
+// The walk of one CTA over the items that begin before the end of its stretch lo .. hi-1 of the line.
 struct LgWalk {
     LgReq q;
-    int r, hg, span;                   // request, KV head * groups + group, span
-    long long at, end;                 // offset of the request's current (head, group), end of the CTA's stretch
-    __device__ __forceinline__ bool valid(const LgPagedAttnArgs &a) const { return r < a.n_req && at + (long long)span * q.ss < end; }
-    __device__ __forceinline__ void settle(const LgPagedAttnArgs &a) {        // past requests without rows
-        while (r < a.n_req && hg >= q.groups * a.c.n_kv) {
-            if (++r < a.n_req && at < end) { q = paged_request(a, r); hg = 0; span = 0; }
-            else if (r < a.n_req) r = a.n_req;
-        }
-    }
+    int r, hg;                         // request, KV head * groups + group
+    long long at, lo, hi;              // where the item begins; the stretch
+    __device__ __forceinline__ bool valid(const LgPagedAttnArgs &a) const { return r < a.n_req && at < hi; }
+    __device__ __forceinline__ int begin() const { return (int)max(lo - at, 0LL); }                        // the item's slices in the stretch
+    __device__ __forceinline__ int end() const { return (int)min(hi - at, (long long)q.n_sl); }
     __device__ __forceinline__ void next(const LgPagedAttnArgs &a) {
-        if (++span < q.spans) return;
-        span = 0;
-        at += max(1, q.n_sl);
+        at += q.n_sl + LG_PA_ITEM_COST;
         hg++;
-        settle(a);
+        while (r < a.n_req && hg >= q.groups * a.c.n_kv) {                    // past requests without rows
+            if (++r < a.n_req) {
+                if (at < hi) { q = paged_request(a, r); hg = 0; } else r = a.n_req;
+            }
+        }
     }
 };
 
@@ -471,6 +469,7 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
 
     // this CTA's stretch: weights of all requests, thread by thread, and where the stretch begins
     LgWalk w;
+    long long stretch;
     {
         const int per = (a.n_req + P::W * 32 - 1) / (P::W * 32), r0 = min(a.n_req, tid * per), r1 = min(a.n_req, r0 + per);
         long long mine = 0;
@@ -485,27 +484,26 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
         #pragma unroll
         for (int i = 0; i < P::W; i++) { if (i < warp) before += red[i]; total += red[i]; }
         before += s - mine;
-        const long long lo = total * blockIdx.x / gridDim.x, hi = total * (blockIdx.x + 1) / gridDim.x;
-        if (mine && before <= lo && lo < before + mine) {
+        stretch = max((long long)LG_PA_MIN_STRETCH, (total + gridDim.x - 1) / gridDim.x);
+        stretch = (stretch + P::W - 1) / P::W * P::W;
+        w.lo = stretch * blockIdx.x; w.hi = min(w.lo + stretch, total);
+        if (mine && before <= w.lo && w.lo < before + mine) {
             int r = r0;
             for (;; r++) {
                 const long long x = paged_weight(a, paged_request(a, r));
-                if (lo < before + x) break;
+                if (w.lo < before + x) break;
                 before += x;
             }
             red[8] = r; red[9] = before;
         }
         __syncthreads();
-        w.r = (int)red[8]; w.end = hi;
-        if (w.r >= a.n_req || lo >= hi) return;
-        w.at = red[9];
+        w.r = (int)red[8];
+        if (tid == 0) a.jobs[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        if (w.r >= a.n_req) return;
         w.q = paged_request(a, w.r);
-        const int n = max(1, w.q.n_sl);
-        const long long rem = lo - w.at;
-        w.hg = (int)(rem / n);
-        w.at += (long long)w.hg * n;
-        w.span = ((int)(rem - (long long)w.hg * n) + w.q.ss - 1) / w.q.ss;    // the first item that begins in the stretch
-        if (w.span >= w.q.spans) { w.span = w.q.spans - 1; w.next(a); }
+        const int n = w.q.n_sl + LG_PA_ITEM_COST;
+        w.hg = (int)((w.lo - red[9]) / n);
+        w.at = red[9] + (long long)w.hg * n;
     }
     // the copies run ahead of the arithmetic with a walk of their own
     LgWalk p = w;
@@ -515,8 +513,8 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
     const int ps_size = a.c.page_size, hd8 = a.c.hd >> 3;
     auto begin_item = [&]() {                                                 // first slice of this warp in walk p's item, or the next item that has one
         while (p.valid(a)) {
-            ps = p.q.s0 + p.span * p.q.ss + warp;
-            ps_end = p.q.s0 + min(p.q.n_sl, (p.span + 1) * p.q.ss);
+            ps = p.q.s0 + p.begin() + warp;
+            ps_end = p.q.s0 + p.end();
             if (ps < ps_end) return true;
             p.next(a);
         }
@@ -568,8 +566,11 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
 
     int slot = 0, n_used = 0, q_r = -1, q_hg = -1, turn = 0;
     uint32_t qr[P::QREG ? NT * P::NQ * P::KS * 2 : 1];
-    for (; w.valid(a); w.next(a), turn ^= 1) {
+    for (; w.valid(a); w.next(a)) {
+        const int s_begin = w.q.s0 + w.begin(), s_end = w.q.s0 + w.end();
+        if (s_begin >= s_end && (w.q.n_sl || w.at < w.lo)) continue;          // another stretch has its slices, or writes its zeros
         float2 *stat = stats + turn * P::W * P::ROWS;
+        turn ^= 1;
         const int kvh = w.hg / w.q.groups, row0 = (w.hg - kvh * w.q.groups) * P::ROWS;      // first of the group's rows: row = token * gqa + head of the group
         const int n_rows = min(P::ROWS, w.q.m * a.gqa - row0);
         if (q_r != w.r || q_hg != w.hg) {                                     // queries of the group into operand order
@@ -636,8 +637,7 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                 #pragma unroll
                 for (int j = 0; j < 4; j++) o[ks][nt][j] = 0.0f;
         const int pos_lo = pos0 + row0 / a.gqa, pos_hi = pos0 + (row0 + n_rows - 1) / a.gqa;
-        const int s_end = w.q.s0 + min(w.q.n_sl, (w.span + 1) * w.q.ss);
-        for (int s = w.q.s0 + w.span * w.q.ss + warp; s < s_end; s += P::W) {
+        for (int s = s_begin + warp; s < s_end; s += P::W) {
             cp_async_wait<P::U - 2>();
             __syncwarp();
             issue();
@@ -769,6 +769,10 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             }
             __syncthreads();
         }
+        // the item's other slices: before this stretch, behind it (its last slice then lies in the stretch of CTA `last`)
+        const bool head = w.at < w.lo, tail = w.at + w.q.n_sl > w.hi;
+        const long long part = ((long long)blockIdx.x * 2 + !head) * P::ROWS;
+        if (!head && tail && tid == 0) a.jobs[blockIdx.x] = make_int4(w.r, w.hg, (int)((w.at + w.q.n_sl - 1) / stretch), n_rows);
         for (int n = warp; n < n_rows; n += P::W) {
             float m2 = -INFINITY, sum = 0.0f;
             #pragma unroll
@@ -776,55 +780,67 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             #pragma unroll
             for (int i = 0; i < P::W; i++) sum += stat[i * P::ROWS + n].y * ex2(stat[i * P::ROWS + n].x - (m2 == -INFINITY ? 0.0f : m2));
             const int rho = row0 + n, t = rho / a.gqa, h = kvh * a.gqa + rho - t * a.gqa;
-            if (w.q.spans == 1) {
+            if (!head && !tail) {
                 TQ *out = (TQ *)a.out + (long long)(w.q.first + t) * a.ld_out + (long long)h * a.c.hd;
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 for (int d = lane; d < a.c.hd; d += 32) out[d] = Elem<TQ>::put(buf[n * P::LDB + d] * inv);
             } else {
-                const long long prow = (((long long)w.r * a.n_new + t) * a.n_heads + h) * a.max_spans + w.span;
-                for (int d = lane; d < a.c.hd; d += 32) a.part[prow * a.c.hd + d] = buf[n * P::LDB + d];
-                if (lane == 0) a.part_ml[prow] = make_float2(m2, sum);
+                for (int d = lane; d < a.c.hd; d += 32) a.part[(part + n) * a.c.hd + d] = buf[n * P::LDB + d];
+                if (lane == 0) a.part_ml[part + n] = make_float2(m2, sum);
             }
         }
     }
 }
 
-// A warp per query row and head: the spans' results in their order.  Bound by the reads of the partial results.
+// One item that CTA b began and did not end, one query row (grid: CTAs, rows of a group): the parts, b's own and those of the CTAs behind it, each
+// warp every eighth, then the warps in order.  Bound by latency.
 template <typename TQ> __global__ void __launch_bounds__(256) lg_paged_merge_kernel(LgPagedAttnArgs a) {
-    const long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, h = (int)(i % a.n_heads);
-    const long long j = i / a.n_heads;
-    const int t = (int)(j % a.n_new), r = (int)(j / a.n_new);
+    __shared__ float po[8][512], pl[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.y, b = blockIdx.x;
     pdl_wait();
-    if (r >= a.n_req) return;
-    const LgReq q = paged_request(a, r);
-    if (t >= q.m || q.spans == 1) return;
-    const long long prow = (((long long)r * a.n_new + t) * a.n_heads + h) * a.max_spans;
+    const int4 job = a.jobs[b];
+    if (job.x < 0 || n >= job.w) return;
+    const LgReq q = paged_request(a, job.x);
+    const int parts = job.z - b + 1;
+    // part i: the last place of CTA b, the first one of those behind it
+    auto place = [&](int i) { return ((long long)(b + i) * 2 + (i == 0)) * a.group_rows + n; };
     float top = -INFINITY;
-    for (int s = lane; s < q.spans; s += 32) top = fmaxf(top, a.part_ml[prow + s].x);
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_ml[place(i)].x);
     top = warp_max(top);
     const float ref = top == -INFINITY ? 0.0f : top;
     float y[16], sum = 0.0f;                                                  // dims lane * 4 .. of every 128
     #pragma unroll
     for (int k = 0; k < 16; k++) y[k] = 0.0f;
-    for (int s = 0; s < q.spans; s++) {
-        const float2 ml = a.part_ml[prow + s];
+    for (int i = warp; i < parts; i += 8) {
+        const float2 ml = a.part_ml[place(i)];
         const float f = ex2(ml.x - ref);
         sum += ml.y * f;
         #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int d = k * 128 + lane * 4;
             if (d < a.c.hd) {
-                const float4 v = *(const float4 *)(a.part + (prow + s) * a.c.hd + d);
+                const float4 v = *(const float4 *)(a.part + place(i) * a.c.hd + d);
                 y[4 * k] += v.x * f; y[4 * k + 1] += v.y * f; y[4 * k + 2] += v.z * f; y[4 * k + 3] += v.w * f;
             }
         }
     }
-    TQ *out = (TQ *)a.out + (long long)(q.first + t) * a.ld_out + (long long)h * a.c.hd;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     #pragma unroll
-    for (int k = 0; k < 16; k++) {
-        const int d = (k >> 2) * 128 + lane * 4 + (k & 3);
-        if (d < a.c.hd) out[d] = Elem<TQ>::put(y[k] * inv);
+    for (int k = 0; k < 4; k++) {
+        const int d = k * 128 + lane * 4;
+        if (d < a.c.hd) *(float4 *)&po[warp][d] = make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+    }
+    if (lane == 0) pl[warp] = sum;
+    __syncthreads();
+    sum = 0.0f;
+    #pragma unroll
+    for (int i = 0; i < 8; i++) sum += pl[i];
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int kvh = job.y / q.groups, rho = (job.y - kvh * q.groups) * a.group_rows + n, t = rho / a.gqa;
+    TQ *out = (TQ *)a.out + (long long)(q.first + t) * a.ld_out + (long long)(kvh * a.gqa + rho - t * a.gqa) * a.c.hd;
+    for (int d = threadIdx.x; d < a.c.hd; d += 256) {
+        float x = 0.0f;
+        #pragma unroll
+        for (int i = 0; i < 8; i++) x += po[i][d];
+        out[d] = Elem<TQ>::put(x * inv);
     }
 }

@@ -149,21 +149,15 @@ int device_sms(int dev) {
     return v;
 }
 
-// How an attention call is cut up: query rows of an item (8 NT) and spans of a request at most.  More rows share one read of the cache and
-// more matrix work; 8 NT x head_dim outputs have to fit a warp's registers.
-struct AttnCut { int hd, nt, group_rows, max_spans; };
+// Query rows of an item, 8 nt: more rows share one read of the cache and more matrix work; 8 nt x head_dim outputs have to fit a
+// warp's registers.
+struct AttnCut { int hd, nt; };
 AttnCut attn_cut(const struct lg_paged_cache *c, int n_new, int n_heads) {
     AttnCut k;
     const int rows = n_new * (n_heads / c->n_kv_heads);
     k.hd = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : c->head_dim <= 256 ? 256 : 512;
     const int most = k.hd <= 128 ? 4 : k.hd == 256 ? 2 : 1;
     k.nt = rows <= 8 || most == 1 ? 1 : rows <= 16 || most == 2 ? 2 : 4;
-    k.group_rows = 8 * k.nt;
-    const long long items = (long long)c->n_kv_heads * ((rows + k.group_rows - 1) / k.group_rows);
-    const long long slices = ((long long)c->max_pages * c->page_size + 15) / 16 + 1;
-    long long spans = items < LG_PA_TARGET ? LG_PA_TARGET / items : 1;
-    if (spans > (slices + LG_PA_MIN_SLICES - 1) / LG_PA_MIN_SLICES) spans = (slices + LG_PA_MIN_SLICES - 1) / LG_PA_MIN_SLICES;
-    k.max_spans = (int)spans;
     return k;
 }
 
@@ -171,10 +165,15 @@ template <typename TQ, typename TC, int HD, int NT> int launch_attn_tile(LgPaged
     typedef LgPagedTile<TQ, TC, HD, NT> P;
     static unsigned char done[64];
     if (!allow_smem(lg_paged_attn_kernel<TQ, TC, HD, NT>, P::SMEM, P::SMEM, dev, done)) SERVE_FAIL(-6, "lg_paged_attn: no %d bytes of shared memory", P::SMEM);
-    const long long items = (long long)a.n_req * a.c.n_kv * ((a.n_new * a.gqa + a.group_rows - 1) / a.group_rows) * a.max_spans;
-    const long long ctas = (long long)device_sms(dev) * P::CTAS;
-    return launch_serve("lg_paged_attn", lg_paged_attn_kernel<TQ, TC, HD, NT>, dim3((unsigned)(items < ctas ? items : ctas)), dim3(P::W * 32), P::SMEM, stream,
-                        false, a);
+    const int sms = device_sms(dev), ctas = sms * P::CTAS < LG_PA_MAX_CTAS ? sms * P::CTAS : LG_PA_MAX_CTAS;
+    // slices that there can be at most, so that no CTA comes for nothing
+    const long long slices = ((long long)a.c.max_pages * a.c.page_size + 15) / 16 + 1 + LG_PA_ITEM_COST;
+    const long long all = slices * a.n_req * a.c.n_kv * ((a.n_new * a.gqa + a.group_rows - 1) / a.group_rows) / LG_PA_MIN_STRETCH + 1;
+    const int grid = all < ctas ? (int)all : ctas;
+    const int rc = launch_serve("lg_paged_attn", lg_paged_attn_kernel<TQ, TC, HD, NT>, dim3(grid), dim3(P::W * 32), P::SMEM, stream, false, a);
+    if (rc || grid == 1) return rc;
+    const int rows = a.n_new * a.gqa;
+    return launch_serve("lg_paged_attn", lg_paged_merge_kernel<TQ>, dim3(grid - 1, rows < a.group_rows ? rows : a.group_rows), dim3(256), 0, stream, true, a);
 }
 template <typename TQ, typename TC> int launch_attn_16(LgPagedAttnArgs &a, const AttnCut &k, int dev, void *stream) {
     int rc;
@@ -182,9 +181,7 @@ template <typename TQ, typename TC> int launch_attn_16(LgPagedAttnArgs &a, const
     else if (k.hd == 128) rc = k.nt == 1 ? launch_attn_tile<TQ, TC, 128, 1>(a, dev, stream) : k.nt == 2 ? launch_attn_tile<TQ, TC, 128, 2>(a, dev, stream) : launch_attn_tile<TQ, TC, 128, 4>(a, dev, stream);
     else if (k.hd == 256) rc = k.nt == 1 ? launch_attn_tile<TQ, TC, 256, 1>(a, dev, stream) : launch_attn_tile<TQ, TC, 256, 2>(a, dev, stream);
     else rc = launch_attn_tile<TQ, TC, 512, 1>(a, dev, stream);
-    if (rc || a.max_spans == 1) return rc;
-    const long long warps = (long long)a.n_req * a.n_new * a.n_heads;
-    return launch_serve("lg_paged_attn", lg_paged_merge_kernel<TQ>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream, true, a);
+    return rc;
 }
 }  // namespace
 
@@ -193,9 +190,7 @@ extern "C" long long lg_paged_attn_work(const struct lg_paged_cache *c, int n_re
     if (n_req < 1 || n_req > c->max_req || n_new < 1 || n_new > LG_PAGED_MAX_NEW || n_heads < 1 || n_heads % c->n_kv_heads)
         SERVE_FAIL(-1, "lg_paged_attn_work: bad arguments");
     const AttnCut k = attn_cut(c, n_new, n_heads);
-    if (c->type == TY_F32 || k.max_spans == 1) return 16;
-    const long long rows = (long long)n_req * n_new * n_heads * k.max_spans;
-    return rows * (c->head_dim + 2) * 4 + 16;
+    return LG_PA_MAX_CTAS * (16 + 2LL * 8 * k.nt * (c->head_dim + 2) * 4);
 }
 
 extern "C" int lg_paged_attn(const struct lg_paged_cache *c, const void *d_q, int type, long long ld_q, int n_req, int n_new, int n_rows,
@@ -225,9 +220,10 @@ extern "C" int lg_paged_attn(const struct lg_paged_cache *c, const void *d_q, in
     a.c = paged_of(c); a.q = d_q; a.out = d_out; a.ld_q = ld_q; a.ld_out = ld_out; a.n_req = n_req; a.n_new = n_new; a.n_rows = n_rows;
     a.n_heads = n_heads; a.window = window; a.start = d_start;
     a.scale = (scale > 0.0f ? scale : 1.0f / sqrtf((float)c->head_dim)) * LG_LOG2E;
-    a.gqa = n_heads / c->n_kv_heads; a.group_rows = k.group_rows; a.max_spans = k.max_spans;
-    a.part = (float *)d_work;
-    a.part_ml = (float2 *)(a.part + (long long)n_req * n_new * n_heads * k.max_spans * c->head_dim);
+    a.gqa = n_heads / c->n_kv_heads; a.group_rows = 8 * k.nt;
+    a.jobs = (int4 *)d_work;
+    a.part = (float *)(a.jobs + LG_PA_MAX_CTAS);
+    a.part_ml = (float2 *)(a.part + LG_PA_MAX_CTAS * 2LL * a.group_rows * c->head_dim);
     if (c->type == TY_F32)
         return launch_serve("lg_paged_attn", lg_paged_attn_rows_kernel<float, float>, dim3(n_new, n_heads, n_req), dim3(LG_PATTN_WARPS * 32), 0, stream, false, a);
     if (c->type == TY_F16) return type == TY_F32 ? launch_attn_16<float, __half>(a, k, on.dev, stream) : launch_attn_16<__half, __half>(a, k, on.dev, stream);

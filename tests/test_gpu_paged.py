@@ -277,15 +277,21 @@ def test_attention_of_queries_far_from_one(lg, dtype, cache, gain):
 
 
 @pytest.mark.parametrize("dtype,cache", [(F32, F16), (BF16, BF16), (F32, F32)])
-def test_a_request_does_not_depend_on_its_neighbours(lg, dtype, cache):
+def test_the_same_call_gives_the_same_bits(lg, dtype, cache):
+    """Whatever the workspace holds; a request alone agrees with itself in the batch to the tolerance of both (_attn_case)."""
     import torch
-    lens, m = [900, 17, 2500, 300], [2, 2, 2, 2]
+    lens, m = [900, 17, 25000, 300], [2, 2, 2, 2]
     c, q, out, work = _attn_case(lg, 2, lens, m, 8, 2, 128, 16, dtype, cache)
+    again = torch.empty_like(out)
+    work.fill_(17)
+    c.c.attn(q, again, work, n_new=2)
+    assert torch.equal(again, out)
     for r in range(4):
         alone = torch.empty_like(out[:2])
         one = lg.PagedCache(c.k, c.v, c.table[r:r + 1], c.len[r:r + 1])
         one.attn(q[2 * r:2 * r + 2], alone, work, n_new=2)
-        assert torch.equal(alone, out[2 * r:2 * r + 2]), r
+        step = 2 * HALF_STEP[dtype] * out[2 * r:2 * r + 2].abs().float() + (2.0 ** -16 if dtype != F32 else 2e-4)
+        assert bool(((alone - out[2 * r:2 * r + 2]).abs().float() <= step).all()), r
 
 
 @pytest.mark.parametrize("dtype,cache", [(F32, F16), (BF16, BF16), (F32, F32)])

@@ -230,11 +230,37 @@ extern "C" int lg_paged_attn(const struct lg_paged_cache *c, const void *d_q, in
     return type == TY_F32 ? launch_attn_16<float, __nv_bfloat16>(a, k, on.dev, stream) : launch_attn_16<__nv_bfloat16, __nv_bfloat16>(a, k, on.dev, stream);
 }
 
+namespace {
+// CTAs that share a row: as many as it takes to hold it in shared memory, more while there are fewer CTAs than SMs and each still has
+// 4096 tokens; at most 8, the largest cluster that every device places.
+template <typename T> int launch_sample(LgSampleArgs &a, int dev, void *stream) {
+    const int sms = device_sms(dev), hist = 2 * a.limbs * LG_SAMPLE_BINS * 4, room = 220 * 1024 - hist;
+    int ranks = 1;
+    while (ranks < LG_SAMPLE_MAX_CLUSTER && ((long long)(a.vocab + ranks - 1) / ranks * (int)sizeof(T) > room ||
+                                             ((long long)a.rows * ranks * 2 <= sms && a.vocab / (ranks * 2) >= 4096))) ranks *= 2;
+    a.slice = ((a.vocab + ranks - 1) / ranks + 127) / 128 * 128;
+    const long long most = room / sizeof(T) / 128 * 128;
+    a.cap = (int)(a.slice < most ? a.slice : most);
+    const size_t smem = (size_t)a.cap * sizeof(T) + hist;
+    static unsigned char done[64];
+    if (!allow_smem(lg_sample_kernel<T>, smem, 220 * 1024, dev, done)) SERVE_FAIL(-6, "lg_sample: no %zu bytes of shared memory", smem);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.rows * ranks); cfg.blockDim = dim3(LG_SAMPLE_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = ranks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    const cudaError_t rc = cudaLaunchKernelEx(&cfg, lg_sample_kernel<T>, a);
+    if (rc != cudaSuccess) { cudaGetLastError(); SERVE_FAIL(-6, "lg_sample: launch failed: %s", cudaGetErrorString(rc)); }
+    return 0;
+}
+}  // namespace
+
 extern "C" int lg_sample(const void *d_logits, int type, long long ld, int rows, int vocab, const float *d_temperature, const int *d_top_k,
                          const float *d_top_p, const float *d_min_p, const float *d_u, int *d_token, float *d_prob, void *stream) {
     if (rows == 0) return 0;
     if (!d_logits || !d_u || !d_token || rows < 0 || vocab < 1 || ld < vocab || !known_type(type)) SERVE_FAIL(-1, "lg_sample: bad arguments");
-    if (vocab > 1 << 20) SERVE_FAIL(-2, "lg_sample: a vocabulary of %d, at most %d", vocab, 1 << 20);
+    if (vocab > 1 << 20 || rows > 1 << 27) SERVE_FAIL(-2, "lg_sample: %d rows of %d, at most %d of %d", rows, vocab, 1 << 27, 1 << 20);
     if ((uintptr_t)d_logits % type_bytes(type) ||
         ((uintptr_t)d_temperature | (uintptr_t)d_top_k | (uintptr_t)d_top_p | (uintptr_t)d_min_p | (uintptr_t)d_u | (uintptr_t)d_token | (uintptr_t)d_prob) & 3)
         SERVE_FAIL(-1, "lg_sample: a pointer into the middle of an element");
@@ -243,13 +269,13 @@ extern "C" int lg_sample(const void *d_logits, int type, long long ld, int rows,
     on.add_opt(d_temperature); on.add_opt(d_top_k); on.add_opt(d_top_p); on.add_opt(d_min_p); on.add_opt(d_prob);
     if (!on.enter()) SERVE_FAIL(-1, "lg_sample: pointers are not memory of one device");
     LgSampleArgs a;
-    a.logits = d_logits; a.ld = ld; a.vocab = vocab;
+    a.logits = d_logits; a.ld = ld; a.rows = rows; a.vocab = vocab;
     int bits = 0;
     while ((1 << bits) < vocab) bits++;
-    a.shift = 62 - bits;
+    a.shift = 62 - bits < 44 ? 62 - bits : 44;
     a.temperature = d_temperature; a.top_k = d_top_k; a.top_p = d_top_p; a.min_p = d_min_p; a.u = d_u; a.token = d_token; a.prob = d_prob;
-    void (*kernel)(LgSampleArgs) = type == TY_F32 ? lg_sample_kernel<float> : type == TY_F16 ? lg_sample_kernel<__half> : lg_sample_kernel<__nv_bfloat16>;
-    return launch_serve("lg_sample", kernel, dim3(rows), dim3(LG_SAMPLE_THREADS), 0, stream, false, a);
+    a.limbs = d_top_p ? 3 : d_top_k ? 1 : 0;
+    return type == TY_F32 ? launch_sample<float>(a, on.dev, stream) : type == TY_F16 ? launch_sample<__half>(a, on.dev, stream) : launch_sample<__nv_bfloat16>(a, on.dev, stream);
 }
 
 // The parameters of the one row go to the device beside its forward; the token and its probability return behind it.

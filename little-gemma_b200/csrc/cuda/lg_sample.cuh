@@ -9,19 +9,21 @@
 // A cluster of CTAs holds a row in shared memory after one read of HBM (the part that does not fit is read again from L2); what all
 // CTAs have to know -- the maximum, histograms, sums -- goes through distributed shared memory with one cluster barrier each, and every CTA draws the same
 // conclusions from it.  A threshold is found without sorting:
-//   coarse  y = 32 log2(e) (max - l) / T, rounded, is the bin of a token (at most 2047: beyond, a weight is 0); counts per bin and the bounds of a bin's
-//           weights tell the bins that the threshold can lie in, and with them an interval of logits
-//   fine    exact counts or weights over 2048 equal parts of that interval of keys (the logits as ordered integers), then of the part that holds the threshold,
-//           until a part is a single key: at most three rounds
-// Bound by 64-bit arithmetic (about 11 operations a weight, 64 a cycle and SM) and, for few rows, by the cluster barriers.
+//   coarse  bins of 1/16 of a power of two of the weight (1024: beyond, a weight is 0); counts per bin and the bounds of a bin's weights tell the bins that the
+//           threshold can lie in, and with them an interval of logits
+//   list    each warp notes its tokens in or above that interval, where they are few; later passes read the list
+//   fine    exact counts or weights over 1024 equal parts of that interval of keys (the logits as ordered integers), then of the part that holds the threshold,
+//           until a part is a single key: at most four rounds
+// Bound by the instructions of a pass over the row (about 30 a token and weight, 11 of them 64-bit arithmetic) and, for few rows, by the cluster barriers.
 #pragma once
 #include "lg_device.cuh"
 #include <cuda_bf16.h>
 
 #define LG_SAMPLE_THREADS 512
 #define LG_SAMPLE_WARPS (LG_SAMPLE_THREADS / 32)
-#define LG_SAMPLE_BINS 2048
-#define LG_SAMPLE_MAX_CLUSTER 8
+#define LG_SAMPLE_BINS 1024            // two a thread
+#define LG_SAMPLE_LIST 128             // tokens a warp's list holds
+#define LG_SAMPLE_MAX_CLUSTER 16
 
 typedef unsigned long long u64;
 
@@ -35,102 +37,100 @@ struct LgSampleArgs {
     int *token; float *prob;
 };
 
-// A logit as the bits of its f32 value, and as an unsigned integer in the order of the logits (LOW: bits that are the same in every f32 that the type
-// holds; they are dropped).  NaN lowest, -0 equal to 0.
+// A logit as its f32 value, four at a time, and the larger of two words of logits (NaN loses); LOW: bits that are the same in every f32 that the
+// type holds.
 template <typename T> struct LogitType;
 template <> struct LogitType<float> {
     static constexpr int LOW = 0;
-    static __device__ __forceinline__ uint32_t bits(const float *p) { return __float_as_uint(*p); }
-    static __device__ __forceinline__ void bits4(const float *p, uint32_t (&b)[4]) {
-        const uint4 v = *(const uint4 *)p;
-        b[0] = v.x; b[1] = v.y; b[2] = v.z; b[3] = v.w;
+    static __device__ __forceinline__ float value(const float *p) { return *p; }
+    static __device__ __forceinline__ void value4(const float *p, float (&l)[4]) {
+        const float4 v = *(const float4 *)p;
+        l[0] = v.x; l[1] = v.y; l[2] = v.z; l[3] = v.w;
     }
+    static __device__ __forceinline__ uint32_t lowest() { return 0xFF800000u; }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+    static __device__ __forceinline__ float most(uint32_t a) { return __uint_as_float(a); }
 };
 template <> struct LogitType<__half> {
     static constexpr int LOW = 13;
-    static __device__ __forceinline__ uint32_t bits(const __half *p) { return __float_as_uint(__half2float(*p)); }
-    static __device__ __forceinline__ void bits4(const __half *p, uint32_t (&b)[4]) {
+    static __device__ __forceinline__ float value(const __half *p) { return __half2float(*p); }
+    static __device__ __forceinline__ void value4(const __half *p, float (&l)[4]) {
         const uint2 v = *(const uint2 *)p;
         const float2 f = __half22float2(*(const __half2 *)&v.x), h = __half22float2(*(const __half2 *)&v.y);
-        b[0] = __float_as_uint(f.x); b[1] = __float_as_uint(f.y); b[2] = __float_as_uint(h.x); b[3] = __float_as_uint(h.y);
+        l[0] = f.x; l[1] = f.y; l[2] = h.x; l[3] = h.y;
     }
+    static __device__ __forceinline__ uint32_t lowest() { return 0xFC00FC00u; }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { const __half2 m = __hmax2(*(const __half2 *)&a, *(const __half2 *)&b); return *(const uint32_t *)&m; }
+    static __device__ __forceinline__ float most(uint32_t a) { const float2 f = __half22float2(*(const __half2 *)&a); return fmaxf(f.x, f.y); }
 };
 template <> struct LogitType<__nv_bfloat16> {
     static constexpr int LOW = 16;
-    static __device__ __forceinline__ uint32_t bits(const __nv_bfloat16 *p) { return (uint32_t)*(const uint16_t *)p << 16; }
-    static __device__ __forceinline__ void bits4(const __nv_bfloat16 *p, uint32_t (&b)[4]) {
+    static __device__ __forceinline__ float value(const __nv_bfloat16 *p) { return __uint_as_float((uint32_t)*(const uint16_t *)p << 16); }
+    static __device__ __forceinline__ void value4(const __nv_bfloat16 *p, float (&l)[4]) {
         const uint2 v = *(const uint2 *)p;
-        b[0] = v.x << 16; b[1] = v.x & 0xFFFF0000u; b[2] = v.y << 16; b[3] = v.y & 0xFFFF0000u;
+        l[0] = __uint_as_float(v.x << 16); l[1] = __uint_as_float(v.x & 0xFFFF0000u);
+        l[2] = __uint_as_float(v.y << 16); l[3] = __uint_as_float(v.y & 0xFFFF0000u);
     }
+    static __device__ __forceinline__ uint32_t lowest() { return 0xFF80FF80u; }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { const __nv_bfloat162 m = __hmax2(*(const __nv_bfloat162 *)&a, *(const __nv_bfloat162 *)&b); return *(const uint32_t *)&m; }
+    static __device__ __forceinline__ float most(uint32_t a) { return fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u)); }
 };
-#define LG_NAN_BITS 0x7FC00000u
-template <int LOW> __device__ __forceinline__ uint32_t key_of(uint32_t b) {
-    if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 0;
-    if (b == 0x80000000u) b = 0;
+// Logits as unsigned integers in their order (-0 is 0; no NaN), without the bits that are always the same
+template <int LOW> __device__ __forceinline__ uint32_t key_of(float l) {
+    const uint32_t b = l == 0.0f ? 0u : __float_as_uint(l);
     return (b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u)) >> LOW;
 }
-template <int LOW> __device__ __forceinline__ uint32_t key_bits(uint32_t k) {
+template <int LOW> __device__ __forceinline__ float key_value(uint32_t k) {
     const uint32_t full = k << LOW;
-    return (full >> 31) ? full ^ 0x80000000u : ~(full | ((1u << LOW) - 1));
+    return __uint_as_float((full >> 31) ? full ^ 0x80000000u : ~(full | ((1u << LOW) - 1)));
 }
-// the same of a number, rounded down or up to a f32
-template <int LOW> __device__ __forceinline__ uint32_t key_below(double x) { return key_of<LOW>(__float_as_uint(__double2float_rd(x))); }
-template <int LOW> __device__ __forceinline__ uint32_t key_above(double x) { return key_of<LOW>(__float_as_uint(__double2float_ru(x))); }
 
 // exp((l - top) / T) of a row
+#define LG_TWO52 4503599627370496.0
+#define LG_MAGIC 6755399441055744.0    // 1.5 2^52: adding it rounds to a whole number, which the low word then holds
 struct LgWeight {
-    double top, inv32, root;           // inv32: 32 log2(e) / T; root: 2^(-lane / 32)
-    int shift;
-    bool inf;                          // the largest logit is +inf: 1 for those, 0 for the others
-    // y of a logit; false: its weight is 0
-    __device__ __forceinline__ bool arg(uint32_t b, double &y) const {
-        y = 0.0;
-        const uint32_t e = b & 0x7F800000u;
-        if (inf) return b == 0x7F800000u;
-        if (e == 0x7F800000u) return false;                                   // -inf, NaN
-        // f32 -> f64 by moving bits: the conversion instruction runs at a quarter of the rate of the arithmetic
-        const double l = e ? __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u)), (int)(b << 29)) : (double)__uint_as_float(b);
-        const double x = (top - l) * inv32;
-        const bool live = (uint32_t)__double2hiint(x) < 0x409FFC00u;          // x < 2047
-        if (live) y = x;
-        return live;
-    }
-    // w = 2^(shift - y / 32), all lanes of a warp together: 2^(-k / 32) of the nearest whole k, from its lane, times a polynomial of the rest
-    // (Taylor, |x| <= ln 2 / 64: the first term left out is below 2^-48).  k: the coarse bin.
-    __device__ __forceinline__ double scaled(double y, int &k) const {
-        const double magic = 6755399441055744.0;                              // 1.5 2^52: adding it rounds to a whole number
-        const double t = y + magic;
+    double top, inv32, root;           // inv32: 32 log2(e) / T; root: 2^(shift - lane / 32).  Where the largest logit is +inf: f32's largest number and 0
+    // y = 32 log2(e) (top - l) / T rounded, and behind it what rounding left over; false: the weight is 0
+    __device__ __forceinline__ bool bin(float l, int &k, double &rest) const {
+        const double d = top - (double)fminf(l, 3.402823466e38f);
+        const double t = fma(d, inv32, LG_MAGIC);
+        rest = fma(d, inv32, -(t - LG_MAGIC));
         k = __double2loint(t);
-        const double x = (y - (t - magic)) * -0.02166084939249829;            // -ln 2 / 32
-        double p = fma(x, 1.0 / 120.0, 1.0 / 24.0);
-        p = fma(p, x, 1.0 / 6.0);
-        p = fma(p, x, 0.5);
-        p = fma(p, x, 1.0);
-        p = fma(p, x, 1.0);
-        const int hi = __shfl_sync(0xffffffffu, __double2hiint(root), k & 31), lo = __shfl_sync(0xffffffffu, __double2loint(root), k & 31);
-        return p * __hiloint2double(hi + ((shift - (k >> 5)) << 20), lo);
+        return __double2hiint(t) == 0x43380000 && (uint32_t)k < 2 * LG_SAMPLE_BINS;
     }
-    static __device__ __forceinline__ u64 whole(double s) {                   // to the nearest integer, s < 2^51
-        return (u64)__double_as_longlong(s + 4503599627370496.0) - 0x4330000000000000ull;
+    // 2^(shift - (k + rest) / 32), all lanes of a warp together: the power of the whole number from a lane's root times a polynomial (Taylor in
+    // rest ln 2 / 32, at most ln 2 / 64: the first term left out is below 2^-48)
+    __device__ __forceinline__ double scaled(int k, double rest) const {
+        const double c = 0.02166084939249829;                                 // ln 2 / 32
+        double p = fma(rest, -c * c * c * c * c / 120.0, c * c * c * c / 24.0);
+        p = fma(p, rest, -c * c * c / 6.0);
+        p = fma(p, rest, c * c / 2.0);
+        p = fma(p, rest, -c);
+        p = fma(p, rest, 1.0);
+        const int hi = __shfl_sync(0xffffffffu, __double2hiint(root), k), lo = __shfl_sync(0xffffffffu, __double2loint(root), k);
+        return p * __hiloint2double(hi - (k & ~31) * 32768, lo);
+    }
+    static __device__ __forceinline__ double whole(double s) { return (s + LG_TWO52) - LG_TWO52; }    // to the nearest integer; s < 2^51
+    // of one logit, the same in all lanes: 0 where it has no weight
+    __device__ __forceinline__ double of(float l) const {
+        int k;
+        double rest;
+        const bool live = bin(l, k, rest) && l > -INFINITY;
+        const double x = scaled(k, rest);
+        return live ? x : 0.0;
     }
 };
 
-__device__ __forceinline__ uint32_t ld_peer_u32(uint32_t addr, uint32_t rank) {
-    uint32_t ra, v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(ra) : "memory");
-    return v;
-}
 __device__ __forceinline__ u64 ld_peer_u64(const u64 *p, uint32_t rank) {
     uint32_t ra; u64 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(smem_u32(p)), "r"(rank));
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(ra) : "memory");
     return v;
 }
-__device__ __forceinline__ uint4 ld_peer_u32x4(const uint32_t *p, uint32_t rank) {
-    uint32_t ra; uint4 v;
+__device__ __forceinline__ uint2 ld_peer_u32x2(const uint32_t *p, uint32_t rank) {
+    uint32_t ra; uint2 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(ra) : "memory");
+    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(ra) : "memory");
     return v;
 }
 __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
@@ -154,18 +154,46 @@ template <typename T> struct LgSampler {
     const T *g;                        // the slice in global memory
     T *data;                           // and in shared memory: cap tokens, the last ones filled up with NaN
     uint32_t *hist;                    // two histograms of `limbs` arrays, used in turn
+    float *lv; int *li;                // this warp's list: logits, places in the slice; -inf behind the last
     u64 *word;                         // words for the other CTAs: a place per exchange
-    u64 *red;                          // [2 * warps] and more, block-wide
+    u64 *red;                          // block-wide
     int n, first, ranks, rank, lane, warp, turn = 0, at_word = 0;             // tokens here, index of the first
-    int w0, w1;                        // this warp's tokens
+    int w0, w1;                        // this warp's tokens: places in the slice, or 0 .. of its list
+    bool listed = false;
     LgWeight w;
 
-    __device__ __forceinline__ void fetch4(int i, uint32_t (&b)[4]) const {
-        if (i + 4 <= a.cap) L::bits4(data + i, b);
+    // four tokens a lane from place i on
+    __device__ __forceinline__ void fetch4(int i, float (&l)[4]) const {
+        if (listed) { const float4 v = *(const float4 *)(lv + i); l[0] = v.x; l[1] = v.y; l[2] = v.z; l[3] = v.w; }
+        else if (i + 4 <= a.cap) L::value4(data + i, l);
         else {
             #pragma unroll
-            for (int j = 0; j < 4; j++) b[j] = i + j < n ? i + j < a.cap ? L::bits(data + i + j) : L::bits(g + i + j) : LG_NAN_BITS;
+            for (int j = 0; j < 4; j++) l[j] = i + j < n ? i + j < a.cap ? L::value(data + i + j) : L::value(g + i + j) : -INFINITY;
         }
+    }
+    // This warp's tokens of at least `least` into its list, in their order, where they fit
+    __device__ void make_list(float least) {
+        if (listed) return;
+        int count = 0;
+        for (int i = w0; i < w1; i += 128) {
+            float l[4];
+            fetch4(i + lane * 4, l);
+            const bool in[4] = {l[0] >= least, l[1] >= least, l[2] >= least, l[3] >= least};
+            if (!__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) continue;
+            int at = count;
+            #pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t m = __ballot_sync(0xffffffffu, in[j]);
+                at += __popc(m & ((1u << lane) - 1));
+                count += __popc(m);
+            }
+            if (count > LG_SAMPLE_LIST) return;
+            #pragma unroll
+            for (int j = 0; j < 4; j++) if (in[j]) { lv[at] = l[j]; li[at++] = i + lane * 4 + j; }
+        }
+        for (int i = count + lane; i < LG_SAMPLE_LIST; i += 32) lv[i] = -INFINITY;
+        __syncwarp();
+        listed = true; w0 = 0; w1 = count;
     }
     // Sums of two numbers a thread over the cluster; each CTA's own sums are left in own[0], own[1]
     __device__ void sum2(u64 x, u64 y, u64 &sx, u64 &sy) {
@@ -197,31 +225,31 @@ template <typename T> struct LgSampler {
         if (const uint32_t v = (uint32_t)(x >> 15) & 0x7FFFu) atomicAdd(h + LG_SAMPLE_BINS + bin, v);
         if (const uint32_t v = (uint32_t)(x >> 30)) atomicAdd(h + 2 * LG_SAMPLE_BINS + bin, v);
     }
-    // This thread's four bins, summed over the cluster
-    __device__ __forceinline__ void bins4(const uint32_t *h, int limbs, u64 (&v)[4]) const {
-        v[0] = v[1] = v[2] = v[3] = 0;
+    // This thread's two bins, summed over the cluster
+    __device__ __forceinline__ void bins2(const uint32_t *h, int limbs, u64 (&v)[2]) const {
+        v[0] = v[1] = 0;
         for (int l = 0; l < limbs; l++)
+            #pragma unroll 4
             for (int c = 0; c < ranks; c++) {
-                const uint4 x = ld_peer_u32x4(h + l * LG_SAMPLE_BINS + threadIdx.x * 4, c);
-                v[0] += (u64)x.x << 15 * l; v[1] += (u64)x.y << 15 * l; v[2] += (u64)x.z << 15 * l; v[3] += (u64)x.w << 15 * l;
+                const uint2 x = ld_peer_u32x2(h + l * LG_SAMPLE_BINS + threadIdx.x * 2, c);
+                v[0] += (u64)x.x << 15 * l; v[1] += (u64)x.y << 15 * l;
             }
     }
     // The first bin at which before + the running sum of v reaches the target, and the sum before it; the last bin where none does (found = false).
     // `slot` keeps two results of one call apart.
-    __device__ bool first_reaching(const u64 (&v)[4], u64 before, u64 target, int slot, int &bin, u64 &sum) {
-        const u64 mine = v[0] + v[1] + v[2] + v[3], incl = warp_scan_u64(mine, lane);
+    __device__ bool first_reaching(const u64 (&v)[2], u64 before, u64 target, int slot, int &bin, u64 &sum) {
+        const u64 mine = v[0] + v[1], incl = warp_scan_u64(mine, lane);
         __syncthreads();
         if (lane == 31) red[warp] = incl;
         if (threadIdx.x == 0) red[2 * LG_SAMPLE_WARPS + slot] = ~0ull;
         __syncthreads();
-        u64 at = before + incl - mine, all = before;
-        #pragma unroll
-        for (int i = 0; i < LG_SAMPLE_WARPS; i++) { if (i < warp) at += red[i]; all += red[i]; }
+        const u64 ws = lane < LG_SAMPLE_WARPS ? red[lane] : 0, wi = warp_scan_u64(ws, lane);
+        u64 at = before + incl - mine + __shfl_sync(0xffffffffu, wi - ws, warp);
+        const u64 all = before + __shfl_sync(0xffffffffu, wi, 31);
         if (at < target && target <= at + mine) {
-            int j = 0;
-            while (at + v[j] < target) at += v[j++];
-            red[2 * LG_SAMPLE_WARPS + slot] = threadIdx.x * 4 + j;
-            red[2 * LG_SAMPLE_WARPS + 2 + slot] = at;
+            const bool second = at + v[0] < target;
+            red[2 * LG_SAMPLE_WARPS + slot] = threadIdx.x * 2 + second;
+            red[2 * LG_SAMPLE_WARPS + 2 + slot] = second ? at + v[0] : at;
         }
         __syncthreads();
         const u64 b = red[2 * LG_SAMPLE_WARPS + slot];
@@ -230,68 +258,64 @@ template <typename T> struct LgSampler {
         sum = found ? red[2 * LG_SAMPLE_WARPS + 2 + slot] : all;
         return found;
     }
-    // Keys of the bins b0 .. b1 of the coarse histogram, a bin more on either side
+    // Keys of the coarse bins b0 .. b1 with room on either side, within low .. top_key
     __device__ void interval(int b0, int b1, uint32_t low, uint32_t top_key, uint32_t &klo, uint32_t &khi) const {
         klo = low; khi = top_key;
-        if (w.inf || !(w.inv32 > 0.0)) return;
-        const double lo = w.top - (b1 + 1) / w.inv32, hi = w.top - (b0 - 1) / w.inv32;
-        klo = max(low, key_below<LOW>(lo));
-        khi = min(top_key, key_above<LOW>(hi));
+        if (!(w.inv32 > 0.0)) return;
+        klo = max(low, key_of<LOW>(__double2float_rd(w.top - (2 * b1 + 2) / w.inv32)));
+        khi = min(top_key, key_of<LOW>(__double2float_ru(w.top - (2 * b0 - 1) / w.inv32)));
     }
-    // The threshold at which counts (weighted: weights) of the keys from the largest down reach the target; it lies in klo .. khi, and all keys
-    // in question are above `floor_key`.  Kept then: keys above t and `ties` of key t.
+    // The threshold at which counts (weighted: weights) of the keys from the largest down reach the target; it lies in klo .. khi.  Kept then: keys
+    // above t and `ties` of key t.
     __device__ void refine(bool weighted, u64 target, uint32_t klo, uint32_t khi, uint32_t &t, u64 &ties) {
         u64 above = 0;
-        for (int round = 0; round < 3; round++) {                             // 11 bits of at most 32 a round
-            const bool begin = round == 0;
+        for (int round = 0; round < 4; round++) {                             // 10 bits of at most 32 a round
             const uint32_t range = khi - klo;
-            const int sh = range >= LG_SAMPLE_BINS ? 21 - __clz(range) : 0;    // range >> sh < 2048
+            const int sh = range >= LG_SAMPLE_BINS ? 22 - __clz(range) : 0;    // range >> sh < 1024
+            const float lo = key_value<LOW>(klo), hi = key_value<LOW>(khi), over_hi = round ? INFINITY : hi;
             uint32_t *h = fresh_hist(weighted ? 3 : 1);
-            u64 over = 0;
+            u64 count = 0;
+            double over = 0.0;
             for (int i = w0; i < w1; i += 128) {
-                uint32_t b[4];
-                fetch4(i + lane * 4, b);
+                float l[4];
+                fetch4(i + lane * 4, l);
                 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const uint32_t k = key_of<LOW>(b[j]);
-                    const bool in = k >= klo && k <= khi, more = begin && k > khi;
+                    const bool in = l[j] >= lo && l[j] <= hi, more = l[j] > over_hi;
+                    if (!__any_sync(0xffffffffu, in || more)) continue;
+                    const int part = (int)((khi - key_of<LOW>(l[j])) >> sh);
                     if (weighted) {
-                        if (!__any_sync(0xffffffffu, in || more)) continue;
-                        double y;
-                        int bin;
-                        const bool live = w.arg(b[j], y);
-                        const u64 x = LgWeight::whole(w.scaled(y, bin));
+                        int k;
+                        double rest;
+                        const bool live = w.bin(l[j], k, rest);
+                        const double x = LgWeight::whole(w.scaled(k, rest));
                         if (live && more) over += x;
-                        if (live && in) add_weight(h, (khi - k) >> sh, x);
+                        if (live && in) add_weight(h, part, (u64)(long long)x);
                     } else {
-                        if (more) over++;
-                        if (in) atomicAdd(h + ((khi - k) >> sh), 1u);
+                        count += more;
+                        if (in) atomicAdd(h + part, 1u);
                     }
                 }
             }
-            if (begin) { u64 none; sum2(over, 0, above, none); }               // (its barrier also makes the histograms complete)
+            if (round == 0) { u64 none; sum2(weighted ? (u64)(long long)over : count, 0, above, none); }   // (its barrier also makes the histograms complete)
             else cluster_sync_all();
-            u64 v[4];
-            int bin;
-            bins4(h, weighted ? 3 : 1, v);
-            first_reaching(v, above, target, 0, bin, above);
-            // `above` is now what lies above the part `bin`
-            khi -= (uint32_t)bin << sh;
+            u64 v[2];
+            int part;
+            bins2(h, weighted ? 3 : 1, v);
+            first_reaching(v, above, target, 0, part, above);                 // `above`: of what lies above the part from now on
+            khi -= (uint32_t)part << sh;
             klo = max(klo, khi - ((1u << sh) - 1) > khi ? 0u : khi - ((1u << sh) - 1));
             if (sh == 0) break;
         }
         t = khi;
         if (!weighted) { ties = target - above; return; }
-        double y;
-        int bin;
-        const bool live = w.arg(key_bits<LOW>(t), y);
-        const u64 one = LgWeight::whole(w.scaled(y, bin));
-        ties = live && one ? (target - above + one - 1) / one : 1;
+        const u64 one = (u64)(long long)LgWeight::whole(w.of(key_value<LOW>(t)));
+        ties = one ? (target - above + one - 1) / one : 1;
     }
 };
 
 // grid: rows x ranks, clusters of `ranks` CTAs
-template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS) lg_sample_kernel(LgSampleArgs a) {
+template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg_sample_kernel(LgSampleArgs a) {
     extern __shared__ __align__(16) unsigned char lg_sample_sm[];
     __shared__ u64 word[48], red[2 * LG_SAMPLE_WARPS + 4];
     typedef LogitType<T> L;
@@ -304,166 +328,180 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS) lg_sa
     s.g = (const T *)a.logits + (long long)row * a.ld + first;
     s.data = (T *)lg_sample_sm;
     s.hist = (uint32_t *)(lg_sample_sm + (size_t)a.cap * sizeof(T));
+    s.lv = (float *)(s.hist + 2 * a.limbs * LG_SAMPLE_BINS) + warp * LG_SAMPLE_LIST * 2; s.li = (int *)(s.lv + LG_SAMPLE_LIST);
     s.word = word; s.red = red; s.n = n; s.first = first; s.ranks = ranks; s.rank = rank; s.lane = lane; s.warp = warp;
     const int per = ((a.slice + LG_SAMPLE_WARPS - 1) / LG_SAMPLE_WARPS + 127) / 128 * 128;
     s.w0 = min(warp * per, n); s.w1 = min(s.w0 + per, n);
     const float T1 = a.temperature ? a.temperature[row] : 1.0f, top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f;
     const int top_k = a.top_k ? a.top_k[row] : 0;
 
-    // the row, once: into shared memory, and its largest logit with its first place
-    u64 best = 0;
-    auto seen = [&](uint32_t b, int i) {
-        const u64 k = (u64)key_of<LOW>(b) << 32 | (uint32_t)~(first + i);
-        best = k > best ? k : best;
-    };
+    // the row, once: into shared memory, and its largest logit
+    float best = -INFINITY;
     {
         constexpr int V = 16 / sizeof(T);
         const int held = min(n, a.cap), vec = ((uintptr_t)s.g & 15) ? 0 : held / V * V;
+        uint32_t m = L::lowest();
         for (int i = tid * V; i < vec; i += LG_SAMPLE_THREADS * V * 4) {
             uint4 v[4];
             #pragma unroll
-            for (int q = 0; q < 4; q++) if (i + q * LG_SAMPLE_THREADS * V < vec) v[q] = ldg_stream16((const uint4 *)(s.g + i + q * LG_SAMPLE_THREADS * V));
+            for (int q = 0; q < 4; q++) {
+                const int at = i + q * LG_SAMPLE_THREADS * V;
+                v[q] = make_uint4(L::lowest(), L::lowest(), L::lowest(), L::lowest());
+                if (at < vec) v[q] = ldg_stream16((const uint4 *)(s.g + at));
+            }
             #pragma unroll
             for (int q = 0; q < 4; q++) {
                 const int at = i + q * LG_SAMPLE_THREADS * V;
-                if (at < vec) {
-                    *(uint4 *)(s.data + at) = v[q];
-                    uint32_t b[4];
-                    #pragma unroll
-                    for (int h = 0; h < V / 4; h++) {
-                        L::bits4((const T *)&v[q] + 4 * h, b);
-                        #pragma unroll
-                        for (int j = 0; j < 4; j++) seen(b[j], at + 4 * h + j);
-                    }
-                }
+                if (at < vec) *(uint4 *)(s.data + at) = v[q];
+                m = L::larger(L::larger(m, L::larger(v[q].x, v[q].y)), L::larger(v[q].z, v[q].w));
             }
         }
-        for (int i = vec + tid; i < held; i += LG_SAMPLE_THREADS) { const T x = s.g[i]; s.data[i] = x; seen(L::bits(&x), i); }
+        best = L::most(m);
+        for (int i = vec + tid; i < held; i += LG_SAMPLE_THREADS) { const T x = s.g[i]; s.data[i] = x; best = fmaxf(best, L::value(&x)); }
         for (int i = held + tid; i < a.cap; i += LG_SAMPLE_THREADS) ((uint16_t *)s.data)[i * (sizeof(T) / 2) + sizeof(T) / 2 - 1] = 0x7FFF;      // NaN in any of the types
-        for (int i = held + tid; i < n; i += LG_SAMPLE_THREADS) seen(L::bits(s.g + i), i);
+        for (int i = held + tid; i < n; i += LG_SAMPLE_THREADS) best = fmaxf(best, L::value(s.g + i));
     }
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { const u64 t = __shfl_xor_sync(0xffffffffu, best, o); best = t > best ? t : best; }
-    if (lane == 0) red[warp] = best;
+    best = warp_max(best);
+    if (lane == 0) red[warp] = __float_as_uint(best);
     __syncthreads();
     if (warp == 0) {
-        best = lane < LG_SAMPLE_WARPS ? red[lane] : 0;
-        #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) { const u64 t = __shfl_xor_sync(0xffffffffu, best, o); best = t > best ? t : best; }
-        if (lane == 0) word[0] = best;
+        best = warp_max(lane < LG_SAMPLE_WARPS ? __uint_as_float((uint32_t)red[lane]) : -INFINITY);
+        if (lane == 0) word[0] = __float_as_uint(best);
     }
     cluster_sync_all();
-    best = 0;
-    for (uint32_t c = 0; c < ranks; c++) { const u64 t = ld_peer_u64(word, c); best = t > best ? t : best; }
+    for (uint32_t c = 0; c < ranks; c++) best = fmaxf(best, __uint_as_float((uint32_t)ld_peer_u64(word, c)));
     s.at_word = 1;
-    const uint32_t top_key = (uint32_t)(best >> 32);
-    if (top_key <= LgSampler<T>::DEAD || !(T1 > 0.0f) || top_k == 1 || top_p <= 0.0f || min_p > 1.0f) {
+    if (best == -INFINITY || !(T1 > 0.0f) || top_k == 1 || top_p <= 0.0f || min_p > 1.0f) {
+        // nothing to draw, or the first token of the order: the lowest place of the largest logit
+        u64 place = ~0ull;
+        if (best > -INFINITY)
+            for (int i = s.w0; i < s.w1; i += 128) {
+                float l[4];
+                s.fetch4(i + lane * 4, l);
+                #pragma unroll
+                for (int j = 3; j >= 0; j--) if (l[j] == best) place = min(place, (u64)(first + i + lane * 4 + j));
+            }
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) place = min(place, (u64)__shfl_xor_sync(0xffffffffu, place, o));
+        __syncthreads();
+        if (lane == 0) red[warp] = place;
+        __syncthreads();
+        if (tid == 0) {
+            for (int i = 1; i < LG_SAMPLE_WARPS; i++) place = min(place, red[i]);
+            word[1] = place;
+        }
+        cluster_sync_all();
         if (rank == 0 && tid == 0) {
-            const bool none = top_key <= LgSampler<T>::DEAD;
-            a.token[row] = none ? -1 : (int)~(uint32_t)best;
-            if (a.prob) a.prob[row] = none ? 0.0f : 1.0f;
+            for (uint32_t c = 1; c < ranks; c++) place = min(place, ld_peer_u64(word + 1, c));
+            a.token[row] = place == ~0ull ? -1 : (int)place;
+            if (a.prob) a.prob[row] = place == ~0ull ? 0.0f : 1.0f;
         }
         cluster_sync_all();                             // no CTA leaves while another reads its words
         return;
     }
-    const uint32_t top_bits = key_bits<LOW>(top_key);
-    s.w.inf = top_bits == 0x7F800000u;
-    s.w.top = (double)__uint_as_float(top_bits); s.w.inv32 = 46.166241308446828 / (double)T1; s.w.root = exp2(-lane / 32.0); s.w.shift = a.shift;
+    const uint32_t top_key = key_of<LOW>(best);
+    s.w.top = (double)fminf(best, 3.402823466e38f); s.w.inv32 = best == INFINITY ? 0.0 : 46.166241308446828 / (double)T1; s.w.root = exp2(a.shift - lane / 32.0);
 
-    uint32_t t = LgSampler<T>::DEAD;                    // threshold; at first everything above -inf
+    uint32_t t = best == INFINITY ? top_key - 1 : LgSampler<T>::DEAD;          // threshold; at first everything above -inf
     u64 ties = 0;
     if (top_k > 0 && top_k < a.vocab) {
         uint32_t *h = s.fresh_hist(1);
+        const float lt = key_value<LOW>(t);
         for (int i = s.w0; i < s.w1; i += 128) {
-            uint32_t b[4];
-            s.fetch4(i + lane * 4, b);
+            float l[4];
+            s.fetch4(i + lane * 4, l);
             #pragma unroll
             for (int j = 0; j < 4; j++) {
-                double y;
-                if (s.w.arg(b[j], y)) atomicAdd(h + __double2loint(y + 6755399441055744.0), 1u);
+                int k;
+                double rest;
+                if (s.w.bin(l[j], k, rest) && l[j] > lt) atomicAdd(h + (k >> 1), 1u);
             }
         }
         cluster_sync_all();
-        u64 v[4], before;
+        u64 v[2], before;
         int bin;
-        s.bins4(h, 1, v);
+        s.bins2(h, 1, v);
         if (s.first_reaching(v, 0, (u64)top_k, 0, bin, before)) {              // otherwise fewer than top_k tokens have a weight
             uint32_t klo, khi;
-            s.interval(bin, bin, LgSampler<T>::DEAD + 1, top_key, klo, khi);
+            s.interval(bin, bin, t + 1, top_key, klo, khi);
+            s.make_list(key_value<LOW>(klo));
             s.refine(false, (u64)top_k, klo, khi, t, ties);
         }
     }
     if (top_p < 1.0f) {
         // weight above the threshold, tokens at it
         uint32_t *h = s.fresh_hist(1);
-        u64 over = 0, at_t = 0;
+        const float lt = key_value<LOW>(t);
+        double sum = 0.0;
+        u64 over, at_t;
+        uint32_t n_at = 0;
         for (int i = s.w0; i < s.w1; i += 128) {
-            uint32_t b[4];
-            s.fetch4(i + lane * 4, b);
+            float l[4];
+            s.fetch4(i + lane * 4, l);
             #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const uint32_t k = key_of<LOW>(b[j]);
-                at_t += k == t;
-                if (!__any_sync(0xffffffffu, k > t)) continue;
-                double y;
-                int bin;
-                const bool live = s.w.arg(b[j], y);
-                const u64 x = LgWeight::whole(s.w.scaled(y, bin));
-                if (live && k > t) { over += x; atomicAdd(h + bin, 1u); }
+                const bool in = l[j] > lt;
+                if (ties) n_at += l[j] == lt;
+                if (!__any_sync(0xffffffffu, in)) continue;
+                int k;
+                double rest;
+                const bool live = s.w.bin(l[j], k, rest);
+                const double x = LgWeight::whole(s.w.scaled(k, rest));
+                if (live && in) { sum += x; atomicAdd(h + (k >> 1), 1u); }
             }
         }
-        s.sum2(over, at_t, over, at_t);
-        double y;
-        int bin;
-        const bool live = s.w.arg(key_bits<LOW>(t), y);
-        u64 one = LgWeight::whole(s.w.scaled(y, bin));
-        if (!live) one = 0;
+        s.sum2((u64)(long long)sum, n_at, over, at_t);
+        const u64 one = (u64)(long long)LgWeight::whole(s.w.of(lt));
         if (ties < at_t) at_t = ties;
         const u64 total = over + at_t * one, p64 = __double2ull_rz((double)top_p * 18446744073709551616.0);
         u64 target = __umul64hi(p64, total) + (p64 * total != 0);
         if (target < 1) target = 1;
         if (target > over) ties = min(ties, one ? (target - over + one - 1) / one : ties);
         else {
-            // weights of a bin: between those of its borders, half a bin to either side of its number
-            u64 c[4], v[4], before;
+            // the weights of a bin lie between those of its borders: half a step above its first number, half a step below its second
+            u64 c[2], v[2], before;
             int b0, b1;
-            s.bins4(h, 1, c);
+            double edge[2];
+            s.bins2(h, 1, c);
             #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = c[j] ? c[j] * (u64)__double2ull_ru(exp2(a.shift - (tid * 4 + j - 0.51) / 32.0)) : 0;
+            for (int j = 0; j < 2; j++) {
+                edge[j] = s.w.scaled(4 * tid + 2 * j, 0.0);
+                v[j] = c[j] * (u64)__double2ull_ru(edge[j] * 1.0111);         // 2^(0.51 / 32) = 1.01111
+            }
             s.first_reaching(v, 0, target, 0, b0, before);
             #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = c[j] ? c[j] * (u64)__double2ull_rd(exp2(a.shift - (tid * 4 + j + 0.51) / 32.0)) : 0;
+            for (int j = 0; j < 2; j++) v[j] = c[j] * (u64)__double2ull_rd(edge[j] * 0.9678);     // 2^(-1.51 / 32) = 0.96782
             s.first_reaching(v, 0, target, 1, b1, before);
             uint32_t klo, khi;
             s.interval(b0, max(b0, b1), t + 1, top_key, klo, khi);
+            s.make_list(key_value<LOW>(klo));
             s.refine(true, target, klo, khi, t, ties);
         }
     }
     // the draw: what each warp's tokens weigh and how many lie at the threshold, then the warp in which the running weight passes the target
     const double floor_w = min_p > 0.0f ? (double)min_p * (double)(1ull << a.shift) : 0.0;
-    u64 over = 0, at_t = 0, one;
-    {
-        double y;
-        int bin;
-        const bool live = s.w.arg(key_bits<LOW>(t), y);
-        const double x = s.w.scaled(y, bin);
-        one = live && x >= floor_w ? LgWeight::whole(x) : 0;
-    }
+    const float lt = key_value<LOW>(t);
+    const double x_t = s.w.of(lt);
+    const u64 one = x_t >= floor_w ? (u64)(long long)LgWeight::whole(x_t) : 0;
+    double sum = 0.0;
+    u64 over, at_t;
+    uint32_t n_at = 0;
     for (int i = s.w0; i < s.w1; i += 128) {
-        uint32_t b[4];
-        s.fetch4(i + lane * 4, b);
+        float l[4];
+        s.fetch4(i + lane * 4, l);
         #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const uint32_t k = key_of<LOW>(b[j]);
-            at_t += k == t;
-            if (!__any_sync(0xffffffffu, k > t)) continue;
-            double y;
-            int bin;
-            const bool live = s.w.arg(b[j], y) && k > t;
-            const double x = s.w.scaled(y, bin);
-            if (live && x >= floor_w) over += LgWeight::whole(x);
+            const bool in = l[j] > lt;
+            if (ties) n_at += l[j] == lt;
+            if (!__any_sync(0xffffffffu, in)) continue;
+            int k;
+            double rest;
+            const bool live = s.w.bin(l[j], k, rest);
+            const double x = s.w.scaled(k, rest);
+            if (live && in && x >= floor_w) sum += LgWeight::whole(x);
         }
     }
+    over = (u64)(long long)sum; at_t = n_at;
     over = warp_sum_u64(over); at_t = warp_sum_u64(at_t);
     __syncthreads();
     if (lane == 0) { red[warp] = over; red[LG_SAMPLE_WARPS + warp] = at_t; }
@@ -496,19 +534,19 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS) lg_sa
     const u64 target = __umul64hi(u64_, total);
     if (run <= target && target < end) {
         for (int i = s.w0; i < s.w1; i += 128) {
-            uint32_t b[4], eq = 0;
+            float l[4];
+            uint32_t eq = 0;
             double x[4];
             u64 v[4], sum = 0;
-            s.fetch4(i + lane * 4, b);
+            s.fetch4(i + lane * 4, l);
             #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const uint32_t k = key_of<LOW>(b[j]);
-                double y;
-                int bin;
-                const bool live = s.w.arg(b[j], y);
-                x[j] = s.w.scaled(y, bin);
-                v[j] = live && k > t && x[j] >= floor_w ? LgWeight::whole(x[j]) : 0;
-                eq |= (uint32_t)(k == t) << j;
+                int k;
+                double rest;
+                const bool live = s.w.bin(l[j], k, rest);
+                x[j] = s.w.scaled(k, rest);
+                v[j] = live && l[j] > lt && x[j] >= floor_w ? (u64)(long long)LgWeight::whole(x[j]) : 0;
+                eq |= (uint32_t)(l[j] == lt) << j;
             }
             const u64 ties_up = warp_scan_u64(__popc(eq), lane);
             u64 rk = rank_t + ties_up - __popc(eq);
@@ -524,7 +562,7 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS) lg_sa
                     u64 at = run + up - sum;
                     int j = 0;
                     while (at + v[j] <= target) at += v[j++];
-                    a.token[row] = first + i + lane * 4 + j;
+                    a.token[row] = first + (s.listed ? s.li[i + lane * 4 + j] : i + lane * 4 + j);
                     if (a.prob) a.prob[row] = (float)(x[j] / (double)total);
                 }
                 break;

@@ -231,25 +231,40 @@ extern "C" int lg_paged_attn(const struct lg_paged_cache *c, const void *d_q, in
 }
 
 namespace {
-// CTAs that share a row: as many as it takes to hold it in shared memory, more while there are fewer CTAs than SMs and each still has
-// 4096 tokens; at most 8, the largest cluster that every device places.
+// CTAs that share a row: as many as it takes to hold it in shared memory with two CTAs per SM, more while they do not fill the SMs twice and
+// each still has 4096 tokens (a row's time goes with the passes over a CTA's tokens; below that the barriers are the larger part).
 template <typename T> int launch_sample(LgSampleArgs &a, int dev, void *stream) {
-    const int sms = device_sms(dev), hist = 2 * a.limbs * LG_SAMPLE_BINS * 4, room = 220 * 1024 - hist;
-    int ranks = 1;
-    while (ranks < LG_SAMPLE_MAX_CLUSTER && ((long long)(a.vocab + ranks - 1) / ranks * (int)sizeof(T) > room ||
-                                             ((long long)a.rows * ranks * 2 <= sms && a.vocab / (ranks * 2) >= 4096))) ranks *= 2;
-    a.slice = ((a.vocab + ranks - 1) / ranks + 127) / 128 * 128;
-    const long long most = room / sizeof(T) / 128 * 128;
-    a.cap = (int)(a.slice < most ? a.slice : most);
-    const size_t smem = (size_t)a.cap * sizeof(T) + hist;
-    static unsigned char done[64];
-    if (!allow_smem(lg_sample_kernel<T>, smem, 220 * 1024, dev, done)) SERVE_FAIL(-6, "lg_sample: no %zu bytes of shared memory", smem);
+    static unsigned char done[64], most_ranks[64];
+    const int sms = device_sms(dev), tools = a.limbs ? 2 * a.limbs * LG_SAMPLE_BINS * 4 + LG_SAMPLE_WARPS * LG_SAMPLE_LIST * 8 : 0, room = 112 * 1024 - tools;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)a.rows * ranks); cfg.blockDim = dim3(LG_SAMPLE_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ranks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(LG_SAMPLE_THREADS); cfg.stream = (cudaStream_t)stream;
     cfg.attrs = at; cfg.numAttrs = 1;
+    if (dev >= 64 || !done[dev]) {
+        if (cudaFuncSetAttribute(lg_sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024) != cudaSuccess) {
+            cudaGetLastError();
+            SERVE_FAIL(-6, "lg_sample: no %d bytes of shared memory", 112 * 1024);
+        }
+        int ranks = 8, n = 0;                                                 // what every device places; 16 where this one does
+        at[0].val.clusterDim.x = LG_SAMPLE_MAX_CLUSTER;
+        cfg.gridDim = dim3(LG_SAMPLE_MAX_CLUSTER); cfg.dynamicSmemBytes = 112 * 1024;
+        if (cudaFuncSetAttribute(lg_sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+            cudaOccupancyMaxActiveClusters(&n, lg_sample_kernel<T>, &cfg) == cudaSuccess && n > 0) ranks = LG_SAMPLE_MAX_CLUSTER;
+        cudaGetLastError();
+        most_ranks[dev & 63] = (unsigned char)ranks;
+        if (dev < 64) done[dev] = 1;
+    }
+    const int most = most_ranks[dev & 63];
+    int ranks = 1;
+    while (ranks < most && ((long long)(a.vocab + ranks - 1) / ranks * (int)sizeof(T) > room || ((long long)a.rows * ranks <= sms && a.vocab / (ranks * 2) >= 4096))) ranks *= 2;
+    a.slice = ((a.vocab + ranks - 1) / ranks + 127) / 128 * 128;
+    const long long held = room / (int)sizeof(T) / 128 * 128;
+    a.cap = (int)(a.slice < held ? a.slice : held);
+    cfg.dynamicSmemBytes = (size_t)a.cap * sizeof(T) + tools;
+    cfg.gridDim = dim3((unsigned)a.rows * ranks);
+    at[0].val.clusterDim.x = ranks;
     const cudaError_t rc = cudaLaunchKernelEx(&cfg, lg_sample_kernel<T>, a);
     if (rc != cudaSuccess) { cudaGetLastError(); SERVE_FAIL(-6, "lg_sample: launch failed: %s", cudaGetErrorString(rc)); }
     return 0;

@@ -13,7 +13,8 @@
 //           threshold can lie in, and with them an interval of logits
 //   list    each warp notes its tokens in or above that interval, where they are few; later passes read the list
 //   fine    exact counts or weights over 1024 equal parts of that interval of keys (the logits as ordered integers), then of the part that holds the threshold,
-//           until a part is a single key: at most four rounds
+//           until a part is a single key: at most four rounds.  Where the lists hold the interval, every CTA fetches its tokens and does the rounds alone;
+//           otherwise (flat rows) the histograms of a round are added up over the cluster
 // Bound by the instructions of a pass over the row (about 30 a token and weight, 11 of them 64-bit arithmetic) and, for few rows, by the cluster barriers.
 #pragma once
 #include "lg_device.cuh"
@@ -22,7 +23,9 @@
 #define LG_SAMPLE_THREADS 512
 #define LG_SAMPLE_WARPS (LG_SAMPLE_THREADS / 32)
 #define LG_SAMPLE_BINS 1024            // two a thread
-#define LG_SAMPLE_LIST 128             // tokens a warp's list holds
+#define LG_SAMPLE_LIST 96              // tokens a warp's list holds
+#define LG_SAMPLE_NEAR 256             // of these, tokens of a CTA whose place at a threshold is open
+#define LG_SAMPLE_TOOLS (LG_SAMPLE_WARPS * LG_SAMPLE_LIST * 8 + LG_SAMPLE_BINS * 8 + LG_SAMPLE_NEAR * 4)
 #define LG_SAMPLE_MAX_CLUSTER 16
 
 typedef unsigned long long u64;
@@ -127,15 +130,20 @@ __device__ __forceinline__ u64 ld_peer_u64(const u64 *p, uint32_t rank) {
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(ra) : "memory");
     return v;
 }
-__device__ __forceinline__ uint2 ld_peer_u32x2(const uint32_t *p, uint32_t rank) {
-    uint32_t ra; uint2 v;
+__device__ __forceinline__ uint32_t ld_peer_u32(const uint32_t *p, uint32_t rank) {
+    uint32_t ra, v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(ra) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(ra) : "memory");
     return v;
 }
 __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
     #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ u64 warp_half_sum_u64(u64 v) {
+    #pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 // Inclusive sum over the lanes
@@ -155,6 +163,7 @@ template <typename T> struct LgSampler {
     T *data;                           // and in shared memory: cap tokens, the last ones filled up with NaN
     uint32_t *hist;                    // two histograms of `limbs` arrays, used in turn
     float *lv; int *li;                // this warp's list: logits, places in the slice; -inf behind the last
+    u64 *fine; uint32_t *near;         // histogram of this CTA alone; keys of its tokens in an interval
     u64 *word;                         // words for the other CTAs: a place per exchange
     u64 *red;                          // block-wide
     int n, first, ranks, rank, lane, warp, turn = 0, at_word = 0;             // tokens here, index of the first
@@ -164,12 +173,24 @@ template <typename T> struct LgSampler {
 
     // four tokens a lane from place i on
     __device__ __forceinline__ void fetch4(int i, float (&l)[4]) const {
-        if (listed) { const float4 v = *(const float4 *)(lv + i); l[0] = v.x; l[1] = v.y; l[2] = v.z; l[3] = v.w; }
+        if (listed) {
+            float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (i < LG_SAMPLE_LIST) v = *(const float4 *)(lv + i);
+            l[0] = v.x; l[1] = v.y; l[2] = v.z; l[3] = v.w;
+        }
         else if (i + 4 <= a.cap) L::value4(data + i, l);
         else {
             #pragma unroll
             for (int j = 0; j < 4; j++) l[j] = i + j < n ? i + j < a.cap ? L::value(data + i + j) : L::value(g + i + j) : -INFINITY;
         }
+    }
+    // Four tokens' bins and weights side by side; in: above lt and with a weight
+    __device__ __forceinline__ void weigh4(const float (&l)[4], float lt, int (&k)[4], double (&x)[4], bool (&in)[4]) const {
+        double rest[4];
+        #pragma unroll
+        for (int j = 0; j < 4; j++) in[j] = w.bin(l[j], k[j], rest[j]) && l[j] > lt;
+        #pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = w.scaled(k[j], rest[j]);
     }
     // This warp's tokens of at least `least` into its list, in their order, where they fit
     __device__ void make_list(float least) {
@@ -195,8 +216,8 @@ template <typename T> struct LgSampler {
         __syncwarp();
         listed = true; w0 = 0; w1 = count;
     }
-    // Sums of two numbers a thread over the cluster; each CTA's own sums are left in own[0], own[1]
-    __device__ void sum2(u64 x, u64 y, u64 &sx, u64 &sy) {
+    // Sums of two numbers a thread over the cluster; `at` (or NULL): the place of the CTAs' own sums
+    __device__ void sum2(u64 x, u64 y, u64 &sx, u64 &sy, const u64 **at = nullptr) {
         x = warp_sum_u64(x); y = warp_sum_u64(y);
         __syncthreads();
         if (lane == 0) { red[warp] = x; red[LG_SAMPLE_WARPS + warp] = y; }
@@ -204,13 +225,13 @@ template <typename T> struct LgSampler {
         u64 *p = word + at_word;
         at_word += 2;
         if (warp == 0) {
-            x = lane < LG_SAMPLE_WARPS ? red[lane] : 0; y = lane < LG_SAMPLE_WARPS ? red[LG_SAMPLE_WARPS + lane] : 0;
-            x = warp_sum_u64(x); y = warp_sum_u64(y);
-            if (lane == 0) { p[0] = x; p[1] = y; }
+            const u64 v = warp_half_sum_u64(red[lane]);                       // 16 warps: x in the lower half of the lanes, y in the upper
+            if ((lane & 15) == 0) p[lane >> 4] = v;
         }
         cluster_sync_all();
-        sx = sy = 0;
-        for (int c = 0; c < ranks; c++) { sx += ld_peer_u64(p, c); sy += ld_peer_u64(p + 1, c); }
+        const u64 v = warp_half_sum_u64((lane & 15) < ranks ? ld_peer_u64(p + (lane >> 4), lane & 15) : 0);
+        sx = __shfl_sync(0xffffffffu, v, 0); sy = __shfl_sync(0xffffffffu, v, 16);
+        if (at) *at = p;
     }
     // An empty histogram (block-wide; the cluster has passed a barrier since the one before it was read)
     __device__ uint32_t *fresh_hist(int limbs) {
@@ -224,16 +245,6 @@ template <typename T> struct LgSampler {
         if (const uint32_t v = (uint32_t)x & 0x7FFFu) atomicAdd(h + bin, v);
         if (const uint32_t v = (uint32_t)(x >> 15) & 0x7FFFu) atomicAdd(h + LG_SAMPLE_BINS + bin, v);
         if (const uint32_t v = (uint32_t)(x >> 30)) atomicAdd(h + 2 * LG_SAMPLE_BINS + bin, v);
-    }
-    // This thread's two bins, summed over the cluster
-    __device__ __forceinline__ void bins2(const uint32_t *h, int limbs, u64 (&v)[2]) const {
-        v[0] = v[1] = 0;
-        for (int l = 0; l < limbs; l++)
-            #pragma unroll 4
-            for (int c = 0; c < ranks; c++) {
-                const uint2 x = ld_peer_u32x2(h + l * LG_SAMPLE_BINS + threadIdx.x * 2, c);
-                v[0] += (u64)x.x << 15 * l; v[1] += (u64)x.y << 15 * l;
-            }
     }
     // The first bin at which before + the running sum of v reaches the target, and the sum before it; the last bin where none does (found = false).
     // `slot` keeps two results of one call apart.
@@ -265,51 +276,158 @@ template <typename T> struct LgSampler {
         klo = max(low, key_of<LOW>(__double2float_rd(w.top - (2 * b1 + 2) / w.inv32)));
         khi = min(top_key, key_of<LOW>(__double2float_ru(w.top - (2 * b0 - 1) / w.inv32)));
     }
+    // What one token adds: its weight, or 1
+    __device__ __forceinline__ u64 mass(bool weighted, float l) const {
+        int k;
+        double rest;
+        const bool live = w.bin(l, k, rest);
+        const double x = LgWeight::whole(w.scaled(k, rest));
+        return !weighted ? 1 : live ? (u64)(long long)x : 0;
+    }
+    // Part of the interval at which the target is reached, and the interval narrowed to it; `above`: of what lies above it
+    static __device__ __forceinline__ void narrow(int part, int sh, uint32_t &klo, uint32_t &khi) {
+        khi -= (uint32_t)part << sh;
+        const uint32_t low = khi - ((1u << sh) - 1);
+        klo = max(klo, low > khi ? 0u : low);
+    }
+    static __device__ __forceinline__ int shift_of(uint32_t range) { return range >= LG_SAMPLE_BINS ? 22 - __clz(range) : 0; }    // range >> shift < 1024
+    // This CTA's share of the bins of a histogram, summed over the cluster and left for the others: adding up all bins in every CTA would
+    // move ranks^2 histograms through the cluster
+    __device__ void share_bins(const uint32_t *h, int limbs) {
+        const int per = LG_SAMPLE_BINS / ranks;
+        for (int b = threadIdx.x; b < per; b += LG_SAMPLE_THREADS) {
+            u64 v = 0;
+            for (int l = 0; l < limbs; l++) {
+                #pragma unroll
+                for (int c = 0; c < LG_SAMPLE_MAX_CLUSTER; c++) if (c < ranks) v += (u64)ld_peer_u32(h + l * LG_SAMPLE_BINS + rank * per + b, c) << 15 * l;
+            }
+            fine[b] = v;
+        }
+        cluster_sync_all();
+    }
+    __device__ __forceinline__ void shared_bins2(u64 (&v)[2]) const {
+        const int per = LG_SAMPLE_BINS / ranks, b = threadIdx.x * 2;
+        v[0] = ld_peer_u64(fine + b % per, b / per);
+        v[1] = ld_peer_u64(fine + (b + 1) % per, (b + 1) / per);
+    }
     // The threshold at which counts (weighted: weights) of the keys from the largest down reach the target; it lies in klo .. khi.  Kept then: keys
-    // above t and `ties` of key t.
-    __device__ void refine(bool weighted, u64 target, uint32_t klo, uint32_t khi, uint32_t &t, u64 &ties) {
-        u64 above = 0;
-        for (int round = 0; round < 4; round++) {                             // 10 bits of at most 32 a round
-            const uint32_t range = khi - klo;
-            const int sh = range >= LG_SAMPLE_BINS ? 22 - __clz(range) : 0;    // range >> sh < 1024
-            const float lo = key_value<LOW>(klo), hi = key_value<LOW>(khi), over_hi = round ? INFINITY : hi;
-            uint32_t *h = fresh_hist(weighted ? 3 : 1);
-            u64 count = 0;
+    // above t and `ties` of key t.  Passes that read the row itself note its tokens in the interval in the warp's list: over_w is then this lane's part
+    // of the warp's weight above the list's tokens and n_list their number; n_list < 0: there is no such list.
+    __device__ void refine(bool weighted, u64 target, uint32_t klo, uint32_t khi, uint32_t &t, u64 &ties, u64 &over_w, int &n_list) {
+        uint32_t *n_near = (uint32_t *)(red + 2 * LG_SAMPLE_WARPS + 4);
+        u64 above, found;
+        for (int wide = 0;; wide++) {
+            // what lies above the interval, and the tokens in it
+            __syncthreads();
+            if (threadIdx.x == 0) *n_near = 0;
+            __syncthreads();
+            const float lo = key_value<LOW>(klo), hi = key_value<LOW>(khi);
+            int open = 0;
+            bool full = false;
             double over = 0.0;
+            found = 0;
             for (int i = w0; i < w1; i += 128) {
                 float l[4];
                 fetch4(i + lane * 4, l);
+                const bool any = l[0] >= lo || l[1] >= lo || l[2] >= lo || l[3] >= lo;
+                if (!__any_sync(0xffffffffu, any)) continue;
+                if (weighted) {
+                    int k[4];
+                    double x[4];
+                    bool in[4];
+                    weigh4(l, hi, k, x, in);
+                    #pragma unroll
+                    for (int j = 0; j < 4; j++) if (in[j]) over += LgWeight::whole(x[j]);
+                } else found += (u64)((l[0] > hi) + (l[1] > hi) + (l[2] > hi) + (l[3] > hi)) << 32;
+                uint32_t m[4], all = 0;
+                #pragma unroll
+                for (int j = 0; j < 4; j++) { m[j] = __ballot_sync(0xffffffffu, l[j] >= lo && l[j] <= hi); all |= m[j]; }
+                if (!all) continue;
+                int at = open;
+                uint32_t put = 0;
+                #pragma unroll
+                for (int j = 0; j < 4; j++) { at += __popc(m[j] & ((1u << lane) - 1)); open += __popc(m[j]); }
+                if (lane == 0) put = atomicAdd(n_near, (uint32_t)(__popc(m[0]) + __popc(m[1]) + __popc(m[2]) + __popc(m[3])));
+                put = __shfl_sync(0xffffffffu, put, 0) + at - (open - __popc(m[0]) - __popc(m[1]) - __popc(m[2]) - __popc(m[3]));
+                #pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (m[j] >> lane & 1) {
+                        if (put < LG_SAMPLE_NEAR) near[put] = key_of<LOW>(l[j]); else full = true;
+                        if (!listed) { if (at < LG_SAMPLE_LIST) { lv[at] = l[j]; li[at] = i + lane * 4 + j; } else full = true; }
+                        put++; at++;
+                    }
+            }
+            if (lane == 0) found += open;
+            if (full) found += 1u << 30;
+            over_w = weighted ? (u64)(long long)over : 0;
+            n_list = listed || !weighted ? -1 : open;
+            const u64 *counts;
+            sum2(weighted ? over_w : found >> 32, found & 0xFFFFFFFFull, above, found, &counts);
+            if (found <= 4 * LG_SAMPLE_THREADS) {
+                // four tokens a thread, from the CTA that has them; the rounds need no other CTA
+                uint32_t key[4];
+                u64 x[4];
+                const uint32_t n_c = (lane < ranks) ? (uint32_t)ld_peer_u64(counts + 1, lane) : 0, up = (uint32_t)warp_scan_u64(n_c, lane);
+                #pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const uint32_t i = threadIdx.x + q * LG_SAMPLE_THREADS;
+                    x[q] = 0; key[q] = 0;
+                    if (q * LG_SAMPLE_THREADS + warp * 32 >= found) continue;
+                    int c = 0;
+                    uint32_t before = 0;
+                    for (int o = 0; o < ranks; o++) { const uint32_t e = __shfl_sync(0xffffffffu, up, o); if (i >= e) { c = o + 1; before = e; } }
+                    if (i < found) key[q] = ld_peer_u32(near + (i - before), c);
+                    const u64 v = mass(weighted, key_value<LOW>(key[q]));
+                    if (i < found) x[q] = v;
+                }
+                for (int round = 0; round < 4; round++) {                     // 10 bits of at most 32 a round
+                    const int sh = shift_of(khi - klo);
+                    fine[2 * threadIdx.x] = fine[2 * threadIdx.x + 1] = 0;
+                    __syncthreads();
+                    #pragma unroll
+                    for (int q = 0; q < 4; q++) if (x[q] && key[q] >= klo && key[q] <= khi) atomicAdd(fine + ((khi - key[q]) >> sh), x[q]);
+                    __syncthreads();
+                    const u64 v[2] = {fine[2 * threadIdx.x], fine[2 * threadIdx.x + 1]};
+                    int part;
+                    first_reaching(v, above, target, 0, part, above);
+                    narrow(part, sh, klo, khi);
+                    if (sh == 0) break;
+                }
+                break;
+            }
+            // too many: one round of the whole cluster
+            const int sh = shift_of(khi - klo);
+            uint32_t *h = fresh_hist(weighted ? 3 : 1);
+            for (int i = w0; i < w1; i += 128) {
+                float l[4];
+                fetch4(i + lane * 4, l);
+                bool in[4];
+                #pragma unroll
+                for (int j = 0; j < 4; j++) in[j] = l[j] >= lo && l[j] <= hi;
+                if (!__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) continue;
                 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const bool in = l[j] >= lo && l[j] <= hi, more = l[j] > over_hi;
-                    if (!__any_sync(0xffffffffu, in || more)) continue;
+                    if (!__any_sync(0xffffffffu, in[j])) continue;
                     const int part = (int)((khi - key_of<LOW>(l[j])) >> sh);
-                    if (weighted) {
-                        int k;
-                        double rest;
-                        const bool live = w.bin(l[j], k, rest);
-                        const double x = LgWeight::whole(w.scaled(k, rest));
-                        if (live && more) over += x;
-                        if (live && in) add_weight(h, part, (u64)(long long)x);
-                    } else {
-                        count += more;
-                        if (in) atomicAdd(h + part, 1u);
-                    }
+                    const u64 x = mass(weighted, l[j]);
+                    if (in[j] && weighted) add_weight(h, part, x);
+                    else if (in[j]) atomicAdd(h + part, 1u);
                 }
             }
-            if (round == 0) { u64 none; sum2(weighted ? (u64)(long long)over : count, 0, above, none); }   // (its barrier also makes the histograms complete)
-            else cluster_sync_all();
+            cluster_sync_all();
+            share_bins(h, weighted ? 3 : 1);
             u64 v[2];
             int part;
-            bins2(h, weighted ? 3 : 1, v);
-            first_reaching(v, above, target, 0, part, above);                 // `above`: of what lies above the part from now on
-            khi -= (uint32_t)part << sh;
-            klo = max(klo, khi - ((1u << sh) - 1) > khi ? 0u : khi - ((1u << sh) - 1));
-            if (sh == 0) break;
+            shared_bins2(v);
+            first_reaching(v, above, target, 0, part, above);
+            narrow(part, sh, klo, khi);
+            n_list = -1;
+            cluster_sync_all();                                               // `fine` and the lists are used again
+            if (sh == 0 || wide == 3) break;
         }
         t = khi;
         if (!weighted) { ties = target - above; return; }
-        const u64 one = (u64)(long long)LgWeight::whole(w.of(key_value<LOW>(t)));
+        const u64 one = mass(true, key_value<LOW>(t));
         ties = one ? (target - above + one - 1) / one : 1;
     }
 };
@@ -317,7 +435,7 @@ template <typename T> struct LgSampler {
 // grid: rows x ranks, clusters of `ranks` CTAs
 template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg_sample_kernel(LgSampleArgs a) {
     extern __shared__ __align__(16) unsigned char lg_sample_sm[];
-    __shared__ u64 word[48], red[2 * LG_SAMPLE_WARPS + 4];
+    __shared__ u64 word[48], red[2 * LG_SAMPLE_WARPS + 5];
     typedef LogitType<T> L;
     constexpr int LOW = L::LOW;
     uint32_t ranks;
@@ -328,7 +446,9 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
     s.g = (const T *)a.logits + (long long)row * a.ld + first;
     s.data = (T *)lg_sample_sm;
     s.hist = (uint32_t *)(lg_sample_sm + (size_t)a.cap * sizeof(T));
-    s.lv = (float *)(s.hist + 2 * a.limbs * LG_SAMPLE_BINS) + warp * LG_SAMPLE_LIST * 2; s.li = (int *)(s.lv + LG_SAMPLE_LIST);
+    s.fine = (u64 *)(s.hist + 2 * a.limbs * LG_SAMPLE_BINS);
+    s.near = (uint32_t *)(s.fine + LG_SAMPLE_BINS);
+    s.lv = (float *)(s.near + LG_SAMPLE_NEAR) + warp * LG_SAMPLE_LIST * 2; s.li = (int *)(s.lv + LG_SAMPLE_LIST);
     s.word = word; s.red = red; s.n = n; s.first = first; s.ranks = ranks; s.rank = rank; s.lane = lane; s.warp = warp;
     const int per = ((a.slice + LG_SAMPLE_WARPS - 1) / LG_SAMPLE_WARPS + 127) / 128 * 128;
     s.w0 = min(warp * per, n); s.w1 = min(s.w0 + per, n);
@@ -403,7 +523,8 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
     s.w.top = (double)fminf(best, 3.402823466e38f); s.w.inv32 = best == INFINITY ? 0.0 : 46.166241308446828 / (double)T1; s.w.root = exp2(a.shift - lane / 32.0);
 
     uint32_t t = best == INFINITY ? top_key - 1 : LgSampler<T>::DEAD;          // threshold; at first everything above -inf
-    u64 ties = 0;
+    u64 ties = 0, over_w = 0;
+    int n_list = -1;                                    // >= 0: this warp's list and over_w say what it keeps (LgSampler::refine)
     if (top_k > 0 && top_k < a.vocab) {
         uint32_t *h = s.fresh_hist(1);
         const float lt = key_value<LOW>(t);
@@ -418,14 +539,15 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
             }
         }
         cluster_sync_all();
+        s.share_bins(h, 1);
         u64 v[2], before;
         int bin;
-        s.bins2(h, 1, v);
+        s.shared_bins2(v);
         if (s.first_reaching(v, 0, (u64)top_k, 0, bin, before)) {              // otherwise fewer than top_k tokens have a weight
             uint32_t klo, khi;
             s.interval(bin, bin, t + 1, top_key, klo, khi);
             s.make_list(key_value<LOW>(klo));
-            s.refine(false, (u64)top_k, klo, khi, t, ties);
+            s.refine(false, (u64)top_k, klo, khi, t, ties, over_w, n_list);
         }
     }
     if (top_p < 1.0f) {
@@ -437,18 +559,16 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
         uint32_t n_at = 0;
         for (int i = s.w0; i < s.w1; i += 128) {
             float l[4];
+            int k[4];
+            double x[4];
+            bool in[4];
             s.fetch4(i + lane * 4, l);
+            if (ties) n_at += (l[0] == lt) + (l[1] == lt) + (l[2] == lt) + (l[3] == lt);
+            if (!__any_sync(0xffffffffu, l[0] > lt || l[1] > lt || l[2] > lt || l[3] > lt)) continue;
+            s.weigh4(l, lt, k, x, in);
             #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool in = l[j] > lt;
-                if (ties) n_at += l[j] == lt;
-                if (!__any_sync(0xffffffffu, in)) continue;
-                int k;
-                double rest;
-                const bool live = s.w.bin(l[j], k, rest);
-                const double x = LgWeight::whole(s.w.scaled(k, rest));
-                if (live && in) { sum += x; atomicAdd(h + (k >> 1), 1u); }
-            }
+            for (int j = 0; j < 4; j++)
+                if (in[j]) { sum += LgWeight::whole(x[j]); atomicAdd(h + (k[j] >> 1), 1u); }
         }
         s.sum2((u64)(long long)sum, n_at, over, at_t);
         const u64 one = (u64)(long long)LgWeight::whole(s.w.of(lt));
@@ -462,7 +582,8 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
             u64 c[2], v[2], before;
             int b0, b1;
             double edge[2];
-            s.bins2(h, 1, c);
+            s.share_bins(h, 1);
+            s.shared_bins2(c);
             #pragma unroll
             for (int j = 0; j < 2; j++) {
                 edge[j] = s.w.scaled(4 * tid + 2 * j, 0.0);
@@ -474,8 +595,7 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
             s.first_reaching(v, 0, target, 1, b1, before);
             uint32_t klo, khi;
             s.interval(b0, max(b0, b1), t + 1, top_key, klo, khi);
-            s.make_list(key_value<LOW>(klo));
-            s.refine(true, target, klo, khi, t, ties);
+            s.refine(true, target, klo, khi, t, ties, over_w, n_list);
         }
     }
     // the draw: what each warp's tokens weigh and how many lie at the threshold, then the warp in which the running weight passes the target
@@ -483,51 +603,53 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
     const float lt = key_value<LOW>(t);
     const double x_t = s.w.of(lt);
     const u64 one = x_t >= floor_w ? (u64)(long long)LgWeight::whole(x_t) : 0;
-    double sum = 0.0;
     u64 over, at_t;
-    uint32_t n_at = 0;
-    for (int i = s.w0; i < s.w1; i += 128) {
-        float l[4];
-        s.fetch4(i + lane * 4, l);
-        #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const bool in = l[j] > lt;
-            if (ties) n_at += l[j] == lt;
-            if (!__any_sync(0xffffffffu, in)) continue;
-            int k;
-            double rest;
-            const bool live = s.w.bin(l[j], k, rest);
-            const double x = s.w.scaled(k, rest);
-            if (live && in && x >= floor_w) sum += LgWeight::whole(x);
+    if (n_list >= 0 && (ties ? x_t : 0.0) >= floor_w) {
+        // min_p takes nothing away: the weight above the list, and the list's own tokens
+        over = over_w; at_t = 0;
+        for (int i = 0; i < n_list; i += 32) {
+            const float l = i + lane < n_list ? s.lv[i + lane] : -INFINITY;
+            const u64 x = s.mass(true, l);
+            if (l > lt) over += x;
+            at_t += l == lt && ties;
         }
-    }
-    over = (u64)(long long)sum; at_t = n_at;
-    over = warp_sum_u64(over); at_t = warp_sum_u64(at_t);
-    __syncthreads();
-    if (lane == 0) { red[warp] = over; red[LG_SAMPLE_WARPS + warp] = at_t; }
-    __syncthreads();
-    u64 *mine = word + s.at_word;
-    if (warp == 0) {
-        const u64 x = warp_sum_u64(lane < LG_SAMPLE_WARPS ? red[lane] : 0), y = warp_sum_u64(lane < LG_SAMPLE_WARPS ? red[LG_SAMPLE_WARPS + lane] : 0);
-        if (lane == 0) { mine[0] = x; mine[1] = y; }
-    }
-    cluster_sync_all();
-    u64 total = 0, tied = 0, run = 0, end = 0, rank_t = 0;                     // run .. end: of this warp; rank_t: ties before it
-    for (uint32_t c = 0; c < ranks; c++) {
-        const u64 x = ld_peer_u64(mine, c), y = ld_peer_u64(mine + 1, c);
-        if ((int)c == rank) {
-            u64 at = total, seen_t = tied;
-            for (int i = 0; i <= warp; i++) {
-                const u64 left = ties > seen_t ? ties - seen_t : 0, m = red[LG_SAMPLE_WARPS + i];
-                run = at; rank_t = seen_t;
-                at += red[i] + (m < left ? m : left) * one;
-                seen_t += m;
-            }
-            end = at;
+    } else {
+        // min_p's own threshold, a little lower: what is below it needs no weight
+        const float from = floor_w > 0.0 && s.w.inv32 > 0.0 ? fmaxf(lt, __double2float_rd(s.w.top + (32.0 * log2((double)min_p) - 0.01) / s.w.inv32)) : lt;
+        double sum = 0.0;
+        uint32_t n_at = 0;
+        for (int i = s.w0; i < s.w1; i += 128) {
+            float l[4];
+            int k[4];
+            double x[4];
+            bool in[4];
+            s.fetch4(i + lane * 4, l);
+            if (ties) n_at += (l[0] == lt) + (l[1] == lt) + (l[2] == lt) + (l[3] == lt);
+            if (!__any_sync(0xffffffffu, l[0] >= from || l[1] >= from || l[2] >= from || l[3] >= from)) continue;
+            s.weigh4(l, lt, k, x, in);
+            #pragma unroll
+            for (int j = 0; j < 4; j++) if (in[j] && x[j] >= floor_w) sum += LgWeight::whole(x[j]);
         }
-        const u64 left = ties > tied ? ties - tied : 0;
-        total += x + (y < left ? y : left) * one;
-        tied += y;
+        over = (u64)(long long)sum; at_t = n_at;
+    }
+    u64 total, run, end, rank_t;                        // run .. end: of this warp; rank_t: ties before it
+    {
+        const u64 *mine;
+        u64 none;
+        s.sum2(over, at_t, total, none, &mine);
+        // the CTAs, then the warps of this one, a lane each: ties before it, of them those that are kept, the weight before it
+        auto before = [&](u64 x, u64 y, u64 ties0, u64 run0, int who, u64 &ties_at, u64 &run_at, u64 &all) {
+            const u64 y_up = warp_scan_u64(y, lane), y0 = ties0 + y_up - y, left = ties > y0 ? ties - y0 : 0, x_all = x + (y < left ? y : left) * one;
+            const u64 x_up = warp_scan_u64(x_all, lane);
+            ties_at = __shfl_sync(0xffffffffu, y0, who);
+            run_at = run0 + __shfl_sync(0xffffffffu, x_up - x_all, who);
+            all = run0 + __shfl_sync(0xffffffffu, x_up, 31);
+            return __shfl_sync(0xffffffffu, x_all, who);
+        };
+        u64 cta_t, cta_run;
+        before(lane < (int)ranks ? ld_peer_u64(mine, lane) : 0, lane < (int)ranks ? ld_peer_u64(mine + 1, lane) : 0, 0, 0, rank, cta_t, cta_run, total);
+        const u64 own = before(lane < LG_SAMPLE_WARPS ? red[lane] : 0, lane < LG_SAMPLE_WARPS ? red[LG_SAMPLE_WARPS + lane] : 0, cta_t, cta_run, warp, rank_t, run, none);
+        end = run + own;
     }
     const float u = a.u[row];
     const u64 u64_ = u > 0.0f ? u < 1.0f ? __double2ull_rz((double)u * 18446744073709551616.0) : ~0ull : 0ull;

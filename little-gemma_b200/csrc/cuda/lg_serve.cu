@@ -235,7 +235,7 @@ namespace {
 // each still has 4096 tokens (a row's time goes with the passes over a CTA's tokens; below that the barriers are the larger part).
 template <typename T> int launch_sample(LgSampleArgs &a, int dev, void *stream) {
     static unsigned char done[64], most_ranks[64];
-    const int sms = device_sms(dev), tools = a.limbs ? 2 * a.limbs * LG_SAMPLE_BINS * 4 + LG_SAMPLE_WARPS * LG_SAMPLE_LIST * 8 : 0, room = 112 * 1024 - tools;
+    const int sms = device_sms(dev), tools = a.limbs ? 2 * a.limbs * LG_SAMPLE_BINS * 4 + LG_SAMPLE_TOOLS : 0, room = 112 * 1024 - tools;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;

@@ -9,9 +9,9 @@
 // A cluster of CTAs holds a row in shared memory after one read of HBM (the part that does not fit is read again from L2); what all
 // CTAs have to know -- the maximum, histograms, sums -- goes through distributed shared memory with one cluster barrier each, and every CTA draws the same
 // conclusions from it.  A threshold is found without sorting:
-//   coarse  bins of 1/16 of a power of two of the weight (1024: beyond, a weight is 0); counts per bin and the bounds of a bin's weights tell the bins that the
-//           threshold can lie in, and with them an interval of logits
-//   list    each warp notes its tokens in or above that interval, where they are few; later passes read the list
+//   coarse  bins of 1/32 of a power of two of the weight (2048: beyond, a weight is 0); the tokens' number, or their weights to a part in 2000, added up per
+//           bin, tell the bin (two where it is close) that the threshold lies in, and with it an interval of logits
+//   list    each warp notes its tokens in that interval (top-k: and above, later passes then read the list instead of the row)
 //   fine    exact counts or weights over 1024 equal parts of that interval of keys (the logits as ordered integers), then of the part that holds the threshold,
 //           until a part is a single key: at most four rounds.  Where the lists hold the interval, every CTA fetches its tokens and does the rounds alone;
 //           otherwise (flat rows) the histograms of a round are added up over the cluster
@@ -22,11 +22,13 @@
 
 #define LG_SAMPLE_THREADS 512
 #define LG_SAMPLE_WARPS (LG_SAMPLE_THREADS / 32)
-#define LG_SAMPLE_BINS 1024            // two a thread
-#define LG_SAMPLE_LIST 96              // tokens a warp's list holds
-#define LG_SAMPLE_NEAR 256             // of these, tokens of a CTA whose place at a threshold is open
-#define LG_SAMPLE_TOOLS (LG_SAMPLE_WARPS * LG_SAMPLE_LIST * 8 + LG_SAMPLE_BINS * 8 + LG_SAMPLE_NEAR * 4)
-#define LG_SAMPLE_MAX_CLUSTER 16
+#define LG_SAMPLE_COARSE 2048          // bins, four a thread
+#define LG_SAMPLE_BINS 1024            // parts of an interval
+#define LG_SAMPLE_LIST 224             // tokens a warp's list holds
+#define LG_SAMPLE_NEAR 3072            // of these, tokens of a CTA whose place at a threshold is open
+#define LG_SAMPLE_HIST 3072            // words of a histogram: the coarse bins, or three arrays of the parts
+#define LG_SAMPLE_TOOLS (2 * LG_SAMPLE_HIST * 4 + LG_SAMPLE_COARSE * 8 + LG_SAMPLE_WARPS * LG_SAMPLE_LIST * 8 + LG_SAMPLE_NEAR * 4)
+#define LG_SAMPLE_MAX_CLUSTER 8
 
 typedef unsigned long long u64;
 
@@ -35,7 +37,6 @@ struct LgSampleArgs {
     long long ld;
     int rows, vocab, shift;
     int slice, cap;                    // tokens per CTA of a cluster; of these, tokens held in shared memory
-    int limbs;                         // histograms: 0 none, 1 counts, 3 weights too
     const float *temperature; const int *top_k; const float *top_p; const float *min_p; const float *u;
     int *token; float *prob;
 };
@@ -99,13 +100,17 @@ struct LgWeight {
         const double t = fma(d, inv32, LG_MAGIC);
         rest = fma(d, inv32, -(t - LG_MAGIC));
         k = __double2loint(t);
-        return __double2hiint(t) == 0x43380000 && (uint32_t)k < 2 * LG_SAMPLE_BINS;
+        return __double2hiint(t) == 0x43380000 && (uint32_t)k < LG_SAMPLE_COARSE;
     }
     // 2^(shift - (k + rest) / 32), all lanes of a warp together: the power of the whole number from a lane's root times a polynomial (Taylor in
     // rest ln 2 / 32, at most ln 2 / 64: the first term left out is below 2^-48)
     __device__ __forceinline__ double scaled(int k, double rest) const {
+        double p;
+        return scaled(k, rest, p);
+    }
+    __device__ __forceinline__ double scaled(int k, double rest, double &p) const {       // p: of that, 2^(-rest / 32)
         const double c = 0.02166084939249829;                                 // ln 2 / 32
-        double p = fma(rest, -c * c * c * c * c / 120.0, c * c * c * c / 24.0);
+        p = fma(rest, -c * c * c * c * c / 120.0, c * c * c * c / 24.0);
         p = fma(p, rest, -c * c * c / 6.0);
         p = fma(p, rest, c * c / 2.0);
         p = fma(p, rest, -c);
@@ -186,11 +191,15 @@ template <typename T> struct LgSampler {
     }
     // Four tokens' bins and weights side by side; in: above lt and with a weight
     __device__ __forceinline__ void weigh4(const float (&l)[4], float lt, int (&k)[4], double (&x)[4], bool (&in)[4]) const {
+        double p[4];
+        weigh4(l, lt, k, x, in, p);
+    }
+    __device__ __forceinline__ void weigh4(const float (&l)[4], float lt, int (&k)[4], double (&x)[4], bool (&in)[4], double (&p)[4]) const {
         double rest[4];
         #pragma unroll
         for (int j = 0; j < 4; j++) in[j] = w.bin(l[j], k[j], rest[j]) && l[j] > lt;
         #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = w.scaled(k[j], rest[j]);
+        for (int j = 0; j < 4; j++) x[j] = w.scaled(k[j], rest[j], p[j]);
     }
     // This warp's tokens of at least `least` into its list, in their order, where they fit
     __device__ void make_list(float least) {
@@ -234,10 +243,10 @@ template <typename T> struct LgSampler {
         if (at) *at = p;
     }
     // An empty histogram (block-wide; the cluster has passed a barrier since the one before it was read)
-    __device__ uint32_t *fresh_hist(int limbs) {
-        uint32_t *h = hist + turn * a.limbs * LG_SAMPLE_BINS;
+    __device__ uint32_t *fresh_hist(int words) {
+        uint32_t *h = hist + turn * LG_SAMPLE_HIST;
         turn ^= 1;
-        for (int i = threadIdx.x; i < limbs * LG_SAMPLE_BINS; i += LG_SAMPLE_THREADS) h[i] = 0;
+        for (int i = threadIdx.x; i < words; i += LG_SAMPLE_THREADS) h[i] = 0;
         __syncthreads();
         return h;
     }
@@ -248,8 +257,11 @@ template <typename T> struct LgSampler {
     }
     // The first bin at which before + the running sum of v reaches the target, and the sum before it; the last bin where none does (found = false).
     // `slot` keeps two results of one call apart.
-    __device__ bool first_reaching(const u64 (&v)[2], u64 before, u64 target, int slot, int &bin, u64 &sum) {
-        const u64 mine = v[0] + v[1], incl = warp_scan_u64(mine, lane);
+    template <int N> __device__ bool first_reaching(const u64 (&v)[N], u64 before, u64 target, int slot, int &bin, u64 &sum) {
+        u64 mine = 0;
+        #pragma unroll
+        for (int j = 0; j < N; j++) mine += v[j];
+        const u64 incl = warp_scan_u64(mine, lane);
         __syncthreads();
         if (lane == 31) red[warp] = incl;
         if (threadIdx.x == 0) red[2 * LG_SAMPLE_WARPS + slot] = ~0ull;
@@ -258,14 +270,16 @@ template <typename T> struct LgSampler {
         u64 at = before + incl - mine + __shfl_sync(0xffffffffu, wi - ws, warp);
         const u64 all = before + __shfl_sync(0xffffffffu, wi, 31);
         if (at < target && target <= at + mine) {
-            const bool second = at + v[0] < target;
-            red[2 * LG_SAMPLE_WARPS + slot] = threadIdx.x * 2 + second;
-            red[2 * LG_SAMPLE_WARPS + 2 + slot] = second ? at + v[0] : at;
+            int k = 0;
+            #pragma unroll
+            for (int j = 0; j < N - 1; j++) if (k == j && at + v[j] < target) { at += v[j]; k++; }
+            red[2 * LG_SAMPLE_WARPS + slot] = threadIdx.x * N + k;
+            red[2 * LG_SAMPLE_WARPS + 2 + slot] = at;
         }
         __syncthreads();
         const u64 b = red[2 * LG_SAMPLE_WARPS + slot];
         const bool found = b != ~0ull;
-        bin = found ? (int)b : LG_SAMPLE_BINS - 1;
+        bin = found ? (int)b : N * LG_SAMPLE_THREADS - 1;
         sum = found ? red[2 * LG_SAMPLE_WARPS + 2 + slot] : all;
         return found;
     }
@@ -273,8 +287,8 @@ template <typename T> struct LgSampler {
     __device__ void interval(int b0, int b1, uint32_t low, uint32_t top_key, uint32_t &klo, uint32_t &khi) const {
         klo = low; khi = top_key;
         if (!(w.inv32 > 0.0)) return;
-        klo = max(low, key_of<LOW>(__double2float_rd(w.top - (2 * b1 + 2) / w.inv32)));
-        khi = min(top_key, key_of<LOW>(__double2float_ru(w.top - (2 * b0 - 1) / w.inv32)));
+        klo = max(low, key_of<LOW>(__double2float_rd(w.top - (b1 + 0.51) / w.inv32)));
+        khi = min(top_key, key_of<LOW>(__double2float_ru(w.top - (b0 - 0.51) / w.inv32)));
     }
     // What one token adds: its weight, or 1
     __device__ __forceinline__ u64 mass(bool weighted, float l) const {
@@ -293,22 +307,22 @@ template <typename T> struct LgSampler {
     static __device__ __forceinline__ int shift_of(uint32_t range) { return range >= LG_SAMPLE_BINS ? 22 - __clz(range) : 0; }    // range >> shift < 1024
     // This CTA's share of the bins of a histogram, summed over the cluster and left for the others: adding up all bins in every CTA would
     // move ranks^2 histograms through the cluster
-    __device__ void share_bins(const uint32_t *h, int limbs) {
-        const int per = LG_SAMPLE_BINS / ranks;
+    __device__ void share_bins(const uint32_t *h, int bins, int limbs) {
+        const int per = bins / ranks;
         for (int b = threadIdx.x; b < per; b += LG_SAMPLE_THREADS) {
             u64 v = 0;
             for (int l = 0; l < limbs; l++) {
                 #pragma unroll
-                for (int c = 0; c < LG_SAMPLE_MAX_CLUSTER; c++) if (c < ranks) v += (u64)ld_peer_u32(h + l * LG_SAMPLE_BINS + rank * per + b, c) << 15 * l;
+                for (int c = 0; c < LG_SAMPLE_MAX_CLUSTER; c++) if (c < ranks) v += (u64)ld_peer_u32(h + l * bins + rank * per + b, c) << 15 * l;
             }
             fine[b] = v;
         }
         cluster_sync_all();
     }
-    __device__ __forceinline__ void shared_bins2(u64 (&v)[2]) const {
-        const int per = LG_SAMPLE_BINS / ranks, b = threadIdx.x * 2;
-        v[0] = ld_peer_u64(fine + b % per, b / per);
-        v[1] = ld_peer_u64(fine + (b + 1) % per, (b + 1) / per);
+    template <int N> __device__ __forceinline__ void shared_bins(u64 (&v)[N]) const {     // N a thread
+        const int per = N * LG_SAMPLE_THREADS / ranks;
+        #pragma unroll
+        for (int j = 0; j < N; j++) { const int b = threadIdx.x * N + j; v[j] = ld_peer_u64(fine + b % per, b / per); }
     }
     // The threshold at which counts (weighted: weights) of the keys from the largest down reach the target; it lies in klo .. khi.  Kept then: keys
     // above t and `ties` of key t.  Passes that read the row itself note its tokens in the interval in the warp's list: over_w is then this lane's part
@@ -363,13 +377,13 @@ template <typename T> struct LgSampler {
             n_list = listed || !weighted ? -1 : open;
             const u64 *counts;
             sum2(weighted ? over_w : found >> 32, found & 0xFFFFFFFFull, above, found, &counts);
-            if (found <= 4 * LG_SAMPLE_THREADS) {
-                // four tokens a thread, from the CTA that has them; the rounds need no other CTA
-                uint32_t key[4];
-                u64 x[4];
+            if (found <= 8 * LG_SAMPLE_THREADS) {
+                // eight tokens a thread, from the CTA that has them; the rounds need no other CTA
+                uint32_t key[8];
+                u64 x[8];
                 const uint32_t n_c = (lane < ranks) ? (uint32_t)ld_peer_u64(counts + 1, lane) : 0, up = (uint32_t)warp_scan_u64(n_c, lane);
                 #pragma unroll
-                for (int q = 0; q < 4; q++) {
+                for (int q = 0; q < 8; q++) {
                     const uint32_t i = threadIdx.x + q * LG_SAMPLE_THREADS;
                     x[q] = 0; key[q] = 0;
                     if (q * LG_SAMPLE_THREADS + warp * 32 >= found) continue;
@@ -385,7 +399,7 @@ template <typename T> struct LgSampler {
                     fine[2 * threadIdx.x] = fine[2 * threadIdx.x + 1] = 0;
                     __syncthreads();
                     #pragma unroll
-                    for (int q = 0; q < 4; q++) if (x[q] && key[q] >= klo && key[q] <= khi) atomicAdd(fine + ((khi - key[q]) >> sh), x[q]);
+                    for (int q = 0; q < 8; q++) if (x[q] && key[q] >= klo && key[q] <= khi) atomicAdd(fine + ((khi - key[q]) >> sh), x[q]);
                     __syncthreads();
                     const u64 v[2] = {fine[2 * threadIdx.x], fine[2 * threadIdx.x + 1]};
                     int part;
@@ -397,7 +411,7 @@ template <typename T> struct LgSampler {
             }
             // too many: one round of the whole cluster
             const int sh = shift_of(khi - klo);
-            uint32_t *h = fresh_hist(weighted ? 3 : 1);
+            uint32_t *h = fresh_hist(weighted ? 3 * LG_SAMPLE_BINS : LG_SAMPLE_BINS);
             for (int i = w0; i < w1; i += 128) {
                 float l[4];
                 fetch4(i + lane * 4, l);
@@ -415,10 +429,10 @@ template <typename T> struct LgSampler {
                 }
             }
             cluster_sync_all();
-            share_bins(h, weighted ? 3 : 1);
+            share_bins(h, LG_SAMPLE_BINS, weighted ? 3 : 1);
             u64 v[2];
             int part;
-            shared_bins2(v);
+            shared_bins(v);
             first_reaching(v, above, target, 0, part, above);
             narrow(part, sh, klo, khi);
             n_list = -1;
@@ -436,6 +450,7 @@ template <typename T> struct LgSampler {
 template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg_sample_kernel(LgSampleArgs a) {
     extern __shared__ __align__(16) unsigned char lg_sample_sm[];
     __shared__ u64 word[48], red[2 * LG_SAMPLE_WARPS + 5];
+    __shared__ int kind[LG_SAMPLE_WARPS];               // tokens of a warp's list, -1: it has the row's own
     typedef LogitType<T> L;
     constexpr int LOW = L::LOW;
     uint32_t ranks;
@@ -446,8 +461,8 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
     s.g = (const T *)a.logits + (long long)row * a.ld + first;
     s.data = (T *)lg_sample_sm;
     s.hist = (uint32_t *)(lg_sample_sm + (size_t)a.cap * sizeof(T));
-    s.fine = (u64 *)(s.hist + 2 * a.limbs * LG_SAMPLE_BINS);
-    s.near = (uint32_t *)(s.fine + LG_SAMPLE_BINS);
+    s.fine = (u64 *)(s.hist + 2 * LG_SAMPLE_HIST);
+    s.near = (uint32_t *)(s.fine + LG_SAMPLE_COARSE);
     s.lv = (float *)(s.near + LG_SAMPLE_NEAR) + warp * LG_SAMPLE_LIST * 2; s.li = (int *)(s.lv + LG_SAMPLE_LIST);
     s.word = word; s.red = red; s.n = n; s.first = first; s.ranks = ranks; s.rank = rank; s.lane = lane; s.warp = warp;
     const int per = ((a.slice + LG_SAMPLE_WARPS - 1) / LG_SAMPLE_WARPS + 127) / 128 * 128;
@@ -526,7 +541,7 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
     u64 ties = 0, over_w = 0;
     int n_list = -1;                                    // >= 0: this warp's list and over_w say what it keeps (LgSampler::refine)
     if (top_k > 0 && top_k < a.vocab) {
-        uint32_t *h = s.fresh_hist(1);
+        uint32_t *h = s.fresh_hist(LG_SAMPLE_COARSE);
         const float lt = key_value<LOW>(t);
         for (int i = s.w0; i < s.w1; i += 128) {
             float l[4];
@@ -535,14 +550,14 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
             for (int j = 0; j < 4; j++) {
                 int k;
                 double rest;
-                if (s.w.bin(l[j], k, rest) && l[j] > lt) atomicAdd(h + (k >> 1), 1u);
+                if (s.w.bin(l[j], k, rest) && l[j] > lt) atomicAdd(h + k, 1u);
             }
         }
         cluster_sync_all();
-        s.share_bins(h, 1);
-        u64 v[2], before;
+        s.share_bins(h, LG_SAMPLE_COARSE, 1);
+        u64 v[4], before;
         int bin;
-        s.shared_bins2(v);
+        s.shared_bins(v);
         if (s.first_reaching(v, 0, (u64)top_k, 0, bin, before)) {              // otherwise fewer than top_k tokens have a weight
             uint32_t klo, khi;
             s.interval(bin, bin, t + 1, top_key, klo, khi);
@@ -552,7 +567,7 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
     }
     if (top_p < 1.0f) {
         // weight above the threshold, tokens at it
-        uint32_t *h = s.fresh_hist(1);
+        uint32_t *h = s.fresh_hist(LG_SAMPLE_COARSE);
         const float lt = key_value<LOW>(t);
         double sum = 0.0;
         u64 over, at_t;
@@ -565,10 +580,11 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
             s.fetch4(i + lane * 4, l);
             if (ties) n_at += (l[0] == lt) + (l[1] == lt) + (l[2] == lt) + (l[3] == lt);
             if (!__any_sync(0xffffffffu, l[0] > lt || l[1] > lt || l[2] > lt || l[3] > lt)) continue;
-            s.weigh4(l, lt, k, x, in);
+            double p[4];
+            s.weigh4(l, lt, k, x, in, p);
             #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (in[j]) { sum += LgWeight::whole(x[j]); atomicAdd(h + (k[j] >> 1), 1u); }
+                if (in[j]) { sum += LgWeight::whole(x[j]); atomicAdd(h + k[j], (uint32_t)__double2loint(fma(p[j], 1000.0, LG_TWO52))); }
         }
         s.sum2((u64)(long long)sum, n_at, over, at_t);
         const u64 one = (u64)(long long)LgWeight::whole(s.w.of(lt));
@@ -578,20 +594,20 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
         if (target < 1) target = 1;
         if (target > over) ties = min(ties, one ? (target - over + one - 1) / one : ties);
         else {
-            // the weights of a bin lie between those of its borders: half a step above its first number, half a step below its second
-            u64 c[2], v[2], before;
+            // a bin's tokens count 989 .. 1011 each: their weights in thousandths of the bin's own, to half of one
+            u64 c[4], v[4], before;
             int b0, b1;
-            double edge[2];
-            s.share_bins(h, 1);
-            s.shared_bins2(c);
+            double edge[4];
+            s.share_bins(h, LG_SAMPLE_COARSE, 1);
+            s.shared_bins(c);
             #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                edge[j] = s.w.scaled(4 * tid + 2 * j, 0.0);
-                v[j] = c[j] * (u64)__double2ull_ru(edge[j] * 1.0111);         // 2^(0.51 / 32) = 1.01111
+            for (int j = 0; j < 4; j++) {
+                edge[j] = (double)c[j] * (s.w.scaled(4 * tid + j, 0.0) * 0.001);
+                v[j] = __double2ull_ru(edge[j] * 1.0006) + c[j];              // (and half a unit for the rounding of each weight)
             }
             s.first_reaching(v, 0, target, 0, b0, before);
             #pragma unroll
-            for (int j = 0; j < 2; j++) v[j] = c[j] * (u64)__double2ull_rd(edge[j] * 0.9678);     // 2^(-1.51 / 32) = 0.96782
+            for (int j = 0; j < 4; j++) { const u64 low = __double2ull_rd(edge[j] * 0.9994); v[j] = low > c[j] ? low - c[j] : 0; }
             s.first_reaching(v, 0, target, 1, b1, before);
             uint32_t klo, khi;
             s.interval(b0, max(b0, b1), t + 1, top_key, klo, khi);
@@ -632,65 +648,90 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
         }
         over = (u64)(long long)sum; at_t = n_at;
     }
-    u64 total, run, end, rank_t;                        // run .. end: of this warp; rank_t: ties before it
-    {
-        const u64 *mine;
-        u64 none;
-        s.sum2(over, at_t, total, none, &mine);
-        // the CTAs, then the warps of this one, a lane each: ties before it, of them those that are kept, the weight before it
-        auto before = [&](u64 x, u64 y, u64 ties0, u64 run0, int who, u64 &ties_at, u64 &run_at, u64 &all) {
-            const u64 y_up = warp_scan_u64(y, lane), y0 = ties0 + y_up - y, left = ties > y0 ? ties - y0 : 0, x_all = x + (y < left ? y : left) * one;
-            const u64 x_up = warp_scan_u64(x_all, lane);
-            ties_at = __shfl_sync(0xffffffffu, y0, who);
-            run_at = run0 + __shfl_sync(0xffffffffu, x_up - x_all, who);
-            all = run0 + __shfl_sync(0xffffffffu, x_up, 31);
-            return __shfl_sync(0xffffffffu, x_all, who);
-        };
-        u64 cta_t, cta_run;
-        before(lane < (int)ranks ? ld_peer_u64(mine, lane) : 0, lane < (int)ranks ? ld_peer_u64(mine + 1, lane) : 0, 0, 0, rank, cta_t, cta_run, total);
-        const u64 own = before(lane < LG_SAMPLE_WARPS ? red[lane] : 0, lane < LG_SAMPLE_WARPS ? red[LG_SAMPLE_WARPS + lane] : 0, cta_t, cta_run, warp, rank_t, run, none);
-        end = run + own;
-    }
+    // ties before one of several pieces of the row (a lane each), the weight before it and in it, where a piece's tokens at the threshold are kept while
+    // there are ties left; `all`: the weight behind the last piece
+    auto before = [&](u64 x, u64 y, u64 ties0, u64 run0, u64 &y0, u64 &x0, u64 &all) {
+        const u64 y_up = warp_scan_u64(y, lane);
+        y0 = ties0 + y_up - y;
+        const u64 left = ties > y0 ? ties - y0 : 0, x_all = x + (y < left ? y : left) * one, x_up = warp_scan_u64(x_all, lane);
+        x0 = run0 + x_up - x_all;
+        all = run0 + __shfl_sync(0xffffffffu, x_up, 31);
+        return x_all;
+    };
+    if (lane == 0) kind[warp] = s.listed ? s.w1 : -1;
+    const u64 *mine;
+    u64 total, none, y0, x0;
+    s.sum2(over, at_t, total, none, &mine);
+    u64 x_all = before(lane < (int)ranks ? ld_peer_u64(mine, lane) : 0, lane < (int)ranks ? ld_peer_u64(mine + 1, lane) : 0, 0, 0, y0, x0, total);
     const float u = a.u[row];
-    const u64 u64_ = u > 0.0f ? u < 1.0f ? __double2ull_rz((double)u * 18446744073709551616.0) : ~0ull : 0ull;
-    const u64 target = __umul64hi(u64_, total);
-    if (run <= target && target < end) {
-        for (int i = s.w0; i < s.w1; i += 128) {
+    const u64 u_64 = u > 0.0f ? u < 1.0f ? __double2ull_rz((double)u * 18446744073709551616.0) : ~0ull : 0ull, target = __umul64hi(u_64, total);
+    uint32_t hit = __ballot_sync(0xffffffffu, x0 <= target && target < x0 + x_all);
+    if (hit && __ffs(hit) - 1 == rank) {
+        // this CTA: the warp in whose tokens the running weight passes the target, then a sixteenth of those, each by a warp
+        u64 ties0 = __shfl_sync(0xffffffffu, y0, rank), run = __shfl_sync(0xffffffffu, x0, rank);
+        x_all = before(lane < LG_SAMPLE_WARPS ? red[lane] : 0, lane < LG_SAMPLE_WARPS ? red[LG_SAMPLE_WARPS + lane] : 0, ties0, run, y0, x0, none);
+        hit = __ballot_sync(0xffffffffu, x0 <= target && target < x0 + x_all);
+        const int who = hit ? __ffs(hit) - 1 : 0;
+        ties0 = __shfl_sync(0xffffffffu, y0, who); run = __shfl_sync(0xffffffffu, x0, who);
+        s.listed = kind[who] >= 0;
+        s.lv += (who - warp) * LG_SAMPLE_LIST * 2; s.li += (who - warp) * LG_SAMPLE_LIST * 2;
+        const int from = s.listed ? 0 : min(who * per, n), to = s.listed ? kind[who] : min(from + per, n), sub = ((to - from + LG_SAMPLE_WARPS - 1) / LG_SAMPLE_WARPS + 127) / 128 * 128;
+        const int i0 = min(from + warp * sub, to), i1 = min(i0 + sub, to);
+        // four tokens a lane: what each weighs if it is kept, ties aside, and which lie at the threshold
+        auto kept4 = [&](int i, double (&x)[4], u64 (&v)[4]) {
             float l[4];
-            uint32_t eq = 0;
-            double x[4];
-            u64 v[4], sum = 0;
+            int k[4];
+            bool in[4];
             s.fetch4(i + lane * 4, l);
+            s.weigh4(l, lt, k, x, in);
+            uint32_t eq = 0;
             #pragma unroll
             for (int j = 0; j < 4; j++) {
-                int k;
-                double rest;
-                const bool live = s.w.bin(l[j], k, rest);
-                x[j] = s.w.scaled(k, rest);
-                v[j] = live && l[j] > lt && x[j] >= floor_w ? (u64)(long long)LgWeight::whole(x[j]) : 0;
-                eq |= (uint32_t)(l[j] == lt) << j;
+                v[j] = in[j] && x[j] >= floor_w ? (u64)(long long)LgWeight::whole(x[j]) : 0;
+                eq |= (uint32_t)(ties && l[j] == lt) << j;
+                if (l[j] == lt) x[j] = x_t;
             }
-            const u64 ties_up = warp_scan_u64(__popc(eq), lane);
-            u64 rk = rank_t + ties_up - __popc(eq);
-            #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (eq >> j & 1) v[j] = rk++ < ties ? one : 0;
-                sum += v[j];
-            }
-            const u64 up = warp_scan_u64(sum, lane);
-            const uint32_t hit = __ballot_sync(0xffffffffu, run + up > target);
-            if (hit) {
-                if (lane == __ffs(hit) - 1) {
-                    u64 at = run + up - sum;
-                    int j = 0;
-                    while (at + v[j] <= target) at += v[j++];
-                    a.token[row] = first + (s.listed ? s.li[i + lane * 4 + j] : i + lane * 4 + j);
-                    if (a.prob) a.prob[row] = (float)(x[j] / (double)total);
+            return eq;
+        };
+        double x[4];
+        u64 v[4];
+        over = at_t = 0;
+        for (int i = i0; i < i1; i += 128) { const uint32_t eq = kept4(i, x, v); over += v[0] + v[1] + v[2] + v[3]; at_t += __popc(eq); }
+        over = warp_sum_u64(over); at_t = warp_sum_u64(at_t);
+        __syncthreads();
+        if (lane == 0) { red[warp] = over; red[LG_SAMPLE_WARPS + warp] = at_t; }
+        __syncthreads();
+        x_all = before(lane < LG_SAMPLE_WARPS ? red[lane] : 0, lane < LG_SAMPLE_WARPS ? red[LG_SAMPLE_WARPS + lane] : 0, ties0, run, y0, x0, none);
+        hit = __ballot_sync(0xffffffffu, x0 <= target && target < x0 + x_all);
+        if (hit && __ffs(hit) - 1 == warp) {
+            run = __shfl_sync(0xffffffffu, x0, warp);
+            u64 rank_t = __shfl_sync(0xffffffffu, y0, warp);
+            for (int i = i0; i < i1; i += 128) {
+                const uint32_t eq = kept4(i, x, v);
+                const u64 ties_up = warp_scan_u64(__popc(eq), lane);
+                u64 rk = rank_t + ties_up - __popc(eq), sum = 0;
+                #pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (eq >> j & 1) v[j] = rk++ < ties ? one : 0;
+                    sum += v[j];
                 }
-                break;
+                const u64 up = warp_scan_u64(sum, lane);
+                hit = __ballot_sync(0xffffffffu, run + up > target);
+                if (hit) {
+                    if (lane == __ffs(hit) - 1) {
+                        u64 at = run + up - sum;
+                        int at_j = 0;
+                        double got = x[0];
+                        #pragma unroll
+                        for (int j = 0; j < 3; j++) if (at_j == j && at + v[j] <= target) { at += v[j]; at_j++; got = x[j + 1]; }
+                        a.token[row] = first + (s.listed ? s.li[i + lane * 4 + at_j] : i + lane * 4 + at_j);
+                        if (a.prob) a.prob[row] = (float)(got / (double)total);
+                    }
+                    break;
+                }
+                run += __shfl_sync(0xffffffffu, up, 31);
+                rank_t += __shfl_sync(0xffffffffu, ties_up, 31);
             }
-            run += __shfl_sync(0xffffffffu, up, 31);
-            rank_t += __shfl_sync(0xffffffffu, ties_up, 31);
         }
     }
     cluster_sync_all();

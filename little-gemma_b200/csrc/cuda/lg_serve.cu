@@ -40,14 +40,16 @@ struct OnDevice {
     ~OnDevice() { if (prev >= 0) cudaSetDevice(prev); }
 };
 
-// early: the kernel may start while the one before it drains (it begins with pdl_wait)
-template <typename... KArgs> int launch_serve(const char *who, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, void *stream, bool early, KArgs... args) {
+// early: the kernel may start while the one before it drains (it begins with pdl_wait); cluster: CTAs of one, along x
+template <typename... KArgs> int launch_serve(const char *who, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, void *stream, bool early, int cluster, KArgs... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at; cfg.numAttrs = early ? 1 : 0;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = early ? 2 : 1;
     const cudaError_t rc = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (rc != cudaSuccess) { cudaGetLastError(); SERVE_FAIL(-6, "%s: launch failed: %s", who, cudaGetErrorString(rc)); }
     return 0;
@@ -107,10 +109,13 @@ extern "C" int lg_paged_step(const struct lg_paged_cache *c, int n_req, const in
     LgStepArgs a;
     a.c = paged_of(c); a.n_req = n_req; a.cap = cap; a.keep = d_keep; a.fresh = d_new;
     a.start = d_start; a.pos = d_pos; a.slot = d_slot; a.req = d_req;
-    const size_t smem = 3 * ((size_t)n_req + 1) * sizeof(int), most = 3 * ((size_t)LG_PAGED_MAX_REQ + 1) * sizeof(int);
+    const size_t smem = (4 * (size_t)n_req + 1) * sizeof(int);
+    // a cluster where one CTA would go over its threads' rows more than twice
+    const int ctas = cap > 2 * LG_STEP_THREADS ? 8 : 1;
     static unsigned char done[64];
-    if (!allow_smem(lg_paged_step_kernel, smem, most, on.dev, done)) SERVE_FAIL(-6, "lg_paged_step: no %zu bytes of shared memory", smem);
-    return launch_serve("lg_paged_step", lg_paged_step_kernel, dim3(1), dim3(LG_STEP_THREADS), smem, stream, false, a);
+    if (!allow_smem(lg_paged_step_kernel<8>, smem, (4 * (size_t)LG_PAGED_MAX_REQ + 1) * sizeof(int), on.dev, done)) SERVE_FAIL(-6, "lg_paged_step: no %zu bytes of shared memory", smem);
+    void (*kernel)(LgStepArgs) = n_req <= LG_STEP_THREADS ? lg_paged_step_kernel<1> : n_req <= 2 * LG_STEP_THREADS ? lg_paged_step_kernel<2> : lg_paged_step_kernel<8>;
+    return launch_serve("lg_paged_step", kernel, dim3(ctas), dim3(LG_STEP_THREADS), smem, stream, false, ctas, a);
 }
 
 extern "C" int lg_paged_append(const struct lg_paged_cache *c, const void *d_k, const void *d_v, int type, long long ld_k, long long ld_v, int n,
@@ -135,7 +140,7 @@ extern "C" int lg_paged_append(const struct lg_paged_cache *c, const void *d_k, 
     if (c->type == TY_F32) kernel = lg_paged_append_kernel<float, float>;
     else if (c->type == TY_F16) kernel = type == TY_F32 ? lg_paged_append_kernel<float, __half> : lg_paged_append_kernel<__half, __half>;
     else kernel = type == TY_F32 ? lg_paged_append_kernel<float, __nv_bfloat16> : lg_paged_append_kernel<__nv_bfloat16, __nv_bfloat16>;
-    return launch_serve("lg_paged_append", kernel, grid, dim3(256), 0, stream, false, a);
+    return launch_serve("lg_paged_append", kernel, grid, dim3(256), 0, stream, false, 1, a);
 }
 
 namespace {
@@ -170,10 +175,10 @@ template <typename TQ, typename TC, int HD, int NT> int launch_attn_tile(LgPaged
     const long long slices = ((long long)a.c.max_pages * a.c.page_size + 15) / 16 + 1 + LG_PA_ITEM_COST;
     const long long all = slices * a.n_req * a.c.n_kv * ((a.n_new * a.gqa + a.group_rows - 1) / a.group_rows) / LG_PA_MIN_STRETCH + 1;
     const int grid = all < ctas ? (int)all : ctas;
-    const int rc = launch_serve("lg_paged_attn", lg_paged_attn_kernel<TQ, TC, HD, NT>, dim3(grid), dim3(P::W * 32), P::SMEM, stream, false, a);
+    const int rc = launch_serve("lg_paged_attn", lg_paged_attn_kernel<TQ, TC, HD, NT>, dim3(grid), dim3(P::W * 32), P::SMEM, stream, false, 1, a);
     if (rc || grid == 1) return rc;
     const int rows = a.n_new * a.gqa;
-    return launch_serve("lg_paged_attn", lg_paged_merge_kernel<TQ>, dim3(grid - 1, rows < a.group_rows ? rows : a.group_rows), dim3(256), 0, stream, true, a);
+    return launch_serve("lg_paged_attn", lg_paged_merge_kernel<TQ>, dim3(grid - 1, rows < a.group_rows ? rows : a.group_rows), dim3(256), 0, stream, true, 1, a);
 }
 template <typename TQ, typename TC> int launch_attn_16(LgPagedAttnArgs &a, const AttnCut &k, int dev, void *stream) {
     int rc;
@@ -225,49 +230,28 @@ extern "C" int lg_paged_attn(const struct lg_paged_cache *c, const void *d_q, in
     a.part = (float *)(a.jobs + LG_PA_MAX_CTAS);
     a.part_ml = (float2 *)(a.part + LG_PA_MAX_CTAS * 2LL * a.group_rows * c->head_dim);
     if (c->type == TY_F32)
-        return launch_serve("lg_paged_attn", lg_paged_attn_rows_kernel<float, float>, dim3(n_new, n_heads, n_req), dim3(LG_PATTN_WARPS * 32), 0, stream, false, a);
+        return launch_serve("lg_paged_attn", lg_paged_attn_rows_kernel<float, float>, dim3(n_new, n_heads, n_req), dim3(LG_PATTN_WARPS * 32), 0, stream, false, 1, a);
     if (c->type == TY_F16) return type == TY_F32 ? launch_attn_16<float, __half>(a, k, on.dev, stream) : launch_attn_16<__half, __half>(a, k, on.dev, stream);
     return type == TY_F32 ? launch_attn_16<float, __nv_bfloat16>(a, k, on.dev, stream) : launch_attn_16<__nv_bfloat16, __nv_bfloat16>(a, k, on.dev, stream);
 }
 
 namespace {
-// CTAs that share a row: as many as it takes to hold it in shared memory with two CTAs per SM, more while they do not fill the SMs twice and
-// each still has 4096 tokens (a row's time goes with the passes over a CTA's tokens; below that the barriers are the larger part).
+// CTAs that share a row (a cluster; 8 at most, which every device places, and 16 were slower).  A row's time goes with the passes over a CTA's
+// tokens, so few rows are shared by more CTAs, as long as each has 4096 tokens; with more rows than that the SMs are filled about three times (two CTAs fit one),
+// with 16384 tokens or more each, since a CTA's fixed work -- barriers, scans of histograms -- is done in each.  Measured, CTAs a row 1 / 2 / 4 / 8: one row of
+// 262144 - / 79 / 55 / 44 us, 48 rows - / 176 / 151 / 145, 200 rows - / 364 / 379 / 498, 64 rows of 32768 42 / 37 / 43 / 85, 512 rows of 32768 47 / 55 / 87 / 163.
 template <typename T> int launch_sample(LgSampleArgs &a, int dev, void *stream) {
-    static unsigned char done[64], most_ranks[64];
-    const int sms = device_sms(dev), tools = a.limbs ? 2 * a.limbs * LG_SAMPLE_BINS * 4 + LG_SAMPLE_TOOLS : 0, room = 112 * 1024 - tools;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    cfg.blockDim = dim3(LG_SAMPLE_THREADS); cfg.stream = (cudaStream_t)stream;
-    cfg.attrs = at; cfg.numAttrs = 1;
-    if (dev >= 64 || !done[dev]) {
-        if (cudaFuncSetAttribute(lg_sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024) != cudaSuccess) {
-            cudaGetLastError();
-            SERVE_FAIL(-6, "lg_sample: no %d bytes of shared memory", 112 * 1024);
-        }
-        int ranks = 8, n = 0;                                                 // what every device places; 16 where this one does
-        at[0].val.clusterDim.x = LG_SAMPLE_MAX_CLUSTER;
-        cfg.gridDim = dim3(LG_SAMPLE_MAX_CLUSTER); cfg.dynamicSmemBytes = 112 * 1024;
-        if (cudaFuncSetAttribute(lg_sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
-            cudaOccupancyMaxActiveClusters(&n, lg_sample_kernel<T>, &cfg) == cudaSuccess && n > 0) ranks = LG_SAMPLE_MAX_CLUSTER;
-        cudaGetLastError();
-        most_ranks[dev & 63] = (unsigned char)ranks;
-        if (dev < 64) done[dev] = 1;
-    }
-    const int most = most_ranks[dev & 63];
+    const int sms = device_sms(dev), tools = a.top_k || a.top_p ? LG_SAMPLE_TOOLS : 0, room = 112 * 1024 - tools;
     int ranks = 1;
-    while (ranks < most && ((long long)(a.vocab + ranks - 1) / ranks * (int)sizeof(T) > room || ((long long)a.rows * ranks <= sms && a.vocab / (ranks * 2) >= 4096))) ranks *= 2;
+    while (ranks < LG_SAMPLE_MAX_CLUSTER && (a.vocab > ranks << 17 || ((long long)a.rows * ranks * 2 <= sms && a.vocab / (ranks * 2) >= 4096) ||
+                                             ((long long)a.rows * ranks * 2 <= 3 * sms && a.vocab / (ranks * 2) >= 16384))) ranks *= 2;
     a.slice = ((a.vocab + ranks - 1) / ranks + 127) / 128 * 128;
     const long long held = room / (int)sizeof(T) / 128 * 128;
     a.cap = (int)(a.slice < held ? a.slice : held);
-    cfg.dynamicSmemBytes = (size_t)a.cap * sizeof(T) + tools;
-    cfg.gridDim = dim3((unsigned)a.rows * ranks);
-    at[0].val.clusterDim.x = ranks;
-    const cudaError_t rc = cudaLaunchKernelEx(&cfg, lg_sample_kernel<T>, a);
-    if (rc != cudaSuccess) { cudaGetLastError(); SERVE_FAIL(-6, "lg_sample: launch failed: %s", cudaGetErrorString(rc)); }
-    return 0;
+    const size_t smem = (size_t)a.cap * sizeof(T) + tools;
+    static unsigned char done[64];
+    if (!allow_smem(lg_sample_kernel<T>, smem, 112 * 1024, dev, done)) SERVE_FAIL(-6, "lg_sample: no %zu bytes of shared memory", smem);
+    return launch_serve("lg_sample", lg_sample_kernel<T>, dim3((unsigned)a.rows * ranks), dim3(LG_SAMPLE_THREADS), smem, stream, false, ranks, a);
 }
 }  // namespace
 
@@ -289,7 +273,6 @@ extern "C" int lg_sample(const void *d_logits, int type, long long ld, int rows,
     while ((1 << bits) < vocab) bits++;
     a.shift = 62 - bits < 44 ? 62 - bits : 44;
     a.temperature = d_temperature; a.top_k = d_top_k; a.top_p = d_top_p; a.min_p = d_min_p; a.u = d_u; a.token = d_token; a.prob = d_prob;
-    a.limbs = d_top_p ? 3 : d_top_k ? 1 : 0;
     return type == TY_F32 ? launch_sample<float>(a, on.dev, stream) : type == TY_F16 ? launch_sample<__half>(a, on.dev, stream) : launch_sample<__nv_bfloat16>(a, on.dev, stream);
 }
 

@@ -331,13 +331,21 @@ def flash_decode_noalloc(d_q: int, d_k: int, d_v: int, M: int, H: int, n_head_kv
 
 
 _SERVE_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 30}
+_dtype_names = {}                       # torch.dtype -> its name: printing one takes longer than the other checks of a tensor together
+
+
+def _dtype(t) -> str:
+    name = _dtype_names.get(t.dtype)
+    if name is None:
+        name = _dtype_names[t.dtype] = str(t.dtype)
+    return name
 
 
 def _array(t, dtype: str, n: int, what: str):
     """Address of a contiguous device tensor of n elements or more; None stays None."""
     if t is None:
         return None
-    if str(t.dtype) != dtype or t.numel() < n or not t.is_contiguous():
+    if _dtype(t) != dtype or t.numel() < n or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous {dtype} tensor of {n} elements is wanted, not {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
@@ -349,7 +357,7 @@ def _rows(t, heads: int, dim: int, what: str):
         ok = shape[1] == heads and shape[2] == dim and (dim == 1 or stride[2] == 1) and (heads == 1 or stride[1] == dim)
     else:
         ok = len(shape) == 2 and shape[1] == heads * dim and stride[1] == 1
-    kind = _SERVE_TYPES.get(str(t.dtype))
+    kind = _SERVE_TYPES.get(_dtype(t))
     if not ok or kind is None:
         raise ValueError(f"{what}: rows of {heads} heads of {dim} are wanted, not {t.dtype} {tuple(shape)} with strides {stride}")
     return t.data_ptr(), kind, max(stride[0], heads * dim) if shape[0] < 2 else stride[0], shape[0]
@@ -368,7 +376,7 @@ class PagedCache:
     The calls enqueue on `stream` (a raw stream handle, 0: the default stream) and wait for nothing."""
 
     def __init__(self, k, v, table, length, free=None, n_free=None, status=None):
-        kind = _SERVE_TYPES.get(str(k.dtype))
+        kind = _SERVE_TYPES.get(_dtype(k))
         if kind is None or k.dtype != v.dtype or k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or (k.shape[3] > 1 and k.stride(3) != 1):
             raise ValueError(f"k and v: two tensors [pages, page_size, kv_heads, head_dim] of one type and layout are wanted, not {k.dtype} {tuple(k.shape)} "
                              f"{k.stride()} and {v.dtype} {tuple(v.shape)} {v.stride()}")
@@ -430,7 +438,7 @@ def sample(logits, u, token, prob=None, temperature=None, top_k=None, top_p=None
     """One token from each row of logits [rows, vocab] (device tensors; float32, float16, bfloat16) into token (int32) with the random
     numbers u in [0, 1) (float32); prob (float32): its share of what was kept.  temperature, top_p, min_p (float32) and top_k (int32) have
     one value a row; None: 1, or off.  The order of the filters and the draw are described in include/lg_serve.h."""
-    kind = _SERVE_TYPES.get(str(logits.dtype))
+    kind = _SERVE_TYPES.get(_dtype(logits))
     if kind is None or len(logits.shape) != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError(f"logits: a float tensor [rows, vocab] with contiguous rows is wanted, not {logits.dtype} {tuple(logits.shape)}")
     rows, vocab = logits.shape

@@ -279,8 +279,9 @@ struct LgPagedAttnArgs {
     float scale;                       // times log2(e)
     const int *start;
     int gqa, group_rows;               // query heads of a KV head, query rows of an item
+    int whole;                         // pages are whole slices
     float *part; float2 *part_ml;      // [CTA][2][query row of an item]: unnormalised output; maximum and sum
-    int4 *jobs;                        // [CTA]: the item that it leaves unfinished (request, head and group, last CTA, rows), or -1
+    int4 *jobs;                        // [CTA]: the item that it leaves unfinished (first row of the request, KV head, last CTA, first of its rows and their number), or -1
 };
 
 // The block of rows of request r: first row, rows to compute, rows it has.
@@ -300,71 +301,6 @@ __device__ __forceinline__ int paged_len(const LgPagedAttnArgs &a, int r) {
     return len;
 }
 
-// One query row and head per CTA (grid: rows of a block, heads, requests), a key per warp at a time, softmax with a running maximum and sum:
-//   m' = max(m, s),  l' = l 2^(m - m') + 2^(s - m'),  o' = o 2^(m - m') + 2^(s - m') v
-// Sums in f32.  The queries of a KV head each read its rows on their own.
-#define LG_PATTN_WARPS 8
-template <typename TQ, typename TC> __global__ void __launch_bounds__(LG_PATTN_WARPS * 32) lg_paged_attn_rows_kernel(LgPagedAttnArgs a) {
-    __shared__ float po[LG_PATTN_WARPS][512], pm[LG_PATTN_WARPS], pl[LG_PATTN_WARPS];
-    const int t = blockIdx.x, h = blockIdx.y, r = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int first, m, held;
-    paged_rows(a, r, first, m, held);
-    if (t >= m) return;
-    const int hd = a.c.hd, units = hd >> 3, ps = a.c.page_size;
-    const int pos = paged_len(a, r) - held + t;
-    const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    const long long head = (long long)(h / (a.n_heads / a.c.n_kv)) * a.c.head_stride;
-    const TQ *q = (const TQ *)a.q + (long long)(first + t) * a.ld_q + (long long)h * hd;
-    float qv[2][8], o[2][8] = {}, x[8], mx = -INFINITY, l = 0.0f;
-    #pragma unroll
-    for (int j = 0; j < 2; j++)
-        #pragma unroll
-        for (int i = 0; i < 8; i++) qv[j][i] = lane + 32 * j < units ? Elem<TQ>::get(q + (lane + 32 * j) * 8 + i) : 0.0f;
-    for (int key = lo + warp; key <= pos; key += LG_PATTN_WARPS) {
-        const int page = a.c.table[(size_t)r * a.c.table_stride + key / ps];
-        if (page < 0 || page >= a.c.n_pages) { paged_raise(a.c, LG_PAGED_BAD_PAGE); continue; }
-        const long long at = (long long)page * a.c.page_stride + (long long)(key % ps) * a.c.row_stride + head;
-        float s = 0.0f;
-        #pragma unroll
-        for (int j = 0; j < 2; j++)
-            if (lane + 32 * j < units) {
-                Elem<TC>::load8((const TC *)a.c.k + at + (lane + 32 * j) * 8, x);
-                #pragma unroll
-                for (int i = 0; i < 8; i++) s += qv[j][i] * x[i];
-            }
-        s = warp_sum(s) * a.scale;
-        const float m2 = fmaxf(mx, s), f = mx == -INFINITY ? 0.0f : exp2f(mx - m2), p = s == -INFINITY ? 0.0f : exp2f(s - m2);
-        mx = m2; l = l * f + p;
-        #pragma unroll
-        for (int j = 0; j < 2; j++)
-            if (lane + 32 * j < units) {
-                Elem<TC>::load8((const TC *)a.c.v + at + (lane + 32 * j) * 8, x);
-                #pragma unroll
-                for (int i = 0; i < 8; i++) o[j][i] = o[j][i] * f + p * x[i];
-            }
-    }
-    #pragma unroll
-    for (int j = 0; j < 2; j++)
-        if (lane + 32 * j < units)
-            #pragma unroll
-            for (int i = 0; i < 8; i++) po[warp][(lane + 32 * j) * 8 + i] = o[j][i];
-    if (lane == 0) { pm[warp] = mx; pl[warp] = l; }
-    __syncthreads();
-    float top = -INFINITY;
-    for (int w = 0; w < LG_PATTN_WARPS; w++) top = fmaxf(top, pm[w]);
-    float sum = 0.0f, f[LG_PATTN_WARPS];
-    #pragma unroll
-    for (int w = 0; w < LG_PATTN_WARPS; w++) { f[w] = pl[w] == 0.0f ? 0.0f : exp2f(pm[w] - top); sum += pl[w] * f[w]; }
-    TQ *out = (TQ *)a.out + (long long)(first + t) * a.ld_out + (long long)h * hd;
-    for (int d = threadIdx.x; d < hd; d += blockDim.x) {
-        float y = 0.0f;
-        #pragma unroll
-        for (int w = 0; w < LG_PATTN_WARPS; w++) y += po[w][d] * f[w];
-        out[d] = Elem<TQ>::put(sum == 0.0f ? 0.0f : y / sum);
-    }
-}
-
-// ---- 16-bit caches: tensor-core tiles, spans over the length, a merge ----------------------------
 // The work is a line of slices of 16 keys: request by request, KV head by KV head, group of 8 NT query rows by group (an item).  Every CTA of a
 // persistent grid takes a stretch of equal length of that line, so ragged lengths cost nothing; an item that one stretch holds is written at once,
 // of one that several stretches share each leaves (max, sum, unnormalised output), and lg_paged_merge_kernel adds those in their order.
@@ -377,7 +313,8 @@ template <typename TQ, typename TC> __global__ void __launch_bounds__(LG_PATTN_W
 //   S^T (16 keys x 8) = K Q^T, softmax with a running maximum per column in the accumulator's own lanes, O^T (16 dims x 8) += V^T P^T,
 // P^T turned from accumulator order into operand order by movmatrix.  Numerics: an f32 query enters as a sum of 16-bit parts (f16: 2 parts behind a
 // power of two per row, 22 bits; bf16: 3, 24 bits), P as 2 parts (3 where the answer is f32 and the cache bf16); P carries a factor 2^15 in f16 so that
-// weights down to 2^-29 of the largest stay normal numbers.  Everything else is f32.
+// weights down to 2^-29 of the largest stay normal numbers.  Everything else is f32.  Rows of an f32 cache are split in registers into three bf16 parts
+// (24 bits); of the nine products of parts the six that reach the last bits of an f32 are computed.
 #define LG_PA_MAX_CTAS 296             // two per SM
 #define LG_PA_ITEM_COST 6              // of an item beside its slices, in slices: queries in, warps' results together, rows out
 #define LG_PA_MIN_STRETCH 8
@@ -403,6 +340,8 @@ template <> __device__ __forceinline__ uint32_t split2<__nv_bfloat16>(float &x, 
     x -= __uint_as_float(w << 16); y -= __uint_as_float(w & 0xFFFF0000u);
     return w;
 }
+__device__ __forceinline__ float lds_f(uint32_t p) { float v; asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(p)); return v; }
+__device__ __forceinline__ float2 lds_f2(uint32_t p) { float2 v; asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(p)); return v; }
 __device__ __forceinline__ uint32_t movm(uint32_t a) {
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -454,13 +393,17 @@ struct LgWalk {
 };
 
 template <typename TQ, typename TC, int HD, int NT> struct LgPagedTile {
-    static constexpr bool SAME = sizeof(TQ) == 2;
+    typedef typename std::conditional<std::is_same<TC, __half>::value, __half, __nv_bfloat16>::type TM;      // the matrix instructions' type
+    static constexpr bool SAME = sizeof(TQ) == 2, F32 = sizeof(TC) == 4;
     static constexpr bool F16 = std::is_same<TC, __half>::value;
     static constexpr int NQ = SAME ? 1 : F16 ? 2 : 3;                         // parts of a query
     static constexpr int NP = SAME || F16 ? 2 : 3;                            // parts of a weight
     static constexpr int KS = HD / 16;
     static constexpr int ROWS = 8 * NT;
-    static constexpr int UNIT = 16 * HD * 2;
+    static constexpr int ROW = HD * (int)sizeof(TC), UNIT = 16 * ROW, CHUNKS = ROW / 16;
+    // Chunk of 16 bytes that a row's chunk c lies in.  16-bit rows: eight rows' chunks in the eight 16-byte columns (ldmatrix); 32-bit rows: pairs of chunks so
+    // that neither rows g .. g + 3 (K) nor rows 0, 2, 4, 6 (V) of a column meet in a bank.
+    static __device__ __forceinline__ int place(int row, int c) { return F32 ? c ^ (((row ^ (row >> 2)) & 3) << 1) : c ^ (row & 7); }
     static constexpr int LDB = HD + 4;                                        // floats from row to row of the merge buffer: no bank conflicts
     static constexpr bool QREG = (NT * NQ * 2 + NT * 4) * KS <= 160;          // queries stay in registers beside the outputs
     static constexpr int Q_BYTES = NT * NQ * KS * 32 * 8, BUF_BYTES = ROWS * LDB * 4;
@@ -469,11 +412,11 @@ template <typename TQ, typename TC, int HD, int NT> struct LgPagedTile {
     // Two CTAs of 4 warps per SM where three units a warp fit (one merges while the other streams), else one of as many warps as fit
     static constexpr int CTAS = fixed(4) + 12 * UNIT <= 115712 ? 2 : 1;
     static constexpr int ROOM = CTAS == 2 ? 115712 : 232448;
-    static constexpr int W = CTAS == 2 ? 4 : fixed(8) + 24 * UNIT <= ROOM ? 8 : fixed(6) + 18 * UNIT <= ROOM ? 6 : fixed(4) + 12 * UNIT <= ROOM ? 4 : 3;
+    static constexpr int W = CTAS == 2 ? 4 : fixed(8) + 24 * UNIT <= ROOM ? 8 : fixed(6) + 18 * UNIT <= ROOM ? 6 : fixed(4) + 12 * UNIT <= ROOM ? 4 : fixed(3) + 9 * UNIT <= ROOM ? 3 : 2;
     static constexpr int U0 = (ROOM - fixed(W)) / (W * UNIT);
     static constexpr int U = U0 > 8 ? 8 : U0;
     static constexpr int SMEM = fixed(W) + W * U * UNIT;
-    static_assert(U >= 3, "a ring of three units at least");
+    static_assert(U >= 2, "a unit in use and one on its way");
 };
 
 template <typename TQ, typename TC, int HD, int NT>
@@ -530,10 +473,10 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
     }
     // the copies run ahead of the arithmetic with a walk of their own
     LgWalk p = w;
-    int ps = 0, ps_end = 0, n_issued = 0, slot_in = 0, page = -1;             // next slice of this warp, end of the item's slices
+    int ps = 0, ps_end = 0, n_issued = 0, slot_in = 0, page = -1, rem = 0, nth = 0;         // next slice of this warp, end of the item's slices
     long long poff = 0;
-    bool pread = false;
-    const int ps_size = a.c.page_size, hd8 = a.c.hd >> 3;
+    uint32_t pok = 0;
+    const int ps_size = a.c.page_size, row_chunks = a.c.hd * (int)sizeof(TC) / 16;
     auto begin_item = [&]() {                                                 // first slice of this warp in walk p's item, or the next item that has one
         while (p.valid(a)) {
             ps = p.q.s0 + p.begin() + warp;
@@ -544,40 +487,48 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
         return false;
     };
     bool more = begin_item();
-    auto fetch_page = [&]() {                                                 // page of this lane's row in slice ps (lanes 16..31: the same rows)
-        page = -1;
-        const int key = ps * 16 + (lane & 15);
+    // Pages ahead of their use.  Pages of whole slices: lane i looks up the page of this warp's i-th slice from here, one round of loads for 32 slices.
+    // Others: a lane per row of the next slice.
+    auto fetch_pages = [&]() {
+        page = -1; nth = 0;
         const int hi = p.q.len - p.q.held + p.q.m, lo = a.window > 0 ? p.q.len - p.q.held - a.window + 1 : 0;
-        if (key < hi && key >= lo) {
-            page = a.c.table[(size_t)p.r * a.c.table_stride + key / ps_size];
+        const int slice = a.whole ? ps + lane * P::W : ps, key = a.whole ? slice * 16 : slice * 16 + (lane & 15);
+        if (slice < ps_end && (a.whole || (key < hi && key >= lo))) {
+            const int n = key / ps_size;
+            page = a.c.table[(size_t)p.r * a.c.table_stride + n];
+            rem = key - n * ps_size;
             if (page < 0 || page >= a.c.n_pages) { paged_raise(a.c, LG_PAGED_BAD_PAGE); page = -1; }
         }
     };
-    if (more) fetch_page();
+    if (more) fetch_pages();
     const uint32_t ring_u32 = smem_u32(ring) + warp * (P::U * P::UNIT);
     auto issue = [&]() {                                                      // one unit: K of a slice, then its V
         if (more) {
             const bool is_v = n_issued & 1;
             if (!is_v) {
-                const int key = ps * 16 + (lane & 15);
-                pread = page >= 0;
-                poff = pread ? ((long long)page * a.c.page_stride + (long long)(key - key / ps_size * ps_size) * a.c.row_stride + (long long)(p.hg / p.q.groups) * a.c.head_stride) * 2 : 0;
-                const uint32_t ok = __ballot_sync(0xffffffffu, pread) & 0xFFFFu;
-                if (lane == 0) vmask[warp * 16 + ((n_issued >> 1) & 15)] = ok;
+                // rows of the slice that some query may see, and where they lie, a lane each (lanes 16 .. 31: the same rows)
+                const int hi = p.q.len - p.q.held + p.q.m, lo = a.window > 0 ? p.q.len - p.q.held - a.window + 1 : 0;
+                const int first = max(lo - ps * 16, 0), last = min(hi - ps * 16, 16);
+                int pg = page, rm = rem;
+                if (a.whole) { pg = __shfl_sync(0xffffffffu, page, nth); rm = __shfl_sync(0xffffffffu, rem, nth) + (lane & 15); }
+                poff = pg >= 0 ? ((long long)pg * a.c.page_stride + (long long)rm * a.c.row_stride + (long long)(p.hg / p.q.groups) * a.c.head_stride) * (int)sizeof(TC) : 0;
+                pok = a.whole ? pg >= 0 ? (0xFFFFu << first) & (0xFFFFu >> (16 - last)) : 0u : __ballot_sync(0xffffffffu, pg >= 0) & 0xFFFFu;
+                if (lane == 0) vmask[warp * 16 + ((n_issued >> 1) & 15)] = pok;
             }
             const unsigned char *base = (const unsigned char *)(is_v ? a.c.v : a.c.k);
             const uint32_t dst = ring_u32 + slot_in * P::UNIT;
             #pragma unroll
-            for (int i = 0; i < HD / 16; i++) {                               // 32 chunks of 16 bytes at a time
-                const int idx = i * 32 + lane, row = idx / (HD / 8), c = idx % (HD / 8);
+            for (int i = 0; i < P::CHUNKS / 2; i++) {                         // 32 chunks of 16 bytes at a time
+                const int idx = i * 32 + lane, row = idx / P::CHUNKS, c = idx % P::CHUNKS;
                 const long long off = __shfl_sync(0xffffffffu, poff, row);
-                const bool rd = __shfl_sync(0xffffffffu, (int)pread, row) && c < hd8;
-                cp_async16_or_zero(dst + row * (HD * 2) + ((c ^ (row & 7)) << 4), rd ? base + off + c * 16 : base, rd);
+                const bool rd = (pok >> row & 1) && c < row_chunks;
+                cp_async16_or_zero(dst + row * P::ROW + (P::place(row, c) << 4), rd ? base + off + c * 16 : base, rd);
             }
             if (is_v) {
                 ps += P::W;
-                if (ps >= ps_end) { p.next(a); more = begin_item(); }
-                if (more) fetch_page();
+                nth++;
+                if (ps >= ps_end) { p.next(a); more = begin_item(); nth = 32; }
+                if (more && (!a.whole || nth == 32)) fetch_pages();
             }
             n_issued++;
             if (++slot_in == P::U) slot_in = 0;
@@ -629,7 +580,7 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                     const int d = 64 * i + 2 * lane, ks = d >> 4, half = (d >> 3) & 1, t = (d & 7) >> 1;
                     #pragma unroll
                     for (int part = 0; part < P::NQ; part++)
-                        sq[((((n >> 3) * P::NQ + part) * P::KS + ks) * 32 + (n & 7) * 4 + t) * 2 + half] = split2<TC>(x[2 * i], x[2 * i + 1]);
+                        sq[((((n >> 3) * P::NQ + part) * P::KS + ks) * 32 + (n & 7) * 4 + t) * 2 + half] = split2<typename P::TM>(x[2 * i], x[2 * i + 1]);
                 }
                 if (lane == 0) cscale[n] = back;
             }
@@ -672,24 +623,33 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             for (int nt = 0; nt < NT; nt++)
                 #pragma unroll
                 for (int j = 0; j < 4; j++) sc[nt][0][j] = sc[nt][1][j] = 0.0f;
-            {
-                const int row = (lane & 7) + (lane & 8), c = lane >> 4;
-                #pragma unroll
-                for (int ks = 0; ks < P::KS; ks++) {
-                    uint32_t k4[4];
-                    ldsm_x4_u32(k4, at + row * (HD * 2) + (((2 * ks + c) ^ (row & 7)) << 4));
+            #pragma unroll
+            for (int ks = 0; ks < P::KS; ks++) {
+                uint32_t k4[P::F32 ? 3 : 1][4];                               // parts of 16 rows x 16 dims
+                if constexpr (P::F32) {
                     #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
+                    for (int e = 0; e < 4; e++) {
+                        const int row = g + (e & 1) * 8;
+                        float2 x = lds_f2(at + row * P::ROW + (P::place(row, 4 * ks + 2 * (e >> 1) + (t4 >> 1)) << 4) + (t4 & 1) * 8);
                         #pragma unroll
-                        for (int part = 0; part < P::NQ; part++) {
-                            const int i = (nt * P::NQ + part) * P::KS + ks;
-                            if (P::QREG) mma_16<TC>(sc[nt][ks & 1], k4, qr[2 * i], qr[2 * i + 1]);
-                            else {
-                                const uint2 v = *(const uint2 *)(sq + (i * 32 + lane) * 2);
-                                mma_16<TC>(sc[nt][ks & 1], k4, v.x, v.y);
-                            }
-                        }
+                        for (int part = 0; part < 3; part++) k4[part][e] = split2<typename P::TM>(x.x, x.y);
+                    }
+                } else {
+                    const int row = (lane & 7) + (lane & 8);
+                    ldsm_x4_u32(k4[0], at + row * P::ROW + (P::place(row, 2 * ks + (lane >> 4)) << 4));
                 }
+                #pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+                    #pragma unroll
+                    for (int part = 0; part < P::NQ; part++) {
+                        const int i = (nt * P::NQ + part) * P::KS + ks;
+                        uint2 v;
+                        if (P::QREG) v = make_uint2(qr[2 * i], qr[2 * i + 1]);
+                        else v = *(const uint2 *)(sq + (i * 32 + lane) * 2);
+                        #pragma unroll
+                        for (int own = 0; own < (P::F32 ? 3 : 1); own++)
+                            if (own + part < 3) mma_16<typename P::TM>(sc[nt][ks & 1], k4[own], v.x, v.y);
+                    }
             }
             const int k0 = s * 16;
             const bool all = ok == 0xFFFFu && k0 + 15 <= pos_lo && (a.window <= 0 || k0 > pos_hi - a.window);
@@ -725,8 +685,8 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                 }
                 #pragma unroll
                 for (int part = 0; part < P::NP; part++) {
-                    pb[nt][part][0] = movm(split2<TC>(x[0], x[1]));
-                    pb[nt][part][1] = movm(split2<TC>(x[2], x[3]));
+                    pb[nt][part][0] = movm(split2<typename P::TM>(x[0], x[1]));
+                    pb[nt][part][1] = movm(split2<typename P::TM>(x[2], x[3]));
                 }
             }
             if (__any_sync(0xffffffffu, moved)) {
@@ -742,17 +702,29 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             issue();
             at = ring_u32 + slot * P::UNIT;
             if (++slot == P::U) slot = 0;
-            {
-                const int row = (lane & 7) + ((lane >> 4) << 3), c = (lane >> 3) & 1;
-                #pragma unroll
-                for (int ks = 0; ks < P::KS; ks++) {
-                    uint32_t v4[4];
-                    ldsm_x4_t_u32(v4, at + row * (HD * 2) + (((2 * ks + c) ^ (row & 7)) << 4));
+            #pragma unroll
+            for (int ks = 0; ks < P::KS; ks++) {
+                uint32_t v4[P::F32 ? 3 : 1][4];                               // parts of 16 dims x 16 rows
+                if constexpr (P::F32) {
                     #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
+                    for (int e = 0; e < 4; e++) {
+                        const int row = 2 * t4 + (e >> 1) * 8, d = 16 * ks + (e & 1) * 8 + g;
+                        float x = lds_f(at + row * P::ROW + (P::place(row, d >> 2) << 4) + (d & 3) * 4);
+                        float y = lds_f(at + (row + 1) * P::ROW + (P::place(row + 1, d >> 2) << 4) + (d & 3) * 4);
                         #pragma unroll
-                        for (int part = 0; part < P::NP; part++) mma_16<TC>(o[ks][nt], v4, pb[nt][part][0], pb[nt][part][1]);
+                        for (int part = 0; part < 3; part++) v4[part][e] = split2<typename P::TM>(x, y);
+                    }
+                } else {
+                    const int row = (lane & 7) + ((lane >> 4) << 3);
+                    ldsm_x4_t_u32(v4[0], at + row * P::ROW + (P::place(row, 2 * ks + ((lane >> 3) & 1)) << 4));
                 }
+                #pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+                    #pragma unroll
+                    for (int part = 0; part < P::NP; part++)
+                        #pragma unroll
+                        for (int own = 0; own < (P::F32 ? 3 : 1); own++)
+                            if (own + part < 3) mma_16<typename P::TM>(o[ks][nt], v4[own], pb[nt][part][0], pb[nt][part][1]);
             }
         }
         // the warps' results into one, in warp order
@@ -795,7 +767,7 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
         // the item's other slices: before this stretch, behind it (its last slice then lies in the stretch of CTA `last`)
         const bool head = w.at < w.lo, tail = w.at + w.q.n_sl > w.hi;
         const long long part = ((long long)blockIdx.x * 2 + !head) * P::ROWS;
-        if (!head && tail && tid == 0) a.jobs[blockIdx.x] = make_int4(w.r, w.hg, (int)((w.at + w.q.n_sl - 1) / stretch), n_rows);
+        if (!head && tail && tid == 0) a.jobs[blockIdx.x] = make_int4(w.q.first, kvh, (int)((w.at + w.q.n_sl - 1) / stretch), row0 << 8 | n_rows);
         for (int n = warp; n < n_rows; n += P::W) {
             float m2 = -INFINITY, sum = 0.0f;
             #pragma unroll
@@ -822,30 +794,34 @@ template <typename TQ> __global__ void __launch_bounds__(256) lg_paged_merge_ker
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.y, b = blockIdx.x;
     pdl_wait();
     const int4 job = a.jobs[b];
-    if (job.x < 0 || n >= job.w) return;
-    const LgReq q = paged_request(a, job.x);
+    if (job.x < 0 || n >= (job.w & 255)) return;
     const int parts = job.z - b + 1;
     // part i: the last place of CTA b, the first one of those behind it
     auto place = [&](int i) { return ((long long)(b + i) * 2 + (i == 0)) * a.group_rows + n; };
+    float4 v[4];                                                              // dims lane * 4 .. of every 128
+    auto load = [&](int i) {
+        #pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int d = k * 128 + lane * 4;
+            if (d < a.c.hd) v[k] = *(const float4 *)(a.part + place(i) * a.c.hd + d);
+        }
+    };
+    if (warp < parts) load(warp);                                             // beside the maxima
     float top = -INFINITY;
     for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_ml[place(i)].x);
     top = warp_max(top);
     const float ref = top == -INFINITY ? 0.0f : top;
-    float y[16], sum = 0.0f;                                                  // dims lane * 4 .. of every 128
+    float y[16], sum = 0.0f;
     #pragma unroll
     for (int k = 0; k < 16; k++) y[k] = 0.0f;
     for (int i = warp; i < parts; i += 8) {
         const float2 ml = a.part_ml[place(i)];
         const float f = ex2(ml.x - ref);
         sum += ml.y * f;
+        if (i != warp) load(i);
         #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int d = k * 128 + lane * 4;
-            if (d < a.c.hd) {
-                const float4 v = *(const float4 *)(a.part + place(i) * a.c.hd + d);
-                y[4 * k] += v.x * f; y[4 * k + 1] += v.y * f; y[4 * k + 2] += v.z * f; y[4 * k + 3] += v.w * f;
-            }
-        }
+        for (int k = 0; k < 4; k++)
+            if (k * 128 + lane * 4 < a.c.hd) { y[4 * k] += v[k].x * f; y[4 * k + 1] += v[k].y * f; y[4 * k + 2] += v[k].z * f; y[4 * k + 3] += v[k].w * f; }
     }
     #pragma unroll
     for (int k = 0; k < 4; k++) {
@@ -858,8 +834,8 @@ template <typename TQ> __global__ void __launch_bounds__(256) lg_paged_merge_ker
     #pragma unroll
     for (int i = 0; i < 8; i++) sum += pl[i];
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int kvh = job.y / q.groups, rho = (job.y - kvh * q.groups) * a.group_rows + n, t = rho / a.gqa;
-    TQ *out = (TQ *)a.out + (long long)(q.first + t) * a.ld_out + (long long)(kvh * a.gqa + rho - t * a.gqa) * a.c.hd;
+    const int rho = (job.w >> 8) + n, t = rho / a.gqa;
+    TQ *out = (TQ *)a.out + (long long)(job.x + t) * a.ld_out + (long long)(job.y * a.gqa + rho - t * a.gqa) * a.c.hd;
     for (int d = threadIdx.x; d < a.c.hd; d += 256) {
         float x = 0.0f;
         #pragma unroll

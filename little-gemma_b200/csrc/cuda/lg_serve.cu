@@ -180,7 +180,7 @@ template <typename TQ, typename TC, int HD, int NT> int launch_attn_tile(LgPaged
     const int rows = a.n_new * a.gqa;
     return launch_serve("lg_paged_attn", lg_paged_merge_kernel<TQ>, dim3(grid - 1, rows < a.group_rows ? rows : a.group_rows), dim3(256), 0, stream, true, 1, a);
 }
-template <typename TQ, typename TC> int launch_attn_16(LgPagedAttnArgs &a, const AttnCut &k, int dev, void *stream) {
+template <typename TQ, typename TC> int launch_attn_type(LgPagedAttnArgs &a, const AttnCut &k, int dev, void *stream) {
     int rc;
     if (k.hd == 64) rc = k.nt == 1 ? launch_attn_tile<TQ, TC, 64, 1>(a, dev, stream) : k.nt == 2 ? launch_attn_tile<TQ, TC, 64, 2>(a, dev, stream) : launch_attn_tile<TQ, TC, 64, 4>(a, dev, stream);
     else if (k.hd == 128) rc = k.nt == 1 ? launch_attn_tile<TQ, TC, 128, 1>(a, dev, stream) : k.nt == 2 ? launch_attn_tile<TQ, TC, 128, 2>(a, dev, stream) : launch_attn_tile<TQ, TC, 128, 4>(a, dev, stream);
@@ -225,14 +225,13 @@ extern "C" int lg_paged_attn(const struct lg_paged_cache *c, const void *d_q, in
     a.c = paged_of(c); a.q = d_q; a.out = d_out; a.ld_q = ld_q; a.ld_out = ld_out; a.n_req = n_req; a.n_new = n_new; a.n_rows = n_rows;
     a.n_heads = n_heads; a.window = window; a.start = d_start;
     a.scale = (scale > 0.0f ? scale : 1.0f / sqrtf((float)c->head_dim)) * LG_LOG2E;
-    a.gqa = n_heads / c->n_kv_heads; a.group_rows = 8 * k.nt;
+    a.gqa = n_heads / c->n_kv_heads; a.group_rows = 8 * k.nt; a.whole = c->page_size % 16 == 0;
     a.jobs = (int4 *)d_work;
     a.part = (float *)(a.jobs + LG_PA_MAX_CTAS);
     a.part_ml = (float2 *)(a.part + LG_PA_MAX_CTAS * 2LL * a.group_rows * c->head_dim);
-    if (c->type == TY_F32)
-        return launch_serve("lg_paged_attn", lg_paged_attn_rows_kernel<float, float>, dim3(n_new, n_heads, n_req), dim3(LG_PATTN_WARPS * 32), 0, stream, false, 1, a);
-    if (c->type == TY_F16) return type == TY_F32 ? launch_attn_16<float, __half>(a, k, on.dev, stream) : launch_attn_16<__half, __half>(a, k, on.dev, stream);
-    return type == TY_F32 ? launch_attn_16<float, __nv_bfloat16>(a, k, on.dev, stream) : launch_attn_16<__nv_bfloat16, __nv_bfloat16>(a, k, on.dev, stream);
+    if (c->type == TY_F32) return launch_attn_type<float, float>(a, k, on.dev, stream);
+    if (c->type == TY_F16) return type == TY_F32 ? launch_attn_type<float, __half>(a, k, on.dev, stream) : launch_attn_type<__half, __half>(a, k, on.dev, stream);
+    return type == TY_F32 ? launch_attn_type<float, __nv_bfloat16>(a, k, on.dev, stream) : launch_attn_type<__nv_bfloat16, __nv_bfloat16>(a, k, on.dev, stream);
 }
 
 namespace {

@@ -371,18 +371,23 @@ __device__ __forceinline__ LgReq paged_request(const LgPagedAttnArgs &a, int r) 
     q.n_sl = ((hi + 15) >> 4) - q.s0;
     return q;
 }
-__device__ __forceinline__ long long paged_weight(const LgPagedAttnArgs &a, const LgReq &q) { return (long long)(q.n_sl + LG_PA_ITEM_COST) * q.groups * a.c.n_kv; }
+// Places of an item in the line: its slices and a cost of its own, or, where short stretches suffice (pad), whole stretches
+template <int W> __device__ __forceinline__ int paged_weight(const LgReq &q, bool pad) {
+    constexpr int least = (LG_PA_MIN_STRETCH + W - 1) / W * W;
+    return pad ? max(1, (q.n_sl + least - 1) / least) * least : q.n_sl + LG_PA_ITEM_COST;
+}
 
 // The walk of one CTA over the items that begin before the end of its stretch lo .. hi-1 of the line.
-struct LgWalk {
+template <int W> struct LgWalk {
     LgReq q;
+    bool pad;
     int r, hg;                         // request, KV head * groups + group
     long long at, lo, hi;              // where the item begins; the stretch
     __device__ __forceinline__ bool valid(const LgPagedAttnArgs &a) const { return r < a.n_req && at < hi; }
     __device__ __forceinline__ int begin() const { return (int)max(lo - at, 0LL); }                        // the item's slices in the stretch
     __device__ __forceinline__ int end() const { return (int)min(hi - at, (long long)q.n_sl); }
     __device__ __forceinline__ void next(const LgPagedAttnArgs &a) {
-        at += q.n_sl + LG_PA_ITEM_COST;
+        at += paged_weight<W>(q, pad);
         hg++;
         while (r < a.n_req && hg >= q.groups * a.c.n_kv) {                    // past requests without rows
             if (++r < a.n_req) {
@@ -408,7 +413,7 @@ template <typename TQ, typename TC, int HD, int NT> struct LgPagedTile {
     static constexpr bool QREG = (NT * NQ * 2 + NT * 4) * KS <= 160;          // queries stay in registers beside the outputs
     static constexpr int Q_BYTES = NT * NQ * KS * 32 * 8, BUF_BYTES = ROWS * LDB * 4;
     static constexpr int SHARED = QREG ? (Q_BYTES > BUF_BYTES ? Q_BYTES : BUF_BYTES) : Q_BYTES + BUF_BYTES;   // in registers they need the room only on the way
-    static constexpr int fixed(int w) { return SHARED + 2 * w * ROWS * 8 + ROWS * 4 + 128 + w * 16 * 4; }
+    static constexpr int fixed(int w) { return SHARED + 2 * w * ROWS * 8 + ROWS * 4 + 144 + w * 16 * 4; }
     // Two CTAs of 4 warps per SM where three units a warp fit (one merges while the other streams), else one of as many warps as fit
     static constexpr int CTAS = fixed(4) + 12 * UNIT <= 115712 ? 2 : 1;
     static constexpr int ROOM = CTAS == 2 ? 115712 : 232448;
@@ -428,51 +433,64 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
     float *buf = P::QREG ? (float *)sq : (float *)((unsigned char *)sq + P::Q_BYTES);      // [row][LDB]
     float2 *stats = (float2 *)((unsigned char *)sq + P::SHARED);              // [2][warp][row]: max, sum; items take turns
     float *cscale = (float *)(stats + 2 * P::W * P::ROWS);                  // [row]: scale of the scores
-    long long *red = (long long *)(cscale + P::ROWS);                         // 16 words
-    uint32_t *vmask = (uint32_t *)(red + 16);                                  // [warp][16]: keys of a slice that are there
+    long long *red = (long long *)(cscale + P::ROWS);                         // 18 words
+    uint32_t *vmask = (uint32_t *)(red + 18);                                  // [warp][16]: keys of a slice that are there
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     pdl_launch();
 
     // this CTA's stretch: weights of all requests, thread by thread, and where the stretch begins
-    LgWalk w;
+    LgWalk<P::W> w;
     long long stretch;
     {
         const int per = (a.n_req + P::W * 32 - 1) / (P::W * 32), r0 = min(a.n_req, tid * per), r1 = min(a.n_req, r0 + per);
-        long long mine = 0;
-        for (int r = r0; r < r1; r++) mine += paged_weight(a, paged_request(a, r));
-        long long s = mine;
+        long long mine[2] = {0, 0}, s[2], before[2] = {0, 0}, total[2] = {0, 0};
+        for (int r = r0; r < r1; r++) {
+            const LgReq q = paged_request(a, r);
+            const int items = q.groups * a.c.n_kv;
+            mine[0] += (long long)paged_weight<P::W>(q, false) * items; mine[1] += (long long)paged_weight<P::W>(q, true) * items;
+        }
         #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += x; }
-        if (lane == 31) red[warp] = s;
-        if (tid == 0) red[8] = a.n_req;
+        for (int k = 0; k < 2; k++) {
+            s[k] = mine[k];
+            #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, s[k], o); if (lane >= o) s[k] += x; }
+            if (lane == 31) red[2 * warp + k] = s[k];
+        }
+        if (tid == 0) red[16] = a.n_req;
         __syncthreads();
-        long long before = 0, total = 0;
         #pragma unroll
-        for (int i = 0; i < P::W; i++) { if (i < warp) before += red[i]; total += red[i]; }
-        before += s - mine;
-        stretch = max((long long)LG_PA_MIN_STRETCH, (total + gridDim.x - 1) / gridDim.x);
-        stretch = (stretch + P::W - 1) / P::W * P::W;
-        w.lo = stretch * blockIdx.x; w.hi = min(w.lo + stretch, total);
-        if (mine && before <= w.lo && w.lo < before + mine) {
+        for (int i = 0; i < P::W; i++)
+            #pragma unroll
+            for (int k = 0; k < 2; k++) { if (i < warp) before[k] += red[2 * i + k]; total[k] += red[2 * i + k]; }
+        // Stretches of the least length, if there are CTAs for them with no item's end inside of one: a CTA then has one item (each further one takes it
+        // about 3 us, of 13 for a short call)
+        constexpr int least = (LG_PA_MIN_STRETCH + P::W - 1) / P::W * P::W;
+        w.pad = total[1] <= (long long)least * gridDim.x;
+        const long long all = w.pad ? total[1] : total[0], own = w.pad ? mine[1] : mine[0];
+        long long at = w.pad ? before[1] + s[1] - mine[1] : before[0] + s[0] - mine[0];
+        stretch = w.pad ? least : max((long long)least, ((all + gridDim.x - 1) / gridDim.x + P::W - 1) / P::W * P::W);
+        w.lo = stretch * blockIdx.x; w.hi = min(w.lo + stretch, all);
+        if (own && at <= w.lo && w.lo < at + own) {
             int r = r0;
             for (;; r++) {
-                const long long x = paged_weight(a, paged_request(a, r));
-                if (w.lo < before + x) break;
-                before += x;
+                const LgReq q = paged_request(a, r);
+                const long long x = (long long)paged_weight<P::W>(q, w.pad) * q.groups * a.c.n_kv;
+                if (w.lo < at + x) break;
+                at += x;
             }
-            red[8] = r; red[9] = before;
+            red[16] = r; red[17] = at;
         }
         __syncthreads();
-        w.r = (int)red[8];
+        w.r = (int)red[16];
         if (tid == 0) a.jobs[blockIdx.x] = make_int4(-1, 0, 0, 0);
         if (w.r >= a.n_req) return;
         w.q = paged_request(a, w.r);
-        const int n = w.q.n_sl + LG_PA_ITEM_COST;
-        w.hg = (int)((w.lo - red[9]) / n);
-        w.at = red[9] + (long long)w.hg * n;
+        const int n = paged_weight<P::W>(w.q, w.pad);
+        w.hg = (int)((w.lo - red[17]) / n);
+        w.at = red[17] + (long long)w.hg * n;
     }
     // the copies run ahead of the arithmetic with a walk of their own
-    LgWalk p = w;
+    LgWalk<P::W> p = w;
     int ps = 0, ps_end = 0, n_issued = 0, slot_in = 0, page = -1, rem = 0, nth = 0;         // next slice of this warp, end of the item's slices
     long long poff = 0;
     uint32_t pok = 0;

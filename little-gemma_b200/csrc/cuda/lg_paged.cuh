@@ -16,30 +16,13 @@ struct LgPaged {                       // struct lg_paged_cache as the kernels n
 
 __device__ __forceinline__ void paged_raise(const LgPaged &c, int bit) { if (c.status) atomicOr(c.status, bit); }
 
-// Element types.  8 elements at a time: one 16-byte word of a 16-bit type, two of f32.
+// Element types.  store8: 8 elements rounded into a 16-byte word.
 template <typename T> struct Elem;
 template <> struct Elem<float> {
-    static __device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
-        const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    }
-    static __device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
-        *(float4 *)p = make_float4(x[0], x[1], x[2], x[3]);
-        *(float4 *)(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
-    }
     static __device__ __forceinline__ float get(const float *p) { return *p; }
     static __device__ __forceinline__ float put(float x) { return x; }
 };
 template <> struct Elem<__half> {
-    static __device__ __forceinline__ void load8(const __half *p, float (&x)[8]) {
-        const uint4 a = *(const uint4 *)p;
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-        #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = __half22float2(*(const __half2 *)&w[i]);
-            x[2 * i] = f.x; x[2 * i + 1] = f.y;
-        }
-    }
     static __device__ __forceinline__ void store8(__half *p, const float (&x)[8]) {
         uint32_t w[4];
         #pragma unroll
@@ -50,12 +33,6 @@ template <> struct Elem<__half> {
     static __device__ __forceinline__ __half put(float x) { return __float2half_rn(x); }
 };
 template <> struct Elem<__nv_bfloat16> {
-    static __device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&x)[8]) {
-        const uint4 a = *(const uint4 *)p;
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-        #pragma unroll
-        for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
-    }
     static __device__ __forceinline__ void store8(__nv_bfloat16 *p, const float (&x)[8]) {
         uint32_t w[4];
         #pragma unroll
@@ -242,29 +219,70 @@ struct LgAppendArgs {
     const int *slot;
 };
 
-// A thread moves 8 elements of a row at a time, K's then V's; bound by the bytes in and out.
-template <typename TI, typename TC> __global__ void __launch_bounds__(256) lg_paged_append_kernel(LgAppendArgs a) {
-    const int per_head = a.c.hd >> 3, half = per_head * a.c.n_kv, units = 2 * half;
-    const long long all = (long long)a.n * units;
-    const long long n_slots = (long long)a.c.n_pages * a.c.page_size;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (long long)gridDim.x * blockDim.x) {
-        const int row = (int)(i / units);
-        int u = (int)(i - (long long)row * units);
-        const bool is_v = u >= half;
-        if (is_v) u -= half;
-        const int slot = a.slot[row];
-        if (slot < 0 || slot >= n_slots) { if (slot != -1) paged_raise(a.c, LG_PAGED_BAD_SLOT); continue; }
-        const int page = slot / a.c.page_size, head = u / per_head;
-        const TI *src = (const TI *)(is_v ? a.v : a.k) + (is_v ? a.ld_v : a.ld_k) * row + u * 8;
-        TC *dst = (TC *)(is_v ? a.c.v : a.c.k) + (long long)page * a.c.page_stride + (long long)(slot - page * a.c.page_size) * a.c.row_stride +
-                  head * a.c.head_stride + (u - head * per_head) * 8;
-        float x[8];
-        if (a.wide) Elem<TI>::load8(src, x);
-        else {
+#define LG_APPEND_THREADS 256
+
+// Eight elements on their way from a row to the cache: as they are, or rounded.
+template <typename TI, typename TC> struct Eight {
+    float x[8];
+    __device__ __forceinline__ void load(const TI *p, bool wide) {
+        if (wide) {
+            const float4 a = __ldcs((const float4 *)p), b = __ldcs((const float4 *)(p + 4));
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        } else {
             #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = Elem<TI>::get(src + j);
+            for (int j = 0; j < 8; j++) x[j] = p[j];
         }
-        Elem<TC>::store8(dst, x);
+    }
+    __device__ __forceinline__ void store(TC *p) const { Elem<TC>::store8(p, x); }
+};
+template <typename T> struct Eight<T, T> {
+    uint4 x[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T *p, bool wide) {
+        if (wide) {
+            #pragma unroll
+            for (int j = 0; j < (int)sizeof(T) / 2; j++) x[j] = __ldcs((const uint4 *)p + j);
+        } else {
+            T *e = (T *)x;
+            #pragma unroll
+            for (int j = 0; j < 8; j++) e[j] = p[j];
+        }
+    }
+    __device__ __forceinline__ void store(T *p) const {
+        #pragma unroll
+        for (int j = 0; j < (int)sizeof(T) / 2; j++) ((uint4 *)p)[j] = x[j];
+    }
+};
+
+// A thread moves 8 elements of a row at a time, two such pieces under way, K's and V's; a CTA has one row, or as many whole ones as its threads cover, and
+// goes on to the next.  Rows of one type are not looked at.  Bound by the bytes in and out, or by latency.
+template <typename TI, typename TC> __global__ void __launch_bounds__(LG_APPEND_THREADS) lg_paged_append_kernel(LgAppendArgs a) {
+    const int per_head = a.c.hd >> 3, half = per_head * a.c.n_kv, units = 2 * half;
+    const int here = units < LG_APPEND_THREADS ? (int)threadIdx.x / units : 0, rows = units < LG_APPEND_THREADS ? LG_APPEND_THREADS / units : 1;
+    const int u0 = (int)threadIdx.x - here * units;
+    const bool packed = a.c.head_stride == a.c.hd;
+    const int n_slots = a.c.n_pages * a.c.page_size;
+    if (here >= rows) return;
+    for (long long row = (long long)blockIdx.x * rows + here; row < a.n; row += (long long)gridDim.x * rows) {
+        const int slot = a.slot[row];
+        const TI *k = (const TI *)a.k + a.ld_k * row, *v = (const TI *)a.v + a.ld_v * row;
+        for (int u = u0; u < units; u += 2 * LG_APPEND_THREADS) {
+            Eight<TI, TC> x[2];                                               // on their way before the slot is looked at
+            #pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const int w = u + q * LG_APPEND_THREADS;
+                if (w < units) x[q].load(w < half ? k + w * 8 : v + (w - half) * 8, a.wide);
+            }
+            if (slot < 0 || slot >= n_slots) { if (slot != -1) paged_raise(a.c, LG_PAGED_BAD_SLOT); break; }
+            const int page = slot / a.c.page_size;
+            const long long to = (long long)page * a.c.page_stride + (long long)(slot - page * a.c.page_size) * a.c.row_stride;
+            #pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const int w = u + q * LG_APPEND_THREADS, c = w < half ? w : w - half;
+                long long at = to + c * 8;
+                if (!packed) { const int head = c / per_head; at += head * (a.c.head_stride - a.c.hd); }
+                if (w < units) x[q].store((TC *)(w < half ? a.c.k : a.c.v) + at);
+            }
+        }
     }
 }
 

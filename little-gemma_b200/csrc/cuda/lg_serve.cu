@@ -62,6 +62,16 @@ template <typename K> bool allow_smem(K *kernel, size_t bytes, size_t most, int 
     return true;
 }
 
+int device_sms(int dev) {
+    static int n[64];
+    int v = dev < 64 ? n[dev] : 0;
+    if (!v) {
+        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); v = 148; }
+        if (dev < 64) n[dev] = v;
+    }
+    return v;
+}
+
 // NULL where the description of a cache is good, else what is wrong with it
 const char *cache_fault(const struct lg_paged_cache *c) {
     if (!c || !c->k || !c->v || !c->table || !c->len) return "a NULL pointer in the cache";
@@ -134,26 +144,17 @@ extern "C" int lg_paged_append(const struct lg_paged_cache *c, const void *d_k, 
     LgAppendArgs a;
     a.c = paged_of(c); a.k = d_k; a.v = d_v; a.ld_k = ld_k; a.ld_v = ld_v; a.n = n; a.slot = d_slot;
     a.wide = !(((uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)(ld_k * eb) | (uintptr_t)(ld_v * eb)) & 15);
-    const long long blocks = ((long long)n * width / 4 + 255) / 256;
-    const dim3 grid((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8));
+    const long long units = width / 4, rows = units < LG_APPEND_THREADS ? LG_APPEND_THREADS / units : 1;
+    const long long ctas = (n + rows - 1) / rows, most = device_sms(on.dev) * 8LL;
+    const dim3 grid((unsigned)(ctas < most ? ctas : most));
     void (*kernel)(LgAppendArgs) = nullptr;
     if (c->type == TY_F32) kernel = lg_paged_append_kernel<float, float>;
     else if (c->type == TY_F16) kernel = type == TY_F32 ? lg_paged_append_kernel<float, __half> : lg_paged_append_kernel<__half, __half>;
     else kernel = type == TY_F32 ? lg_paged_append_kernel<float, __nv_bfloat16> : lg_paged_append_kernel<__nv_bfloat16, __nv_bfloat16>;
-    return launch_serve("lg_paged_append", kernel, grid, dim3(256), 0, stream, false, 1, a);
+    return launch_serve("lg_paged_append", kernel, grid, dim3(LG_APPEND_THREADS), 0, stream, false, 1, a);
 }
 
 namespace {
-int device_sms(int dev) {
-    static int n[64];
-    int v = dev < 64 ? n[dev] : 0;
-    if (!v) {
-        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); v = 148; }
-        if (dev < 64) n[dev] = v;
-    }
-    return v;
-}
-
 // Query rows of an item, 8 nt: more rows share one read of the cache and more matrix work; 8 nt x head_dim outputs have to fit a
 // warp's registers.
 struct AttnCut { int hd, nt; };

@@ -256,15 +256,14 @@ template <typename T> struct LgSampler {
         if (const uint32_t v = (uint32_t)(x >> 30)) atomicAdd(h + 2 * LG_SAMPLE_BINS + bin, v);
     }
     // The first bin at which before + the running sum of v reaches the target, and the sum before it; the last bin where none does (found = false).
-    // `slot` keeps two results of one call apart.
-    template <int N> __device__ bool first_reaching(const u64 (&v)[N], u64 before, u64 target, int slot, int &bin, u64 &sum) {
+    template <int N> __device__ bool first_reaching(const u64 (&v)[N], u64 before, u64 target, int &bin, u64 &sum) {
         u64 mine = 0;
         #pragma unroll
         for (int j = 0; j < N; j++) mine += v[j];
         const u64 incl = warp_scan_u64(mine, lane);
         __syncthreads();
         if (lane == 31) red[warp] = incl;
-        if (threadIdx.x == 0) red[2 * LG_SAMPLE_WARPS + slot] = ~0ull;
+        if (threadIdx.x == 0) red[2 * LG_SAMPLE_WARPS] = ~0ull;
         __syncthreads();
         const u64 ws = lane < LG_SAMPLE_WARPS ? red[lane] : 0, wi = warp_scan_u64(ws, lane);
         u64 at = before + incl - mine + __shfl_sync(0xffffffffu, wi - ws, warp);
@@ -273,15 +272,36 @@ template <typename T> struct LgSampler {
             int k = 0;
             #pragma unroll
             for (int j = 0; j < N - 1; j++) if (k == j && at + v[j] < target) { at += v[j]; k++; }
-            red[2 * LG_SAMPLE_WARPS + slot] = threadIdx.x * N + k;
-            red[2 * LG_SAMPLE_WARPS + 2 + slot] = at;
+            red[2 * LG_SAMPLE_WARPS] = threadIdx.x * N + k;
+            red[2 * LG_SAMPLE_WARPS + 1] = at;
         }
         __syncthreads();
-        const u64 b = red[2 * LG_SAMPLE_WARPS + slot];
+        const u64 b = red[2 * LG_SAMPLE_WARPS];
         const bool found = b != ~0ull;
         bin = found ? (int)b : N * LG_SAMPLE_THREADS - 1;
-        sum = found ? red[2 * LG_SAMPLE_WARPS + 2 + slot] : all;
+        sum = found ? red[2 * LG_SAMPLE_WARPS + 1] : all;
         return found;
+    }
+    // The bins at which the running sums of `up` and of `low` (smaller ones) first reach the target, four bins a thread
+    __device__ void bracket(const u64 (&up)[4], const u64 (&low)[4], u64 target, int &b0, int &b1) {
+        const u64 mine[2] = {up[0] + up[1] + up[2] + up[3], low[0] + low[1] + low[2] + low[3]}, incl[2] = {warp_scan_u64(mine[0], lane), warp_scan_u64(mine[1], lane)};
+        __syncthreads();
+        if (lane == 31) { red[warp] = incl[0]; red[LG_SAMPLE_WARPS + warp] = incl[1]; }
+        if (threadIdx.x < 2) red[2 * LG_SAMPLE_WARPS + threadIdx.x] = LG_SAMPLE_COARSE - 1;
+        __syncthreads();
+        #pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const u64 ws = lane < LG_SAMPLE_WARPS ? red[h * LG_SAMPLE_WARPS + lane] : 0, wi = warp_scan_u64(ws, lane);
+            u64 at = incl[h] - mine[h] + __shfl_sync(0xffffffffu, wi - ws, warp);
+            if (at < target && target <= at + mine[h]) {
+                int k = 0;
+                #pragma unroll
+                for (int j = 0; j < 3; j++) { const u64 v = h ? low[j] : up[j]; if (k == j && at + v < target) { at += v; k++; } }
+                red[2 * LG_SAMPLE_WARPS + h] = threadIdx.x * 4 + k;
+            }
+        }
+        __syncthreads();
+        b0 = (int)red[2 * LG_SAMPLE_WARPS]; b1 = (int)red[2 * LG_SAMPLE_WARPS + 1];
     }
     // Keys of the coarse bins b0 .. b1 with room on either side, within low .. top_key
     __device__ void interval(int b0, int b1, uint32_t low, uint32_t top_key, uint32_t &klo, uint32_t &khi) const {
@@ -324,10 +344,39 @@ template <typename T> struct LgSampler {
         #pragma unroll
         for (int j = 0; j < N; j++) { const int b = threadIdx.x * N + j; v[j] = ld_peer_u64(fine + b % per, b / per); }
     }
+    // The keys of a row's tokens from some threshold up, where every CTA has them (refine leaves them here): the histograms' place
+    __device__ __forceinline__ uint32_t *pool() const { return hist; }
+    // Rounds over tokens that this CTA has, eight a thread (x: what each counts): klo .. khi narrowed to the key at which the target is reached, `above`
+    // brought to what lies above it
+    __device__ void settle(const uint32_t (&key)[8], const u64 (&x)[8], u64 &above, u64 target, uint32_t &klo, uint32_t &khi) {
+        for (int round = 0; round < 4; round++) {                             // 10 bits of at most 32 a round
+            const int sh = shift_of(khi - klo);
+            fine[2 * threadIdx.x] = fine[2 * threadIdx.x + 1] = 0;
+            __syncthreads();
+            #pragma unroll
+            for (int q = 0; q < 8; q++) if (x[q] && key[q] >= klo && key[q] <= khi) atomicAdd(fine + ((khi - key[q]) >> sh), x[q]);
+            __syncthreads();
+            const u64 v[2] = {fine[2 * threadIdx.x], fine[2 * threadIdx.x + 1]};
+            int part;
+            first_reaching(v, above, target, part, above);
+            narrow(part, sh, klo, khi);
+            if (sh == 0) break;
+        }
+    }
+    // Sums of two numbers a thread over this CTA
+    __device__ void own_sum2(u64 x, u64 y, u64 &sx, u64 &sy) {
+        x = warp_sum_u64(x); y = warp_sum_u64(y);
+        __syncthreads();
+        if (lane == 0) { red[warp] = x; red[LG_SAMPLE_WARPS + warp] = y; }
+        __syncthreads();
+        const u64 v = warp_half_sum_u64(red[lane]);
+        sx = __shfl_sync(0xffffffffu, v, 0); sy = __shfl_sync(0xffffffffu, v, 16);
+    }
     // The threshold at which counts (weighted: weights) of the keys from the largest down reach the target; it lies in klo .. khi.  Kept then: keys
     // above t and `ties` of key t.  Passes that read the row itself note its tokens in the interval in the warp's list: over_w is then this lane's part
-    // of the warp's weight above the list's tokens and n_list their number; n_list < 0: there is no such list.
-    __device__ void refine(bool weighted, u64 target, uint32_t klo, uint32_t khi, uint32_t &t, u64 &ties, u64 &over_w, int &n_list) {
+    // of the warp's weight above the list's tokens and n_list their number; n_list < 0: there is no such list.  n_pool (or NULL): receives the number
+    // of keys left in pool(), where every CTA has fetched all of the interval's.
+    __device__ void refine(bool weighted, u64 target, uint32_t klo, uint32_t khi, uint32_t &t, u64 &ties, u64 &over_w, int &n_list, int *n_pool) {
         uint32_t *n_near = (uint32_t *)(red + 2 * LG_SAMPLE_WARPS + 4);
         u64 above, found;
         for (int wide = 0;; wide++) {
@@ -394,19 +443,12 @@ template <typename T> struct LgSampler {
                     const u64 v = mass(weighted, key_value<LOW>(key[q]));
                     if (i < found) x[q] = v;
                 }
-                for (int round = 0; round < 4; round++) {                     // 10 bits of at most 32 a round
-                    const int sh = shift_of(khi - klo);
-                    fine[2 * threadIdx.x] = fine[2 * threadIdx.x + 1] = 0;
-                    __syncthreads();
+                if (n_pool && wide == 0) {
                     #pragma unroll
-                    for (int q = 0; q < 8; q++) if (x[q] && key[q] >= klo && key[q] <= khi) atomicAdd(fine + ((khi - key[q]) >> sh), x[q]);
-                    __syncthreads();
-                    const u64 v[2] = {fine[2 * threadIdx.x], fine[2 * threadIdx.x + 1]};
-                    int part;
-                    first_reaching(v, above, target, 0, part, above);
-                    narrow(part, sh, klo, khi);
-                    if (sh == 0) break;
+                    for (int q = 0; q < 8; q++) if (threadIdx.x + q * LG_SAMPLE_THREADS < found) pool()[threadIdx.x + q * LG_SAMPLE_THREADS] = key[q];
+                    *n_pool = (int)found;
                 }
+                settle(key, x, above, target, klo, khi);
                 break;
             }
             // too many: one round of the whole cluster
@@ -433,7 +475,7 @@ template <typename T> struct LgSampler {
             u64 v[2];
             int part;
             shared_bins(v);
-            first_reaching(v, above, target, 0, part, above);
+            first_reaching(v, above, target, part, above);
             narrow(part, sh, klo, khi);
             n_list = -1;
             cluster_sync_all();                                               // `fine` and the lists are used again
@@ -539,6 +581,7 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
 
     uint32_t t = best == INFINITY ? top_key - 1 : LgSampler<T>::DEAD;          // threshold; at first everything above -inf
     u64 ties = 0, over_w = 0;
+    int n_pool = 0;                                     // keys in pool(): all from the threshold up
     int n_list = -1;                                    // >= 0: this warp's list and over_w say what it keeps (LgSampler::refine)
     if (top_k > 0 && top_k < a.vocab) {
         uint32_t *h = s.fresh_hist(LG_SAMPLE_COARSE);
@@ -558,14 +601,46 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
         u64 v[4], before;
         int bin;
         s.shared_bins(v);
-        if (s.first_reaching(v, 0, (u64)top_k, 0, bin, before)) {              // otherwise fewer than top_k tokens have a weight
+        if (s.first_reaching(v, 0, (u64)top_k, bin, before)) {              // otherwise fewer than top_k tokens have a weight
             uint32_t klo, khi;
             s.interval(bin, bin, t + 1, top_key, klo, khi);
             s.make_list(key_value<LOW>(klo));
-            s.refine(false, (u64)top_k, klo, khi, t, ties, over_w, n_list);
+            // few: every CTA fetches them all, and needs no other for top_p either
+            if (top_k <= 2048) khi = top_key;
+            s.refine(false, (u64)top_k, klo, khi, t, ties, over_w, n_list, top_k <= 2048 ? &n_pool : nullptr);
         }
     }
-    if (top_p < 1.0f) {
+    const u64 p64 = top_p < 1.0f ? __double2ull_rz((double)top_p * 18446744073709551616.0) : 0;
+    // the weight that top_p asks for of `total`
+    auto share = [&](u64 total) { const u64 w = __umul64hi(p64, total) + (p64 * total != 0); return w < 1 ? (u64)1 : w; };
+    if (top_p < 1.0f && n_pool) {
+        uint32_t key[8];
+        u64 x[8], over = 0, at_t = 0;
+        __syncthreads();
+        #pragma unroll
+        for (int q = 0; q < 8; q++) {
+            x[q] = 0; key[q] = 0;
+            if (q * LG_SAMPLE_THREADS + warp * 32 >= n_pool) continue;
+            const int i = tid + q * LG_SAMPLE_THREADS;
+            if (i < n_pool) key[q] = s.pool()[i];
+            const u64 v = s.mass(true, key_value<LOW>(key[q]));
+            if (i < n_pool && key[q] > t) { x[q] = v; over += v; }
+            at_t += i < n_pool && key[q] == t;
+        }
+        s.own_sum2(over, at_t, over, at_t);
+        const u64 one = s.mass(true, key_value<LOW>(t));
+        if (ties < at_t) at_t = ties;
+        const u64 target = share(over + at_t * one);
+        if (target > over) ties = min(ties, one ? (target - over + one - 1) / one : ties);
+        else {
+            uint32_t klo = t + 1, khi = top_key;
+            u64 above = 0;
+            s.settle(key, x, above, target, klo, khi);
+            t = khi;
+            const u64 w_t = s.mass(true, key_value<LOW>(t));
+            ties = w_t ? (target - above + w_t - 1) / w_t : 1;
+        }
+    } else if (top_p < 1.0f) {
         // weight above the threshold, tokens at it
         uint32_t *h = s.fresh_hist(LG_SAMPLE_COARSE);
         const float lt = key_value<LOW>(t);
@@ -589,29 +664,25 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
         s.sum2((u64)(long long)sum, n_at, over, at_t);
         const u64 one = (u64)(long long)LgWeight::whole(s.w.of(lt));
         if (ties < at_t) at_t = ties;
-        const u64 total = over + at_t * one, p64 = __double2ull_rz((double)top_p * 18446744073709551616.0);
-        u64 target = __umul64hi(p64, total) + (p64 * total != 0);
-        if (target < 1) target = 1;
+        const u64 target = share(over + at_t * one);
         if (target > over) ties = min(ties, one ? (target - over + one - 1) / one : ties);
         else {
             // a bin's tokens count 989 .. 1011 each: their weights in thousandths of the bin's own, to half of one
-            u64 c[4], v[4], before;
+            u64 c[4], v[4], low[4];
             int b0, b1;
-            double edge[4];
             s.share_bins(h, LG_SAMPLE_COARSE, 1);
             s.shared_bins(c);
             #pragma unroll
             for (int j = 0; j < 4; j++) {
-                edge[j] = (double)c[j] * (s.w.scaled(4 * tid + j, 0.0) * 0.001);
-                v[j] = __double2ull_ru(edge[j] * 1.0006) + c[j];              // (and half a unit for the rounding of each weight)
+                const double edge = (double)c[j] * (s.w.scaled(4 * tid + j, 0.0) * 0.001);
+                const u64 least = __double2ull_rd(edge * 0.9994);
+                v[j] = __double2ull_ru(edge * 1.0006) + c[j];                 // (and half a unit for the rounding of each weight)
+                low[j] = least > c[j] ? least - c[j] : 0;
             }
-            s.first_reaching(v, 0, target, 0, b0, before);
-            #pragma unroll
-            for (int j = 0; j < 4; j++) { const u64 low = __double2ull_rd(edge[j] * 0.9994); v[j] = low > c[j] ? low - c[j] : 0; }
-            s.first_reaching(v, 0, target, 1, b1, before);
+            s.bracket(v, low, target, b0, b1);
             uint32_t klo, khi;
             s.interval(b0, max(b0, b1), t + 1, top_key, klo, khi);
-            s.refine(true, target, klo, khi, t, ties, over_w, n_list);
+            s.refine(true, target, klo, khi, t, ties, over_w, n_list, nullptr);
         }
     }
     // the draw: what each warp's tokens weigh and how many lie at the threshold, then the warp in which the running weight passes the target

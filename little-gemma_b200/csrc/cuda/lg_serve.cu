@@ -241,16 +241,18 @@ namespace {
 // with 16384 tokens or more each, since a CTA's fixed work -- barriers, scans of histograms -- is done in each.  Measured, CTAs a row 1 / 2 / 4 / 8: one row of
 // 262144 - / 79 / 55 / 44 us, 48 rows - / 176 / 151 / 145, 200 rows - / 364 / 379 / 498, 64 rows of 32768 42 / 37 / 43 / 85, 512 rows of 32768 47 / 55 / 87 / 163.
 template <typename T> int launch_sample(LgSampleArgs &a, int dev, void *stream) {
-    const int sms = device_sms(dev), tools = a.top_k || a.top_p ? LG_SAMPLE_TOOLS : 0, room = 112 * 1024 - tools;
+    const int sms = device_sms(dev), tools = a.top_k || a.top_p ? LG_SAMPLE_TOOLS : 0;
     int ranks = 1;
     while (ranks < LG_SAMPLE_MAX_CLUSTER && (a.vocab > ranks << 17 || ((long long)a.rows * ranks * 2 <= sms && a.vocab / (ranks * 2) >= 4096) ||
                                              ((long long)a.rows * ranks * 2 <= 3 * sms && a.vocab / (ranks * 2) >= 16384))) ranks *= 2;
     a.slice = ((a.vocab + ranks - 1) / ranks + 127) / 128 * 128;
-    const long long held = room / (int)sizeof(T) / 128 * 128;
+    // shared memory for one CTA per SM where there are no more, else for two; what of the slice does not fit is read again
+    const int most = (long long)a.rows * ranks <= sms ? 220 * 1024 : 112 * 1024;
+    const long long held = (most - tools) / (int)sizeof(T) / 128 * 128;
     a.cap = (int)(a.slice < held ? a.slice : held);
     const size_t smem = (size_t)a.cap * sizeof(T) + tools;
     static unsigned char done[64];
-    if (!allow_smem(lg_sample_kernel<T>, smem, 112 * 1024, dev, done)) SERVE_FAIL(-6, "lg_sample: no %zu bytes of shared memory", smem);
+    if (!allow_smem(lg_sample_kernel<T>, smem, 220 * 1024, dev, done)) SERVE_FAIL(-6, "lg_sample: no %zu bytes of shared memory", smem);
     return launch_serve("lg_sample", lg_sample_kernel<T>, dim3((unsigned)a.rows * ranks), dim3(LG_SAMPLE_THREADS), smem, stream, false, ranks, a);
 }
 }  // namespace

@@ -82,6 +82,26 @@ def test_ties_go_to_the_lowest_index(lg, dtype):
     assert token.tolist() == [0, 249, 250]
 
 
+@pytest.mark.parametrize("dtype,vocab", [("float32", 262144), ("bfloat16", 262144), ("float32", 1000000), ("float16", 20000)])
+@pytest.mark.parametrize("spread", [1e-4, 0.05, 1.0])
+def test_flat_rows(lg, dtype, vocab, spread):
+    """Hundreds of thousands of tokens near a threshold: more than lists and single CTAs hold."""
+    rng = np.random.default_rng(vocab)
+    rows = 3
+    x = _logits(rows, vocab, dtype, seed=vocab, spread=spread)
+    x[:, ::7] = x[:, :1]
+    for f in (dict(top_p=0.5), dict(top_k=vocab // 3, top_p=0.7), dict(top_k=1500, top_p=0.9), dict(top_k=2049), dict(top_p=0.99, min_p=0.4), dict(temperature=5.0, top_p=0.3)):
+        _check(lg, x, rng.random(rows, dtype=np.float32), **f)
+
+
+@pytest.mark.parametrize("rows,vocab", [(40, 100000), (200, 33000), (90, 262144)])
+def test_rows_shared_by_other_numbers_of_ctas(lg, rows, vocab):
+    rng = np.random.default_rng(rows)
+    x = _logits(rows, vocab, "bfloat16", seed=rows)
+    for f in (dict(top_p=0.9), dict(top_k=60, top_p=0.8, min_p=0.05)):
+        _check(lg, x, rng.random(rows, dtype=np.float32), temperature=rng.choice([0.5, 1.0, 1.5, 0.0], rows), **f)
+
+
 def test_ruled_out_tokens_and_empty_rows(lg):
     import torch
     inf = float("inf")

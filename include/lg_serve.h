@@ -31,7 +31,8 @@ enum { LG_PAGED_NO_PAGES = 1, LG_PAGED_TOO_LONG = 2, LG_PAGED_NO_ROWS = 4, LG_PA
 
 /* A cache of many requests in pages of page_size rows.  The caller owns all of it.  Element (page, row, head, d) of k is
  * k[page * page_stride + row * row_stride + head * head_stride + d], the same for v: rows or heads may come first, and k and v may
- * lie in one array.  Strides are in elements and multiples of 8, as head_dim is (at most 512); k and v are 16-byte aligned. */
+ * lie in one array.  Strides are in elements and multiples of 8, as head_dim is (at most 512); k and v are 16-byte aligned; a request has
+ * at most 2^30 rows (max_pages * page_size), the cache at most 2^31 - 1. */
 struct lg_paged_cache {
     void *k, *v;
     long long page_stride, row_stride, head_stride;
@@ -67,7 +68,7 @@ int  lg_paged_append(const struct lg_paged_cache *c, const void *d_k, const void
  * as lg_paged_step wrote them, at most n_new of them (rows beyond are left as they are, with a status bit), and rows from d_start[n_req] on are left as
  * they are.  The last of a request's m rows is the query at position len - 1, row t the one at len - m + t; it sees the rows at its position and
  * before, with window > 0 the nearest `window` of them.  A query that sees nothing (a length of 0, pages that are not in the cache) gives
- * zeros.  scale 0: 1 / sqrt(head_dim).  Rows that a query sees are finite.  Every sum has an order that the call's sizes and lengths
+ * zeros.  scale 0: 1 / sqrt(head_dim).  What a query does not see does not reach it, inf and NaN included; K rows that it sees are finite.  Every sum has an order that the call's sizes and lengths
  * fix: the same call gives the same bits.
  * d_work: lg_paged_attn_work bytes, 16-byte aligned, this call's alone until the call's work has ended: calls and graphs that may
  * overlap have workspaces of their own. */

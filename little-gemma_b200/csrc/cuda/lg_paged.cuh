@@ -360,6 +360,25 @@ template <> __device__ __forceinline__ uint32_t split2<__nv_bfloat16>(float &x, 
 }
 __device__ __forceinline__ float lds_f(uint32_t p) { float v; asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(p)); return v; }
 __device__ __forceinline__ float2 lds_f2(uint32_t p) { float2 v; asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(p)); return v; }
+__device__ __forceinline__ uint4 lds_u4(uint32_t p) { uint4 v; asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p)); return v; }
+__device__ __forceinline__ uint16_t lds_u16(uint32_t p) { uint16_t v; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(p)); return v; }
+// One of two packed 16-bit numbers; one element of a cache in shared memory; whether inf or NaN is among 16 bytes of a cache
+template <typename T> __device__ __forceinline__ float half16(uint32_t w, int high);
+template <> __device__ __forceinline__ float half16<__half>(uint32_t w, int high) { const __half2 h = *(const __half2 *)&w; return high ? __high2float(h) : __low2float(h); }
+template <> __device__ __forceinline__ float half16<__nv_bfloat16>(uint32_t w, int high) { return __uint_as_float(high ? w & 0xFFFF0000u : w << 16); }
+template <typename T> __device__ __forceinline__ float lds_elem(uint32_t p);
+template <> __device__ __forceinline__ float lds_elem<float>(uint32_t p) { return lds_f(p); }
+template <> __device__ __forceinline__ float lds_elem<__half>(uint32_t p) { return __half2float(__ushort_as_half(lds_u16(p))); }
+template <> __device__ __forceinline__ float lds_elem<__nv_bfloat16>(uint32_t p) { return __uint_as_float((uint32_t)lds_u16(p) << 16); }
+template <typename T> __device__ __forceinline__ bool not_finite(uint4 v) {
+    constexpr uint32_t e = sizeof(T) == 4 ? 0x7F800000u : std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
+    bool odd = false;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    #pragma unroll
+    for (int i = 0; i < 4; i++)
+        odd |= sizeof(T) == 4 ? (w[i] & e) == e : (w[i] & e & 0xFFFF0000u) == (e & 0xFFFF0000u) || (w[i] & e & 0xFFFFu) == (e & 0xFFFFu);
+    return odd;
+}
 __device__ __forceinline__ uint32_t movm(uint32_t a) {
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -738,6 +757,39 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             issue();
             at = ring_u32 + slot * P::UNIT;
             if (++slot == P::U) slot = 0;
+            // A row that some queries of the block see and others do not (the last rows of a block, the first of its windows): if its V holds inf or NaN, 0 times that
+            // would reach those that do not see it, so such a slice is multiplied key by key.
+            bool plain = true;
+            if (!all && pos_lo != pos_hi) {
+                bool odd = false;
+                for (int i = lane; i < P::UNIT / 16; i += 32) odd |= not_finite<TC>(lds_u4(at + i * 16));
+                plain = !__any_sync(0xffffffffu, odd);
+            }
+            if (!plain) {
+                #pragma unroll
+                for (int half = 0; half < 2; half++)
+                    #pragma unroll 1
+                    for (int k = 0; k < 8; k++) {
+                        const int row = half * 8 + k, key = k0 + row;
+                        #pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+                            #pragma unroll
+                            for (int j = 0; j < 2; j++) {
+                                float x = 0.0f;                               // the weight, from the lane that has it as an operand
+                                #pragma unroll
+                                for (int part = P::NP - 1; part >= 0; part--) x += half16<typename P::TM>(__shfl_sync(0xffffffffu, pb[nt][part][half], (2 * t4 + j) * 4 + (k >> 1)), k & 1);
+                                if (!(ok >> row & 1) || key > top[nt][j] || (a.window > 0 && key <= top[nt][j] - a.window)) continue;
+                                #pragma unroll
+                                for (int ks = 0; ks < P::KS; ks++)
+                                    #pragma unroll
+                                    for (int h = 0; h < 2; h++) {
+                                        const int d = 16 * ks + 8 * h + g, byte = d * (int)sizeof(TC);
+                                        o[ks][nt][2 * h + j] += x * lds_elem<TC>(at + row * P::ROW + (P::place(row, byte >> 4) << 4) + (byte & 15));
+                                    }
+                            }
+                    }
+                continue;
+            }
             #pragma unroll
             for (int ks = 0; ks < P::KS; ks++) {
                 uint32_t v4[P::F32 ? 3 : 1][4];                               // parts of 16 dims x 16 rows

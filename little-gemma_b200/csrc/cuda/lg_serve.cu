@@ -80,7 +80,7 @@ const char *cache_fault(const struct lg_paged_cache *c) {
         return "a size of the cache out of range";
     if (c->head_dim < 8 || c->head_dim > 512 || c->head_dim % 8) return "head_dim is not a multiple of 8 up to 512";
     if ((long long)c->n_pages * c->page_size > 0x7fffffffLL) return "more slots than 2^31 - 1";
-    if ((long long)c->max_pages * c->page_size > 0x7fffffffLL - LG_PAGED_MAX_REQ) return "more rows in a request than fit an int";
+    if ((long long)c->max_pages * c->page_size > 1LL << 30 || c->n_kv_heads > 65535) return "more rows in a request than 2^30, or more KV heads than 65535";
     if (c->page_stride < 0 || c->row_stride < 0 || c->head_stride < 0 || (c->page_stride | c->row_stride | c->head_stride) % 8)
         return "a stride is negative or not a multiple of 8";
     if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return "k and v must be 16-byte aligned";
@@ -214,7 +214,7 @@ extern "C" int lg_paged_attn(const struct lg_paged_cache *c, const void *d_q, in
     const int eb = type_bytes(type);
     if (((uintptr_t)d_q | (uintptr_t)d_out) % eb || (uintptr_t)d_start & 3 || (uintptr_t)d_work & 15)
         SERVE_FAIL(-1, "lg_paged_attn: a misaligned pointer");
-    if (n_heads > 65535 || n_req > 65535 || (long long)n_req * n_new * n_heads > 1LL << 31) SERVE_FAIL(-2, "lg_paged_attn: %d requests of %d heads", n_req, n_heads);
+    if (n_heads > 65535 || n_rows > 1 << 30) SERVE_FAIL(-2, "lg_paged_attn: %d rows of %d heads", n_rows, n_heads);
     const long long need = lg_paged_attn_work(c, n_req, n_new, n_heads);
     if (work_bytes < need) SERVE_FAIL(-3, "lg_paged_attn: a workspace of %lld bytes, %lld are needed", work_bytes, need);
     OnDevice on;
@@ -224,7 +224,8 @@ extern "C" int lg_paged_attn(const struct lg_paged_cache *c, const void *d_q, in
     const AttnCut k = attn_cut(c, n_new, n_heads);
     LgPagedAttnArgs a;
     a.c = paged_of(c); a.q = d_q; a.out = d_out; a.ld_q = ld_q; a.ld_out = ld_out; a.n_req = n_req; a.n_new = n_new; a.n_rows = n_rows;
-    a.n_heads = n_heads; a.window = window; a.start = d_start;
+    a.n_heads = n_heads; a.start = d_start;
+    a.window = window < (long long)c->max_pages * c->page_size ? window : 0;             // a window of all rows is none
     a.scale = (scale > 0.0f ? scale : 1.0f / sqrtf((float)c->head_dim)) * LG_LOG2E;
     a.gqa = n_heads / c->n_kv_heads; a.group_rows = 8 * k.nt; a.whole = c->page_size % 16 == 0;
     a.jobs = (int4 *)d_work;

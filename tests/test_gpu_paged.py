@@ -351,6 +351,52 @@ def test_infinities_and_nan_in_visible_rows(lg, dtype, cache):
     assert torch.equal(out[0, 1], good[0, 1])
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,window", [(2, 1, 64, 0), (8, 1, 128, 0), (4, 2, 256, 20), (2, 2, 512, 3)])
+def test_a_bad_row_reaches_only_the_queries_that_see_it(lg, dtype, cache, heads, kv_heads, dim, window):
+    """V rows of inf and NaN at the end of a verify block and at the beginning of its windows: the block's other queries are as without them."""
+    import torch
+    lens, m = [100, 21, 4], [4, 4, 4]
+    c, q, out, work = _attn_case(lg, 21, lens, m, heads, kv_heads, dim, 16, dtype, cache, window=window)
+    good, table = out.clone(), c.oracle.table
+    for r, n in enumerate(lens):
+        c.v[table[r, (n - 2) // 16], (n - 2) % 16] = float("nan")                 # rows 2 and 3 of the block see it
+        if window:
+            first = max(0, n - 4 - window + 1)
+            if first + window <= n - 4 + 1:
+                c.v[table[r, first // 16], first % 16] = float("inf")             # row 0 alone sees it
+    c.c.attn(q, out, work, n_new=4, window=window)
+    for r, n in enumerate(lens):
+        spoilt = window and max(0, n - 4 - window + 1) + window <= n - 4 + 1
+        for t in range(4):
+            got, want = out[4 * r + t].float(), good[4 * r + t].float()
+            if t >= 2:
+                assert bool(got.isnan().all())
+            elif t == 0 and spoilt:
+                assert not bool(got.isfinite().any())
+            else:
+                # another order of the same sums: f32 rounding of up to 104 terms, then the type's
+                assert bool(((got - want).abs() <= 2.0 ** -15 * c.v.float().nan_to_num(0, 0, 0).abs().max() + 2 * HALF_STEP[dtype] * want.abs()).all()), (r, t)
+
+
+def test_a_window_of_everything(lg):
+    for window in (1 << 20, (1 << 31) - 1):
+        _attn_case(lg, 3, [40, 7], [2, 2], 4, 2, 64, 16, F16, F16, window=window)
+
+
+def test_calls_on_two_streams_with_workspaces_of_their_own(lg):
+    import torch
+    cases = [_attn_case(lg, s, [5000, 900, 64], [1, 1, 1], 8, 2, 128, 16, F32, F16) for s in (31, 32)]
+    want = [x[2].clone() for x in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (c, q, out, work), st in zip(cases, streams):
+            c.c.attn(q, out, work, stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x[2], w) for x, w in zip(cases, want))
+
+
 # ------------------------------------------------------------------------------------------------------------------------
 # together
 # ------------------------------------------------------------------------------------------------------------------------

@@ -26,9 +26,9 @@ def _desc(lg, **kw):
     return lg.PagedDesc(*[d[n] for n, _ in lg.PagedDesc._fields_])
 
 
-BAD = [dict(k=None), dict(v=None), dict(table=None), dict(len=None), dict(type=2), dict(n_pages=0), dict(page_size=0), dict(n_kv_heads=0), dict(max_req=0),
+BAD = [dict(k=None), dict(v=None), dict(table=None), dict(len=None), dict(type=2), dict(n_pages=0), dict(page_size=0), dict(n_kv_heads=0), dict(n_kv_heads=65536), dict(max_req=0),
        dict(max_pages=0), dict(table_stride=4), dict(head_dim=0), dict(head_dim=12), dict(head_dim=520), dict(n_pages=1 << 28, page_size=16),
-       dict(max_pages=1 << 28, table_stride=1 << 28), dict(page_stride=-8), dict(row_stride=4), dict(head_stride=65), dict(k=4104), dict(v=8194), dict(len=513)]
+       dict(max_pages=1 << 28, table_stride=1 << 28), dict(n_pages=1, max_pages=(1 << 26) + 1, table_stride=1 << 27), dict(page_stride=-8), dict(row_stride=4), dict(head_stride=65), dict(k=4104), dict(v=8194), dict(len=513)]
 
 
 @pytest.mark.parametrize("bad", BAD, ids=lambda b: ",".join(b))

@@ -414,21 +414,20 @@ template <int W> __device__ __forceinline__ int paged_weight(const LgReq &q, boo
     return pad ? max(1, (q.n_sl + least - 1) / least) * least : q.n_sl + LG_PA_ITEM_COST;
 }
 
-// The walk of one CTA over the items that begin before the end of its stretch lo .. hi-1 of the line.
+// The walk of one CTA over the items that begin before the end of its stretch: places 0 .. length-1, the item's beginning at `at` (below 0: another stretch has
+// its first slices).
 template <int W> struct LgWalk {
     LgReq q;
-    bool pad;
-    int r, hg;                         // request, KV head * groups + group
-    long long at, lo, hi;              // where the item begins; the stretch
-    __device__ __forceinline__ bool valid(const LgPagedAttnArgs &a) const { return r < a.n_req && at < hi; }
-    __device__ __forceinline__ int begin() const { return (int)max(lo - at, 0LL); }                        // the item's slices in the stretch
-    __device__ __forceinline__ int end() const { return (int)min(hi - at, (long long)q.n_sl); }
-    __device__ __forceinline__ void next(const LgPagedAttnArgs &a) {
+    int r, hg, at;                     // request, KV head * groups + group
+    __device__ __forceinline__ bool valid(const LgPagedAttnArgs &a, int length) const { return r < a.n_req && at < length; }
+    __device__ __forceinline__ int begin() const { return max(-at, 0); }                                   // the item's slices in the stretch
+    __device__ __forceinline__ int end(int length) const { return min(length - at, q.n_sl); }
+    __device__ __forceinline__ void next(const LgPagedAttnArgs &a, int length, bool pad) {
         at += paged_weight<W>(q, pad);
         hg++;
         while (r < a.n_req && hg >= q.groups * a.c.n_kv) {                    // past requests without rows
             if (++r < a.n_req) {
-                if (at < hi) { q = paged_request(a, r); hg = 0; } else r = a.n_req;
+                if (at < length) { q = paged_request(a, r); hg = 0; } else r = a.n_req;
             }
         }
     }
@@ -440,6 +439,9 @@ template <typename TQ, typename TC, int HD, int NT> struct LgPagedTile {
     static constexpr bool F16 = std::is_same<TC, __half>::value;
     static constexpr int NQ = SAME ? 1 : F16 ? 2 : 3;                         // parts of a query
     static constexpr int NP = SAME || F16 ? 2 : 3;                            // parts of a weight
+    // f32 answers: a slice's products are added to the outputs with rounding to nearest; the matrix instructions' own additions cut off, which over the
+    // 500 slices of a warp's stretch cost 2.4e-6 of the result where this leaves 0.8e-6.  (The factor of a moved maximum goes into the same operation.)
+    static constexpr bool RN = sizeof(TQ) == 4;
     static constexpr int KS = HD / 16;
     static constexpr int ROWS = 8 * NT;
     static constexpr int ROW = HD * (int)sizeof(TC), UNIT = 16 * ROW, CHUNKS = ROW / 16;
@@ -477,7 +479,8 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
 
     // this CTA's stretch: weights of all requests, thread by thread, and where the stretch begins
     LgWalk<P::W> w;
-    long long stretch;
+    int stretch, length;                                                      // of every CTA; of this one (the last may be shorter)
+    bool pad;
     {
         const int per = (a.n_req + P::W * 32 - 1) / (P::W * 32), r0 = min(a.n_req, tid * per), r1 = min(a.n_req, r0 + per);
         long long mine[2] = {0, 0}, s[2], before[2] = {0, 0}, total[2] = {0, 0};
@@ -502,17 +505,18 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
         // Stretches of the least length, if there are CTAs for them with no item's end inside of one: a CTA then has one item (each further one takes it
         // about 3 us, of 13 for a short call)
         constexpr int least = (LG_PA_MIN_STRETCH + P::W - 1) / P::W * P::W;
-        w.pad = total[1] <= (long long)least * gridDim.x;
-        const long long all = w.pad ? total[1] : total[0], own = w.pad ? mine[1] : mine[0];
-        long long at = w.pad ? before[1] + s[1] - mine[1] : before[0] + s[0] - mine[0];
-        stretch = w.pad ? least : max((long long)least, ((all + gridDim.x - 1) / gridDim.x + P::W - 1) / P::W * P::W);
-        w.lo = stretch * blockIdx.x; w.hi = min(w.lo + stretch, all);
-        if (own && at <= w.lo && w.lo < at + own) {
+        pad = total[1] <= (long long)least * gridDim.x;
+        const long long all = pad ? total[1] : total[0], own = pad ? mine[1] : mine[0];
+        long long at = pad ? before[1] + s[1] - mine[1] : before[0] + s[0] - mine[0];
+        stretch = pad ? least : (int)max((long long)least, ((all + gridDim.x - 1) / gridDim.x + P::W - 1) / P::W * P::W);
+        const long long lo = (long long)stretch * blockIdx.x;
+        length = (int)max(0LL, min((long long)stretch, all - lo));
+        if (own && at <= lo && lo < at + own) {
             int r = r0;
             for (;; r++) {
                 const LgReq q = paged_request(a, r);
-                const long long x = (long long)paged_weight<P::W>(q, w.pad) * q.groups * a.c.n_kv;
-                if (w.lo < at + x) break;
+                const long long x = (long long)paged_weight<P::W>(q, pad) * q.groups * a.c.n_kv;
+                if (lo < at + x) break;
                 at += x;
             }
             red[16] = r; red[17] = at;
@@ -522,9 +526,9 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
         if (tid == 0) a.jobs[blockIdx.x] = make_int4(-1, 0, 0, 0);
         if (w.r >= a.n_req) return;
         w.q = paged_request(a, w.r);
-        const int n = paged_weight<P::W>(w.q, w.pad);
-        w.hg = (int)((w.lo - red[17]) / n);
-        w.at = red[17] + (long long)w.hg * n;
+        const int n = paged_weight<P::W>(w.q, pad);
+        w.hg = (int)((lo - red[17]) / n);
+        w.at = (int)(red[17] + (long long)w.hg * n - lo);
     }
     // the copies run ahead of the arithmetic with a walk of their own
     LgWalk<P::W> p = w;
@@ -533,11 +537,11 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
     uint32_t pok = 0;
     const int ps_size = a.c.page_size, row_chunks = a.c.hd * (int)sizeof(TC) / 16;
     auto begin_item = [&]() {                                                 // first slice of this warp in walk p's item, or the next item that has one
-        while (p.valid(a)) {
+        while (p.valid(a, length)) {
             ps = p.q.s0 + p.begin() + warp;
-            ps_end = p.q.s0 + p.end();
+            ps_end = p.q.s0 + p.end(length);
             if (ps < ps_end) return true;
-            p.next(a);
+            p.next(a, length, pad);
         }
         return false;
     };
@@ -582,7 +586,7 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             if (is_v) {
                 ps += P::W;
                 nth++;
-                if (ps >= ps_end) { p.next(a); more = begin_item(); nth = 32; }
+                if (ps >= ps_end) { p.next(a, length, pad); more = begin_item(); nth = 32; }
                 if (more && (!a.whole || nth == 32)) fetch_pages();
             }
             n_issued++;
@@ -595,9 +599,9 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
 
     int slot = 0, n_used = 0, q_r = -1, q_hg = -1, turn = 0;
     uint32_t qr[P::QREG ? NT * P::NQ * P::KS * 2 : 1];
-    for (; w.valid(a); w.next(a)) {
-        const int s_begin = w.q.s0 + w.begin(), s_end = w.q.s0 + w.end();
-        if (s_begin >= s_end && (w.q.n_sl || w.at < w.lo)) continue;          // another stretch has its slices, or writes its zeros
+    for (; w.valid(a, length); w.next(a, length, pad)) {
+        const int s_begin = w.q.s0 + w.begin(), s_end = w.q.s0 + w.end(length);
+        if (s_begin >= s_end && (w.q.n_sl || w.at < 0)) continue;          // another stretch has its slices, or writes its zeros
         float2 *stat = stats + turn * P::W * P::ROWS;
         turn ^= 1;
         const int kvh = w.hg / w.q.groups, row0 = (w.hg - kvh * w.q.groups) * P::ROWS;      // first of the group's rows: row = token * gqa + head of the group
@@ -744,6 +748,7 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                     pb[nt][part][1] = movm(split2<typename P::TM>(x[2], x[3]));
                 }
             }
+            if (P::RN) moved = false;                                         // see below
             if (__any_sync(0xffffffffu, moved)) {
                 #pragma unroll
                 for (int ks = 0; ks < P::KS; ks++)
@@ -766,6 +771,14 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                 plain = !__any_sync(0xffffffffu, odd);
             }
             if (!plain) {
+                if (P::RN) {
+                    #pragma unroll
+                    for (int ks = 0; ks < P::KS; ks++)
+                        #pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+                            #pragma unroll
+                            for (int j = 0; j < 4; j++) o[ks][nt][j] *= f[nt][j & 1];
+                }
                 #pragma unroll
                 for (int half = 0; half < 2; half++)
                     #pragma unroll 1
@@ -807,12 +820,19 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                     ldsm_x4_t_u32(v4[0], at + row * P::ROW + (P::place(row, 2 * ks + ((lane >> 3) & 1)) << 4));
                 }
                 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                for (int nt = 0; nt < NT; nt++) {
+                    float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float (&to)[4] = P::RN ? add : o[ks][nt];
                     #pragma unroll
                     for (int part = 0; part < P::NP; part++)
                         #pragma unroll
                         for (int own = 0; own < (P::F32 ? 3 : 1); own++)
-                            if (own + part < 3) mma_16<typename P::TM>(o[ks][nt], v4[own], pb[nt][part][0], pb[nt][part][1]);
+                            if (own + part < 3) mma_16<typename P::TM>(to, v4[own], pb[nt][part][0], pb[nt][part][1]);
+                    if (P::RN) {
+                        #pragma unroll
+                        for (int j = 0; j < 4; j++) o[ks][nt][j] = fmaf(o[ks][nt][j], f[nt][j & 1], add[j]);
+                    }
+                }
             }
         }
         // the warps' results into one, in warp order
@@ -853,9 +873,9 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             __syncthreads();
         }
         // the item's other slices: before this stretch, behind it (its last slice then lies in the stretch of CTA `last`)
-        const bool head = w.at < w.lo, tail = w.at + w.q.n_sl > w.hi;
+        const bool head = w.at < 0, tail = w.at + w.q.n_sl > length;
         const long long part = ((long long)blockIdx.x * 2 + !head) * P::ROWS;
-        if (!head && tail && tid == 0) a.jobs[blockIdx.x] = make_int4(w.q.first, kvh, (int)((w.at + w.q.n_sl - 1) / stretch), row0 << 8 | n_rows);
+        if (!head && tail && tid == 0) a.jobs[blockIdx.x] = make_int4(w.q.first, kvh, (int)blockIdx.x + (w.at + w.q.n_sl - 1) / stretch, row0 << 8 | n_rows);
         for (int n = warp; n < n_rows; n += P::W) {
             float m2 = -INFINITY, sum = 0.0f;
             #pragma unroll

@@ -45,6 +45,9 @@ struct lg_paged_cache {
     int *status;                       /* or NULL; the caller clears it */
 };
 
+/* Where the kernels look for a row of a page and a head: elements from the beginning of k (or v), -1 where the cache has no such row.  Needs no GPU. */
+long long lg_debug_paged_place(const struct lg_paged_cache *c, int page, int row, int head);
+
 /* One step of requests 0 .. n_req-1: request r keeps its first d_keep[r] rows (NULL: all of them) and gets d_new[r] new ones behind
  * them.  Pages that this takes come from the top of the stack, in the order of the requests and of their rows; pages that it
  * gives up go back in the opposite order, so that a step which rolls a step back leaves the stack as it was.  Updated: table

@@ -37,7 +37,7 @@ ABI_SYMBOLS = [
 ]
 
 # every symbol include/lg_serve.h declares
-SERVE_SYMBOLS = ["lg_paged_step", "lg_paged_append", "lg_paged_attn_work", "lg_paged_attn", "lg_sample", "lg_forward_sample"]
+SERVE_SYMBOLS = ["lg_debug_paged_place", "lg_paged_step", "lg_paged_append", "lg_paged_attn_work", "lg_paged_attn", "lg_sample", "lg_forward_sample"]
 
 class PlanLayer(C.Structure):
     """struct lg_plan_layer of include/lg_plan.h"""
@@ -148,6 +148,7 @@ def load() -> C.CDLL:
     for name, args, res in (("lg_paged_step", [vp, i, vp, vp, i, vp, vp, vp, vp, vp], i),
                             ("lg_paged_append", [vp, vp, vp, i, ll, ll, i, vp, vp], i),
                             ("lg_paged_attn_work", [vp, i, i, i], ll),
+                            ("lg_debug_paged_place", [vp, i, i, i], ll),
                             ("lg_paged_attn", [vp, vp, i, ll, i, i, i, vp, i, fl, i, vp, ll, vp, ll, vp], i),
                             ("lg_sample", [vp, i, ll, i, i, vp, vp, vp, vp, vp, vp, vp, vp], i),
                             ("lg_forward_sample", [vp, vp, i, i, fl, i, fl, fl, fl, C.POINTER(C.c_float)], i)):

@@ -14,6 +14,11 @@ struct LgPaged {                       // struct lg_paged_cache as the kernels n
     int *table, *len, *free_pages, *n_free, *status;
 };
 
+// Where a row of a page begins, for one head, in elements; -1: there is no such row.
+__host__ __device__ __forceinline__ long long paged_place(const LgPaged &c, int page, int row, int head) {
+    if (page < 0 || page >= c.n_pages || row < 0 || row >= c.page_size || head < 0 || head >= c.n_kv) return -1;
+    return (long long)page * c.page_stride + (long long)row * c.row_stride + (long long)head * c.head_stride;
+}
 __device__ __forceinline__ void paged_raise(const LgPaged &c, int bit) { if (c.status) atomicOr(c.status, bit); }
 
 // Element types.  store8: 8 elements rounded into a 16-byte word.
@@ -83,7 +88,8 @@ __device__ __forceinline__ void block_scan3(long long (&v)[3], long long (&total
 // returned pages; what the old state is read for lies before the cluster's barrier, what overwrites it behind.  Sums over the requests -- pages
 // taken, tokens, pages returned -- say where each request's things go, and every token and page then finds its place on its own.  Where
 // pages or rows do not suffice, two more sums decide who is served: a request that is not takes no pages, and neither does any later one
-// that needs some, so the pages taken are always the top of the stack in one piece.  Bound by latency: 48 requests 4 us, 2048 with 40000 tokens 12 us (one CTA 137).
+// that needs some, so the pages taken are always the top of the stack in one piece.  Bound by latency: a step and its roll-back
+// take 9.4 us for 48 requests, 23 us for 2048 with 40576 tokens (one CTA, with the requests looked up again for every token: 274).
 template <int PER> __global__ void __launch_bounds__(LG_STEP_THREADS, 1) lg_paged_step_kernel(LgStepArgs a) {
     extern __shared__ int sm[];
     __shared__ long long red[32][3];
@@ -254,7 +260,8 @@ template <typename T> struct Eight<T, T> {
 };
 
 // A thread moves 8 elements of a row at a time, two such pieces under way, K's and V's; a CTA has one row, or as many whole ones as its threads cover, and
-// goes on to the next.  Rows of one type are not looked at.  Bound by the bytes in and out, or by latency.
+// goes on to the next.  Rows of one type are not looked at.  Bound by the bytes in and out: 8191 rows of 8 heads of 256 in bf16 take 18.6 to 25 us (134 MB; a division a piece and
+// conversion through f32 cost 30), 48 rows 1.9 us.
 template <typename TI, typename TC> __global__ void __launch_bounds__(LG_APPEND_THREADS) lg_paged_append_kernel(LgAppendArgs a) {
     const int per_head = a.c.hd >> 3, half = per_head * a.c.n_kv, units = 2 * half;
     const int here = units < LG_APPEND_THREADS ? (int)threadIdx.x / units : 0, rows = units < LG_APPEND_THREADS ? LG_APPEND_THREADS / units : 1;
@@ -274,7 +281,7 @@ template <typename TI, typename TC> __global__ void __launch_bounds__(LG_APPEND_
             }
             if (slot < 0 || slot >= n_slots) { if (slot != -1) paged_raise(a.c, LG_PAGED_BAD_SLOT); break; }
             const int page = slot / a.c.page_size;
-            const long long to = (long long)page * a.c.page_stride + (long long)(slot - page * a.c.page_size) * a.c.row_stride;
+            const long long to = paged_place(a.c, page, slot - page * a.c.page_size, 0);
             #pragma unroll
             for (int q = 0; q < 2; q++) {
                 const int w = u + q * LG_APPEND_THREADS, c = w < half ? w : w - half;
@@ -322,8 +329,8 @@ __device__ __forceinline__ int paged_len(const LgPagedAttnArgs &a, int r) {
 // The work is a line of slices of 16 keys: request by request, KV head by KV head, group of 8 NT query rows by group (an item).  Every CTA of a
 // persistent grid takes a stretch of equal length of that line, so ragged lengths cost nothing; an item that one stretch holds is written at once,
 // of one that several stretches share each leaves (max, sum, unnormalised output), and lg_paged_merge_kernel adds those in their order.
-// (Spans fixed by a request's own length were the first form: 876 us for 96 requests of 1.6K to 16K rows, where this takes less; short spans cost merges,
-// and about as many items as CTAs leave SMs idle: 153 us for two requests of 120000 rows with 58 % of the SMs' time in use.)
+// (Spans fixed by a request's own length: 876 us for 96 requests of 1.6K to 16K rows where this takes 539, the copy's bandwidth; short spans cost merges, and
+// about as many items as CTAs leave SMs idle: 153 us for two requests of 120000 rows where this takes 97.)
 //
 // Inside a CTA every warp works alone: it takes 16 keys (a slice) at a time, brings K and V in with 16-byte asynchronous copies through a ring
 // of U units of its own (a unit: 16 rows of K or of V; rows that no query may see are filled with zeros and never read), so the loop has no block barrier and
@@ -570,7 +577,7 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                 const int first = max(lo - ps * 16, 0), last = min(hi - ps * 16, 16);
                 int pg = page, rm = rem;
                 if (a.whole) { pg = __shfl_sync(0xffffffffu, page, nth); rm = __shfl_sync(0xffffffffu, rem, nth) + (lane & 15); }
-                poff = pg >= 0 ? ((long long)pg * a.c.page_stride + (long long)rm * a.c.row_stride + (long long)(p.hg / p.q.groups) * a.c.head_stride) * (int)sizeof(TC) : 0;
+                poff = max(paged_place(a.c, pg, rm, p.hg / p.q.groups), 0LL) * (int)sizeof(TC);
                 pok = a.whole ? pg >= 0 ? (0xFFFFu << first) & (0xFFFFu >> (16 - last)) : 0u : __ballot_sync(0xffffffffu, pg >= 0) & 0xFFFFu;
                 if (lane == 0) vmask[warp * 16 + ((n_issued >> 1) & 15)] = pok;
             }

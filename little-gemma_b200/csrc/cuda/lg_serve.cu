@@ -103,6 +103,12 @@ void add_cache(OnDevice &on, const struct lg_paged_cache *c) {
 
 }  // namespace
 
+// The kernels' own arithmetic, on the host
+extern "C" long long lg_debug_paged_place(const struct lg_paged_cache *c, int page, int row, int head) {
+    if (const char *f = cache_fault(c)) SERVE_FAIL(-2, "lg_debug_paged_place: %s", f);
+    return paged_place(paged_of(c), page, row, head);
+}
+
 extern "C" int lg_paged_step(const struct lg_paged_cache *c, int n_req, const int *d_keep, const int *d_new, int cap, int *d_start, int *d_pos,
                              int *d_slot, int *d_req, void *stream) {
     if (const char *f = cache_fault(c)) SERVE_FAIL(-1, "lg_paged_step: %s", f);

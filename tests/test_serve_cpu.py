@@ -42,6 +42,19 @@ def test_bad_caches_are_refused(lg, bad, capfd):
     assert L.lg_paged_attn_work(None, 1, 1, 2) == -1
 
 
+@pytest.mark.parametrize("pages,page,heads,dim,order", [(7, 16, 2, 64, "rows"), (5, 24, 3, 80, "heads"), (1, 1, 1, 8, "rows"), (60000, 128, 8, 128, "rows")])
+def test_places_stay_in_the_cache_and_bad_pages_have_none(lg, pages, page, heads, dim, order):
+    rs, hs = (heads * dim, dim) if order == "rows" else (dim, page * dim)
+    c = _desc(lg, n_pages=pages, page_size=page, n_kv_heads=heads, head_dim=dim, page_stride=page * heads * dim, row_stride=rs, head_stride=hs)
+    place = lambda *at: lg.load().lg_debug_paged_place(C.byref(c), *at)  # noqa: E731
+    rng = np.random.default_rng(pages)
+    for p, r, h in [(0, 0, 0), (pages - 1, page - 1, heads - 1)] + [tuple(rng.integers(0, (pages, page, heads))) for _ in range(200)]:
+        at = place(int(p), int(r), int(h))
+        assert at == int(p) * page * heads * dim + int(r) * rs + int(h) * hs and 0 <= at <= pages * page * heads * dim - dim      # past 2^31 in the last case
+    for bad in ((-1, 0, 0), (pages, 0, 0), (1 << 30, 0, 0), (-(1 << 31), 0, 0), (0, -1, 0), (0, page, 0), (0, 0, heads), (0, 0, -1)):
+        assert place(*bad) == -1
+
+
 def test_bad_steps_are_refused(lg):
     L, c, r = lg.load(), _desc(lg), C.byref
     call = lambda desc=c, n=1, keep=None, new=64, cap=0, start=64, pos=None: L.lg_paged_step(r(desc), n, keep, new, cap, start, pos, None, None, None)  # noqa: E731

@@ -449,6 +449,7 @@ template <typename TQ, typename TC, int HD, int NT> struct LgPagedTile {
     // f32 answers: a slice's products are added to the outputs with rounding to nearest; the matrix instructions' own additions cut off, which over the
     // 500 slices of a warp's stretch cost 2.4e-6 of the result where this leaves 0.8e-6.  (The factor of a moved maximum goes into the same operation.)
     static constexpr bool RN = sizeof(TQ) == 4;
+    static constexpr bool LONG = RN && HD > 128;                              // scores added up so too, every 128 dims
     static constexpr int KS = HD / 16;
     static constexpr int ROWS = 8 * NT;
     static constexpr int ROW = HD * (int)sizeof(TC), UNIT = 16 * ROW, CHUNKS = ROW / 16;
@@ -648,7 +649,7 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                     for (int part = 0; part < P::NQ; part++)
                         sq[((((n >> 3) * P::NQ + part) * P::KS + ks) * 32 + (n & 7) * 4 + t) * 2 + half] = split2<typename P::TM>(x[2 * i], x[2 * i + 1]);
                 }
-                if (lane == 0) cscale[n] = back;
+                if (lane == 0) cscale[n] = fmaxf(back, 1e-37f);               // above 0: a masked score times it is -inf
             }
             __syncthreads();
             if (P::QREG) {
@@ -689,6 +690,11 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             for (int nt = 0; nt < NT; nt++)
                 #pragma unroll
                 for (int j = 0; j < 4; j++) sc[nt][0][j] = sc[nt][1][j] = 0.0f;
+            float sum[P::LONG ? NT : 1][4];
+            if (P::LONG) {
+                #pragma unroll
+                for (int nt = 0; nt < NT; nt++) sum[nt][0] = sum[nt][1] = sum[nt][2] = sum[nt][3] = 0.0f;
+            }
             #pragma unroll
             for (int ks = 0; ks < P::KS; ks++) {
                 uint32_t k4[P::F32 ? 3 : 1][4];                               // parts of 16 rows x 16 dims
@@ -716,6 +722,12 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                         for (int own = 0; own < (P::F32 ? 3 : 1); own++)
                             if (own + part < 3) mma_16<typename P::TM>(sc[nt][ks & 1], k4[own], v.x, v.y);
                     }
+                if (P::LONG && ks % 8 == 7 && ks != P::KS - 1) {
+                    #pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+                        #pragma unroll
+                        for (int j = 0; j < 4; j++) { sum[nt][j] += sc[nt][0][j] + sc[nt][1][j]; sc[nt][0][j] = sc[nt][1][j] = 0.0f; }
+                }
             }
             const int k0 = s * 16;
             const bool all = ok == 0xFFFFu && k0 + 15 <= pos_lo && (a.window <= 0 || k0 > pos_hi - a.window);
@@ -727,7 +739,8 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                 float x[4];
                 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    x[j] = (sc[nt][0][j] + sc[nt][1][j]) * cs[nt][j & 1];
+                    x[j] = sc[nt][0][j] + sc[nt][1][j];
+                    if (P::LONG) x[j] += sum[nt][j];
                     if (!all) {
                         const int key = k0 + g + (j >> 1) * 8, pos = top[nt][j & 1];
                         if (!(ok >> (g + (j >> 1) * 8) & 1) || key > pos || (a.window > 0 && key <= pos - a.window)) x[j] = -INFINITY;
@@ -735,7 +748,7 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                 }
                 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    float m2 = fmaxf(x[j], x[j + 2]);
+                    float m2 = fmaxf(x[j], x[j + 2]) * cs[nt][j];
                     m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, 4));
                     m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, 8));
                     m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, 16));
@@ -745,8 +758,9 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                     moved |= m2 != mx[nt][j];
                     mx[nt][j] = m2;
                     const float up = P::F16 ? 15.0f : 0.0f;
-                    x[j] = ex2(x[j] - ref + up);
-                    x[j + 2] = ex2(x[j + 2] - ref + up);
+                    // score minus maximum in one rounding: small next to the maximum, where the weight is
+                    x[j] = ex2(fmaf(x[j], cs[nt][j], up - ref));
+                    x[j + 2] = ex2(fmaf(x[j + 2], cs[nt][j], up - ref));
                     l[nt][j] = l[nt][j] * f[nt][j] + (x[j] + x[j + 2]);
                 }
                 #pragma unroll

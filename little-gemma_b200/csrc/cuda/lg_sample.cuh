@@ -117,9 +117,9 @@ struct LgWeight {
         p = fma(p, rest, -c);
         p = fma(p, rest, 1.0);
         const int hi = __shfl_sync(0xffffffffu, __double2hiint(root), k), lo = __shfl_sync(0xffffffffu, __double2loint(root), k);
-        return p * __hiloint2double(hi - (k & ~31) * 32768, lo);
+        return __dmul_rn(p, __hiloint2double(hi - (k & ~31) * 32768, lo));    // (never joined with an addition: a weight is the same wherever it is computed)
     }
-    static __device__ __forceinline__ double whole(double s) { return (s + LG_TWO52) - LG_TWO52; }    // to the nearest integer; s < 2^51
+    static __device__ __forceinline__ double whole(double s) { return __dadd_rn(__dadd_rn(s, LG_TWO52), -LG_TWO52); }    // to the nearest integer; s < 2^51
     // of one logit, the same in all lanes: 0 where it has no weight
     __device__ __forceinline__ double of(float l) const {
         int k;
@@ -340,10 +340,10 @@ template <typename T> struct LgSampler {
         }
         cluster_sync_all();
     }
-    template <int N> __device__ __forceinline__ void shared_bins(u64 (&v)[N]) const {     // N a thread
-        const int per = N * LG_SAMPLE_THREADS / ranks;
+    template <int N> __device__ __forceinline__ void shared_bins(u64 (&v)[N]) const {     // N a thread; ranks is a power of two
+        const int per = N * LG_SAMPLE_THREADS / ranks, log = 31 - __clz(per);
         #pragma unroll
-        for (int j = 0; j < N; j++) { const int b = threadIdx.x * N + j; v[j] = ld_peer_u64(fine + b % per, b / per); }
+        for (int j = 0; j < N; j++) { const int b = threadIdx.x * N + j; v[j] = ld_peer_u64(fine + (b & (per - 1)), b >> log); }
     }
     // The keys of a row's tokens from some threshold up, where every CTA has them (refine leaves them here): the histograms' place
     __device__ __forceinline__ uint32_t *pool() const { return hist; }
@@ -493,7 +493,7 @@ template <typename T> struct LgSampler {
 template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg_sample_kernel(LgSampleArgs a) {
     extern __shared__ __align__(16) unsigned char lg_sample_sm[];
     __shared__ u64 word[48], red[2 * LG_SAMPLE_WARPS + 5];
-    __shared__ int kind[LG_SAMPLE_WARPS];               // tokens of a warp's list, -1: it has the row's own
+    __shared__ int kind[LG_SAMPLE_WARPS];               // tokens of a warp's list; -1: it has the row's own, -2: and min_p takes none of those above the threshold
     typedef LogitType<T> L;
     constexpr int LOW = L::LOW;
     uint32_t ranks;
@@ -692,7 +692,8 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
     const double x_t = s.w.of(lt);
     const u64 one = x_t >= floor_w ? (u64)(long long)LgWeight::whole(x_t) : 0;
     u64 over, at_t;
-    if (n_list >= 0 && (ties ? x_t : 0.0) >= floor_w) {
+    const bool noted = n_list >= 0 && (ties ? x_t : 0.0) >= floor_w;
+    if (noted) {
         // min_p takes nothing away: the weight above the list, and the list's own tokens
         over = over_w; at_t = 0;
         for (int i = 0; i < n_list; i += 32) {
@@ -730,7 +731,7 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
         all = run0 + __shfl_sync(0xffffffffu, x_up, 31);
         return x_all;
     };
-    if (lane == 0) kind[warp] = s.listed ? s.w1 : -1;
+    if (lane == 0) kind[warp] = s.listed ? s.w1 : noted ? -2 : -1;
     const u64 *mine;
     u64 total, none, y0, x0;
     s.sum2(over, at_t, total, none, &mine);
@@ -746,6 +747,7 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
         const int who = hit ? __ffs(hit) - 1 : 0;
         ties0 = __shfl_sync(0xffffffffu, y0, who); run = __shfl_sync(0xffffffffu, x0, who);
         s.listed = kind[who] >= 0;
+        const double least = kind[who] == -2 ? 0.0 : floor_w;
         s.lv += (who - warp) * LG_SAMPLE_LIST * 2; s.li += (who - warp) * LG_SAMPLE_LIST * 2;
         const int from = s.listed ? 0 : min(who * per, n), to = s.listed ? kind[who] : min(from + per, n), sub = ((to - from + LG_SAMPLE_WARPS - 1) / LG_SAMPLE_WARPS + 127) / 128 * 128;
         const int i0 = min(from + warp * sub, to), i1 = min(i0 + sub, to);
@@ -759,7 +761,7 @@ template <typename T> __global__ void __launch_bounds__(LG_SAMPLE_THREADS, 2) lg
             uint32_t eq = 0;
             #pragma unroll
             for (int j = 0; j < 4; j++) {
-                v[j] = in[j] && x[j] >= floor_w ? (u64)(long long)LgWeight::whole(x[j]) : 0;
+                v[j] = in[j] && x[j] >= least ? (u64)(long long)LgWeight::whole(x[j]) : 0;
                 eq |= (uint32_t)(ties && l[j] == lt) << j;
                 if (l[j] == lt) x[j] = x_t;
             }

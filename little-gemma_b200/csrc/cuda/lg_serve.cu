@@ -246,7 +246,8 @@ namespace {
 // CTAs that share a row (a cluster; 8 at most, which every device places, and 16 were slower).  A row's time goes with the passes over a CTA's
 // tokens, so few rows are shared by more CTAs, as long as each has 4096 tokens; with more rows than that the SMs are filled about three times (two CTAs fit one),
 // with 16384 tokens or more each, since a CTA's fixed work -- barriers, scans of histograms -- is done in each.  Measured, CTAs a row 1 / 2 / 4 / 8: one row of
-// 262144 - / 79 / 55 / 44 us, 48 rows - / 176 / 151 / 145, 200 rows - / 364 / 379 / 498, 64 rows of 32768 42 / 37 / 43 / 85, 512 rows of 32768 47 / 55 / 87 / 163.
+// 262144 - / 69 / 47 / 30 us, 48 rows - / 166 / 149 / 138, 200 rows - / 355 / 374 / 488, 64 rows of 32768 28 / 25 / 34 / 66, 512 rows of 32768 48 / 55 / 86 / 162
+// (5 a row 127 for the 48 rows, but 3 and 6 a row slower than 2 and 4: odd clusters leave SMs over).
 template <typename T> int launch_sample(LgSampleArgs &a, int dev, void *stream) {
     const int sms = device_sms(dev), tools = a.top_k || a.top_p ? LG_SAMPLE_TOOLS : 0;
     int ranks = 1;

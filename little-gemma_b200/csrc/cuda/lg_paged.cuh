@@ -458,9 +458,10 @@ template <typename TQ, typename TC, int HD, int NT> struct LgPagedTile {
     static __device__ __forceinline__ int place(int row, int c) { return F32 ? c ^ (((row ^ (row >> 2)) & 3) << 1) : c ^ (row & 7); }
     static constexpr int LDB = HD + 4;                                        // floats from row to row of the merge buffer: no bank conflicts
     static constexpr bool QREG = (NT * NQ * 2 + NT * 4) * KS <= 160;          // queries stay in registers beside the outputs
-    static constexpr int Q_BYTES = NT * NQ * KS * 32 * 8, BUF_BYTES = ROWS * LDB * 4;
+    static constexpr bool OWN = UNIT >= ROWS * HD * 4;                        // a warp's outputs fit the ring's free unit on their way to the others'
+    static constexpr int Q_BYTES = NT * NQ * KS * 32 * 8, BUF_BYTES = OWN ? 0 : ROWS * LDB * 4;
     static constexpr int SHARED = QREG ? (Q_BYTES > BUF_BYTES ? Q_BYTES : BUF_BYTES) : Q_BYTES + BUF_BYTES;   // in registers they need the room only on the way
-    static constexpr int fixed(int w) { return SHARED + 2 * w * ROWS * 8 + ROWS * 4 + 144 + w * 16 * 4; }
+    static constexpr int fixed(int w) { return SHARED + 2 * w * ROWS * 8 + ROWS * 4 + 144 + w * 17 * 4; }
     // Two CTAs of 4 warps per SM where three units a warp fit (one merges while the other streams), else one of as many warps as fit
     static constexpr int CTAS = fixed(4) + 12 * UNIT <= 115712 ? 2 : 1;
     static constexpr int ROOM = CTAS == 2 ? 115712 : 232448;
@@ -482,6 +483,7 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
     float *cscale = (float *)(stats + 2 * P::W * P::ROWS);                  // [row]: scale of the scores
     long long *red = (long long *)(cscale + P::ROWS);                         // 18 words
     uint32_t *vmask = (uint32_t *)(red + 18);                                  // [warp][16]: keys of a slice that are there
+    int *free_of = (int *)(vmask + P::W * 16);                                // [warp]: its ring's free unit
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     pdl_launch();
 
@@ -616,7 +618,7 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
         const int n_rows = min(P::ROWS, w.q.m * a.gqa - row0);
         if (q_r != w.r || q_hg != w.hg) {                                     // queries of the group into operand order
             q_r = w.r; q_hg = w.hg;
-            if (P::QREG) __syncthreads();                                     // the merge buffer lies there
+            if (P::QREG && !P::OWN) __syncthreads();                          // the merge buffer lies there
             for (int n = warp; n < P::ROWS; n += P::W) {
                 const int rho = row0 + n, t = rho / a.gqa;
                 const TQ *src = (const TQ *)a.q + (long long)(w.q.first + t) * a.ld_q + (long long)(kvh * a.gqa + rho - t * a.gqa) * a.c.hd;
@@ -867,51 +869,79 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                 x += __shfl_xor_sync(0xffffffffu, x, 16);
                 if (g == 0) stat[warp * P::ROWS + nt * 8 + 2 * t4 + j] = make_float2(mx[nt][j], x);
             }
-        __syncthreads();
-        float f[NT][2];
-        #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-            #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                float m2 = -INFINITY;
-                #pragma unroll
-                for (int i = 0; i < P::W; i++) m2 = fmaxf(m2, stat[i * P::ROWS + nt * 8 + 2 * t4 + j].x);
-                f[nt][j] = ex2(mx[nt][j] - (m2 == -INFINITY ? 0.0f : m2));
-            }
-        for (int i = 0; i < P::W; i++) {
-            if (warp == i) {
-                #pragma unroll
-                for (int ks = 0; ks < P::KS; ks++)
-                    #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-                        #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            float *e = buf + (nt * 8 + 2 * t4 + (j & 1)) * P::LDB + ks * 16 + g + (j >> 1) * 8;
-                            const float x = o[ks][nt][j] * f[nt][j & 1];
-                            *e = i ? *e + x : x;
-                        }
-            }
-            __syncthreads();
-        }
         // the item's other slices: before this stretch, behind it (its last slice then lies in the stretch of CTA `last`)
         const bool head = w.at < 0, tail = w.at + w.q.n_sl > length;
         const long long part = ((long long)blockIdx.x * 2 + !head) * P::ROWS;
         if (!head && tail && tid == 0) a.jobs[blockIdx.x] = make_int4(w.q.first, kvh, (int)blockIdx.x + (w.at + w.q.n_sl - 1) / stretch, row0 << 8 | n_rows);
-        for (int n = warp; n < n_rows; n += P::W) {
-            float m2 = -INFINITY, sum = 0.0f;
+        // row n of the item: its maximum, sum and the warps' factors, then (put) its numbers
+        auto finish = [&](int n, int first, int step, auto &&number) {
+            float m2 = -INFINITY, sum = 0.0f, fw[P::W];
             #pragma unroll
             for (int i = 0; i < P::W; i++) m2 = fmaxf(m2, stat[i * P::ROWS + n].x);
             #pragma unroll
-            for (int i = 0; i < P::W; i++) sum += stat[i * P::ROWS + n].y * ex2(stat[i * P::ROWS + n].x - (m2 == -INFINITY ? 0.0f : m2));
+            for (int i = 0; i < P::W; i++) { fw[i] = ex2(stat[i * P::ROWS + n].x - (m2 == -INFINITY ? 0.0f : m2)); sum += stat[i * P::ROWS + n].y * fw[i]; }
             const int rho = row0 + n, t = rho / a.gqa, h = kvh * a.gqa + rho - t * a.gqa;
             if (!head && !tail) {
                 TQ *out = (TQ *)a.out + (long long)(w.q.first + t) * a.ld_out + (long long)h * a.c.hd;
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                for (int d = lane; d < a.c.hd; d += 32) out[d] = Elem<TQ>::put(buf[n * P::LDB + d] * inv);
+                for (int d = first; d < a.c.hd; d += step) out[d] = Elem<TQ>::put(number(d, fw) * inv);
             } else {
-                for (int d = lane; d < a.c.hd; d += 32) a.part[(part + n) * a.c.hd + d] = buf[n * P::LDB + d];
-                if (lane == 0) a.part_ml[part + n] = make_float2(m2, sum);
+                for (int d = first; d < a.c.hd; d += step) a.part[(part + n) * a.c.hd + d] = number(d, fw);
+                if (first == 0) a.part_ml[part + n] = make_float2(m2, sum);
             }
+        };
+        if constexpr (P::OWN) {
+            // each warp's outputs into the unit of its ring that no copy is under way to; the columns of a row pair moved by 8 so that a store meets no bank twice
+            float *mine = (float *)(ring + warp * (P::U * P::UNIT) + slot_in * P::UNIT);
+            #pragma unroll
+            for (int ks = 0; ks < P::KS; ks++)
+                #pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+                    #pragma unroll
+                    for (int j = 0; j < 4; j++) mine[(nt * 8 + 2 * t4 + (j & 1)) * HD + ((ks * 16 + g + (j >> 1) * 8) ^ (t4 << 3))] = o[ks][nt][j];
+            if (lane == 0) free_of[warp] = slot_in;
+            __syncthreads();
+            const float *from[P::W];
+            #pragma unroll
+            for (int i = 0; i < P::W; i++) from[i] = (const float *)(ring + i * (P::U * P::UNIT) + free_of[i] * P::UNIT);
+            const bool each = n_rows >= P::W;                                 // a row a warp, or every row by all of them
+            for (int n = each ? warp : 0; n < n_rows; n += each ? P::W : 1)
+                finish(n, each ? lane : tid, each ? 32 : P::W * 32, [&](int d, const float (&fw)[P::W]) {
+                    const int at = n * HD + (d ^ (((n >> 1) & 3) << 3));
+                    float y = 0.0f;
+                    #pragma unroll
+                    for (int i = 0; i < P::W; i++) y += from[i][at] * fw[i];
+                    return y;
+                });
+            __syncthreads();                                                  // before the units are filled again
+        } else {
+            __syncthreads();
+            float f[NT][2];
+            #pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+                #pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float m2 = -INFINITY;
+                    #pragma unroll
+                    for (int i = 0; i < P::W; i++) m2 = fmaxf(m2, stat[i * P::ROWS + nt * 8 + 2 * t4 + j].x);
+                    f[nt][j] = ex2(mx[nt][j] - (m2 == -INFINITY ? 0.0f : m2));
+                }
+            for (int i = 0; i < P::W; i++) {
+                if (warp == i) {
+                    #pragma unroll
+                    for (int ks = 0; ks < P::KS; ks++)
+                        #pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+                            #pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                float *e = buf + (nt * 8 + 2 * t4 + (j & 1)) * P::LDB + ks * 16 + g + (j >> 1) * 8;
+                                const float x = o[ks][nt][j] * f[nt][j & 1];
+                                *e = i ? *e + x : x;
+                            }
+                }
+                __syncthreads();
+            }
+            for (int n = warp; n < n_rows; n += P::W) finish(n, lane, 32, [&](int d, const float (&)[P::W]) { return buf[n * P::LDB + d]; });
         }
     }
 }

@@ -329,8 +329,8 @@ template <typename T> struct LgSampler {
     // This CTA's share of the bins of a histogram, summed over the cluster and left for the others: adding up all bins in every CTA would
     // move ranks^2 histograms through the cluster
     __device__ void share_bins(const uint32_t *h, int bins, int limbs) {
-        const int per = bins / ranks;
-        for (int b = threadIdx.x; b < per; b += LG_SAMPLE_THREADS) {
+        const int per = (bins + ranks - 1) / ranks;
+        for (int b = threadIdx.x; b < per && rank * per + b < bins; b += LG_SAMPLE_THREADS) {
             u64 v = 0;
             for (int l = 0; l < limbs; l++) {
                 #pragma unroll
@@ -340,10 +340,10 @@ template <typename T> struct LgSampler {
         }
         cluster_sync_all();
     }
-    template <int N> __device__ __forceinline__ void shared_bins(u64 (&v)[N]) const {     // N a thread; ranks is a power of two
-        const int per = N * LG_SAMPLE_THREADS / ranks, log = 31 - __clz(per);
+    template <int N> __device__ __forceinline__ void shared_bins(u64 (&v)[N]) const {     // N a thread
+        const int per = (N * LG_SAMPLE_THREADS + ranks - 1) / ranks;
         #pragma unroll
-        for (int j = 0; j < N; j++) { const int b = threadIdx.x * N + j; v[j] = ld_peer_u64(fine + (b & (per - 1)), b >> log); }
+        for (int j = 0; j < N; j++) { const int b = threadIdx.x * N + j, c = b / per; v[j] = ld_peer_u64(fine + b - c * per, c); }
     }
     // The keys of a row's tokens from some threshold up, where every CTA has them (refine leaves them here): the histograms' place
     __device__ __forceinline__ uint32_t *pool() const { return hist; }

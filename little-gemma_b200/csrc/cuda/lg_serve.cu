@@ -1,5 +1,6 @@
 // lg_serve.cu -- operators of a decode step of many requests (include/lg_serve.h): the entry points, their checks and launches.
 // Kernels: lg_paged.cuh (block tables and slots, append, attention of a paged cache), lg_sample.cuh.
+#include <algorithm>
 #include "lg_engine.h"
 #include "lg_serve.h"
 #include "lg_paged.cuh"
@@ -243,24 +244,42 @@ extern "C" int lg_paged_attn(const struct lg_paged_cache *c, const void *d_q, in
 }
 
 namespace {
-// CTAs that share a row (a cluster; 8 at most, which every device places, and 16 were slower).  A row's time goes with the passes over a CTA's
-// tokens, so few rows are shared by more CTAs, as long as each has 4096 tokens; with more rows than that the SMs are filled about three times (two CTAs fit one),
-// with 16384 tokens or more each, since a CTA's fixed work -- barriers, scans of histograms -- is done in each.  Measured, CTAs a row 1 / 2 / 4 / 8: one row of
-// 262144 - / 69 / 47 / 30 us, 48 rows - / 166 / 149 / 138, 200 rows - / 355 / 374 / 488, 64 rows of 32768 28 / 25 / 34 / 66, 512 rows of 32768 48 / 55 / 86 / 162
-// (5 a row 127 for the 48 rows, but 3 and 6 a row slower than 2 and 4: odd clusters leave SMs over).
+// CTAs that share a row, a cluster of at most 8 (what every device places; 16 were slower).  A CTA's time goes with its tokens, and its fixed work -- barriers, scans of
+// histograms -- with some 10000 more; two on an SM take 1.7 times as long as one; clusters that the device cannot hold at once follow in rounds.  That
+// estimate is within 15 % of what was measured, and its choice within 5 % of the best: CTAs a row 1 / 2 / 3 / 4 / 5 / 6 / 8, rows of 262144 with top-p:
+//   1 row - / 69 / 55 / 47 / 43 / 40 / 29 us     18 - / 160 / 114 / 92 / 78 / 70 / 81     48 - / 167 / 195 / 149 / 127 / 148 / 142     100 - / 262 / 251 / 232 / 225 / 241 / 250
+// and 512 rows of 32768 without filters 48 / 55 / 79 / 86 / 107 / 126 / 162.
 template <typename T> int launch_sample(LgSampleArgs &a, int dev, void *stream) {
-    const int sms = device_sms(dev), tools = a.top_k || a.top_p ? LG_SAMPLE_TOOLS : 0;
-    int ranks = 1;
-    while (ranks < LG_SAMPLE_MAX_CLUSTER && (a.vocab > ranks << 17 || ((long long)a.rows * ranks * 2 <= sms && a.vocab / (ranks * 2) >= 4096) ||
-                                             ((long long)a.rows * ranks * 2 <= 3 * sms && a.vocab / (ranks * 2) >= 16384))) ranks *= 2;
+    static unsigned char done[64];
+    static int fit[64][2][LG_SAMPLE_MAX_CLUSTER + 1];                         // clusters of so many CTAs that are on the device at once, with one and two CTAs per SM
+    const int both[2] = {220 * 1024, 112 * 1024}, tools = a.top_k || a.top_p ? LG_SAMPLE_TOOLS : 0, slot = dev & 63;
+    if (!allow_smem(lg_sample_kernel<T>, both[0], both[0], dev, done)) SERVE_FAIL(-6, "lg_sample: no %d bytes of shared memory", both[0]);
+    if (!fit[slot][1][1] || dev >= 64)
+        for (int two = 0; two < 2; two++)
+            for (int r = LG_SAMPLE_MAX_CLUSTER; r >= 1; r--) {
+                cudaLaunchConfig_t cfg = {};
+                cudaLaunchAttribute at[1];
+                at[0].id = cudaLaunchAttributeClusterDimension;
+                at[0].val.clusterDim.x = r; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+                cfg.gridDim = dim3(r); cfg.blockDim = dim3(LG_SAMPLE_THREADS); cfg.dynamicSmemBytes = both[two]; cfg.attrs = at; cfg.numAttrs = 1;
+                int n = 0;
+                if (cudaOccupancyMaxActiveClusters(&n, lg_sample_kernel<T>, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = std::max(1, (two + 1) * device_sms(dev) / r); }
+                fit[slot][two][r] = n;
+            }
+    int ranks = 0;
+    double least = 0.0;
+    for (int r = 1; r <= LG_SAMPLE_MAX_CLUSTER; r++) {
+        if (a.vocab > r << 17 || (r > 1 && a.vocab / r < 4096)) continue;
+        const int rest = a.rows % fit[slot][1][r];
+        const double cost = (a.vocab / r + 10000.0) * (a.rows / fit[slot][1][r] * 1.7 + (rest == 0 ? 0.0 : rest <= fit[slot][0][r] ? 1.0 : 1.7));
+        if (!ranks || cost < least) { ranks = r; least = cost; }
+    }
     a.slice = ((a.vocab + ranks - 1) / ranks + 127) / 128 * 128;
-    // shared memory for one CTA per SM where there are no more, else for two; what of the slice does not fit is read again
-    const int most = (long long)a.rows * ranks <= sms ? 220 * 1024 : 112 * 1024;
+    // what of the slice does not fit is read again
+    const int most = both[a.rows > fit[slot][0][ranks]];
     const long long held = (most - tools) / (int)sizeof(T) / 128 * 128;
     a.cap = (int)(a.slice < held ? a.slice : held);
     const size_t smem = (size_t)a.cap * sizeof(T) + tools;
-    static unsigned char done[64];
-    if (!allow_smem(lg_sample_kernel<T>, smem, 220 * 1024, dev, done)) SERVE_FAIL(-6, "lg_sample: no %zu bytes of shared memory", smem);
     return launch_serve("lg_sample", lg_sample_kernel<T>, dim3((unsigned)a.rows * ranks), dim3(LG_SAMPLE_THREADS), smem, stream, false, ranks, a);
 }
 }  // namespace

@@ -486,6 +486,41 @@ def test_captured_calls_follow_lengths_and_tables(lg):
             assert (err <= _tolerance(want, qd, kk, vv, dim ** -0.5, BF16, BF16)).all()
 
 
+FIRST_CALLS = """
+import importlib, torch
+lg = importlib.import_module("little-gemma_b200")
+i32 = lambda *n: torch.zeros(n, dtype=torch.int32, device="cuda")
+x, u, token, p = torch.randn(5, 40000, device="cuda"), torch.rand(5, device="cuda"), i32(5), torch.full((5,), 0.9, device="cuda")
+k, q = torch.randn(20, 16, 2, 128, device="cuda").half(), torch.randn(2, 4, 128, device="cuda")
+c = lg.PagedCache(k, k, torch.arange(20, device="cuda").int().view(2, 10), i32(2) + 100, i32(20), i32(1))
+many = lg.PagedCache(k, k, i32(8192, 1), i32(8192), i32(20), i32(1))
+out, work, start, start2 = torch.empty_like(q), torch.empty(c.attn_work(2, 1, 4), dtype=torch.uint8, device="cuda"), i32(3), i32(8193)
+none, none2, g = i32(2), i32(8192), torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(g):
+    s = torch.cuda.current_stream().cuda_stream
+    c.step(none, start, stream=s)
+    many.step(none2, start2, stream=s)
+    c.attn(q, out, work, stream=s)
+    lg.sample(x, u, token, top_p=p, stream=s)
+g.replay()
+torch.cuda.synchronize()
+want, got = out.clone(), token.clone()
+c.attn(q, out, work)
+lg.sample(x, u, token, top_p=p)
+assert torch.equal(out, want) and torch.equal(token, got) and bool(out.isfinite().all())
+print("the same")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    from tests.conftest import ROOT
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "the same" in r.stdout, r.stderr[-2000:]
+
+
 def test_host_memory_is_refused(lg):
     """Pointers that are no device memory: nothing is launched."""
     import torch

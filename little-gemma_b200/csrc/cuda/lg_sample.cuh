@@ -26,8 +26,8 @@
 #define LG_SAMPLE_COARSE 2048          // bins, four a thread
 #define LG_SAMPLE_BINS 1024            // parts of an interval
 #define LG_SAMPLE_LIST 224             // tokens a warp's list holds
-#define LG_SAMPLE_NEAR 3072            // of these, tokens of a CTA whose place at a threshold is open
-#define LG_SAMPLE_HIST 3072            // words of a histogram: the coarse bins, or three arrays of the parts
+#define LG_SAMPLE_NEAR 2816            // of these, tokens of a CTA whose place at a threshold is open
+#define LG_SAMPLE_HIST (3 * LG_SAMPLE_BINS)    // words of a histogram: the coarse bins, or three arrays of the parts
 #define LG_SAMPLE_TOOLS (2 * LG_SAMPLE_HIST * 4 + LG_SAMPLE_COARSE * 8 + LG_SAMPLE_WARPS * LG_SAMPLE_LIST * 8 + LG_SAMPLE_NEAR * 4)
 #define LG_SAMPLE_MAX_CLUSTER 8
 

@@ -379,6 +379,32 @@ def test_a_bad_row_reaches_only_the_queries_that_see_it(lg, dtype, cache, heads,
                 assert bool(((got - want).abs() <= 2.0 ** -15 * c.v.float().nan_to_num(0, 0, 0).abs().max() + 2 * HALF_STEP[dtype] * want.abs()).all()), (r, t)
 
 
+@pytest.mark.parametrize("dtype,page", [(F16, 16), (BF16, 10)])
+def test_rows_past_two_to_the_31_elements(lg, dtype, page):
+    """A cache of 2.4 G elements: append and attention at its end."""
+    import torch
+    dt, heads, dim = getattr(torch, dtype), 2, 128
+    pages = 2_400_000_000 // (page * heads * dim)
+    k, v = (torch.empty((pages, page, heads, dim), dtype=dt, device="cuda") for _ in range(2))
+    n = 3 * page - 4
+    table = _i32([[pages - 1, pages // 2, pages - 2]])
+    slot = np.concatenate([p * page + np.arange(page) for p in table.cpu().numpy()[0]])[:n]
+    torch.manual_seed(1)
+    rows = [torch.randn((n, heads, dim), device="cuda").to(dt) for _ in range(2)]
+    status = _i32([0])
+    c = lg.PagedCache(k, v, table, _i32([n]), status=status)
+    c.append(rows[0], rows[1], _i32(slot))
+    assert all(torch.equal(x.view(-1, heads, dim)[_i32(slot).long()], r) for x, r in zip((k, v), rows))
+    q = torch.randn((1, 4, dim), device="cuda")
+    out = torch.empty_like(q)
+    c.attn(q, out, torch.empty(c.attn_work(1, 1, 4), dtype=torch.uint8, device="cuda"))
+    kk, vv, qd = rows[0].double().cpu().numpy(), rows[1].double().cpu().numpy(), q.double().cpu().numpy()
+    want = attention(qd, kk, vv, dim ** -0.5, [n - 1])
+    assert (np.abs(out.double().cpu().numpy() - want) <= _tolerance(want, qd, kk, vv, dim ** -0.5, F32, dtype)).all() and status.item() == 0
+    del k, v, c
+    torch.cuda.empty_cache()
+
+
 def test_a_window_of_everything(lg):
     for window in (1 << 20, (1 << 31) - 1):
         _attn_case(lg, 3, [40, 7], [2, 2], 4, 2, 64, 16, F16, F16, window=window)

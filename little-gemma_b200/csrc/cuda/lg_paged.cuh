@@ -336,8 +336,12 @@ __device__ __forceinline__ int paged_len(const LgPagedAttnArgs &a, int r) {
 // of U units of its own (a unit: 16 rows of K or of V; rows that no query may see are filled with zeros and never read), so the loop has no block barrier and
 // runs ahead across items.  Both products have the keys / head dims on the 16-row side and 8 queries as columns:
 //   S^T (16 keys x 8) = K Q^T, softmax with a running maximum per column in the accumulator's own lanes, O^T (16 dims x 8) += V^T P^T,
-// P^T turned from accumulator order into operand order by movmatrix.  Numerics: an f32 query enters as a sum of 16-bit parts (f16: 2 parts behind a
-// power of two per row, 22 bits; bf16: 3, 24 bits), P as 2 parts (3 where the answer is f32 and the cache bf16); P carries a factor 2^15 in f16 so that
+// P^T turned from accumulator order into operand order by movmatrix.  A slice's products are added to the outputs outside of the matrix instructions, with rounding
+// to nearest and the factor of a moved maximum in the same operation: the instructions' own additions cut off, always towards zero, which over 131072 f16 rows of
+// one sign took 8.6e-5 from the result (0.18 of half a step) where this is 1.7e-6 off.  It costs nothing where copies are the bound (96 bf16 requests up to 16383
+// rows: 558 us either way), 17 % with 16-bit heads of 512, 5 to 11 % with 32 query rows a KV head.  Numerics: an f32 query enters as a sum of 16-bit parts (f16: 2 parts behind a
+// power of two per row, 22 bits; bf16: 3, 24 bits), P as 2 parts (3 where the answer is f32 and the cache bf16; 2 of bf16 are 16 bits of a weight, off by 2^-18 of it
+// at most, for an answer of 8 bits); P carries a factor 2^15 in f16 so that
 // weights down to 2^-29 of the largest stay normal numbers.  Everything else is f32.  Rows of an f32 cache are split in registers into three bf16 parts
 // (24 bits); of the nine products of parts the six that reach the last bits of an f32 are computed.
 #define LG_PA_MAX_CTAS 296             // two per SM
@@ -385,6 +389,11 @@ template <typename T> __device__ __forceinline__ bool not_finite(uint4 v) {
     for (int i = 0; i < 4; i++)
         odd |= sizeof(T) == 4 ? (w[i] & e) == e : (w[i] & e & 0xFFFF0000u) == (e & 0xFFFF0000u) || (w[i] & e & 0xFFFFu) == (e & 0xFFFFu);
     return odd;
+}
+// x = x f + a, y = y g + b in one instruction
+__device__ __forceinline__ void fma2(float &x, float &y, float f, float g, float a, float b) {
+    asm("{\n.reg .b64 o, f, a;\nmov.b64 o, {%0, %1};\nmov.b64 f, {%2, %3};\nmov.b64 a, {%4, %5};\nfma.rn.f32x2 o, o, f, a;\nmov.b64 {%0, %1}, o;\n}"
+        : "+f"(x), "+f"(y) : "f"(f), "f"(g), "f"(a), "f"(b));
 }
 __device__ __forceinline__ uint32_t movm(uint32_t a) {
     uint32_t d;
@@ -446,10 +455,7 @@ template <typename TQ, typename TC, int HD, int NT> struct LgPagedTile {
     static constexpr bool F16 = std::is_same<TC, __half>::value;
     static constexpr int NQ = SAME ? 1 : F16 ? 2 : 3;                         // parts of a query
     static constexpr int NP = SAME || F16 ? 2 : 3;                            // parts of a weight
-    // f32 answers: a slice's products are added to the outputs with rounding to nearest; the matrix instructions' own additions cut off, which over the
-    // 500 slices of a warp's stretch cost 2.4e-6 of the result where this leaves 0.8e-6.  (The factor of a moved maximum goes into the same operation.)
-    static constexpr bool RN = sizeof(TQ) == 4;
-    static constexpr bool LONG = RN && HD > 128;                              // scores added up so too, every 128 dims
+    static constexpr bool LONG = sizeof(TQ) == 4 && HD > 128;                 // f32 answers: scores added up with rounding to nearest too, every 128 dims
     static constexpr int KS = HD / 16;
     static constexpr int ROWS = 8 * NT;
     static constexpr int ROW = HD * (int)sizeof(TC), UNIT = 16 * ROW, CHUNKS = ROW / 16;
@@ -734,7 +740,6 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             const int k0 = s * 16;
             const bool all = ok == 0xFFFFu && k0 + 15 <= pos_lo && (a.window <= 0 || k0 > pos_hi - a.window);
             uint32_t pb[NT][P::NP][2];
-            bool moved = false;
             float f[NT][2];
             #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
@@ -757,7 +762,6 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                     m2 = fmaxf(m2, mx[nt][j]);
                     const float ref = m2 == -INFINITY ? 0.0f : m2;
                     f[nt][j] = ex2(mx[nt][j] - ref);
-                    moved |= m2 != mx[nt][j];
                     mx[nt][j] = m2;
                     const float up = P::F16 ? 15.0f : 0.0f;
                     // score minus maximum in one rounding: small next to the maximum, where the weight is
@@ -770,15 +774,6 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                     pb[nt][part][0] = movm(split2<typename P::TM>(x[0], x[1]));
                     pb[nt][part][1] = movm(split2<typename P::TM>(x[2], x[3]));
                 }
-            }
-            if (P::RN) moved = false;                                         // see below
-            if (__any_sync(0xffffffffu, moved)) {
-                #pragma unroll
-                for (int ks = 0; ks < P::KS; ks++)
-                    #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-                        #pragma unroll
-                        for (int j = 0; j < 4; j++) o[ks][nt][j] *= f[nt][j & 1];
             }
             cp_async_wait<P::U - 2>();
             __syncwarp();
@@ -794,14 +789,12 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                 plain = !__any_sync(0xffffffffu, odd);
             }
             if (!plain) {
-                if (P::RN) {
+                #pragma unroll
+                for (int ks = 0; ks < P::KS; ks++)
                     #pragma unroll
-                    for (int ks = 0; ks < P::KS; ks++)
+                    for (int nt = 0; nt < NT; nt++)
                         #pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-                            #pragma unroll
-                            for (int j = 0; j < 4; j++) o[ks][nt][j] *= f[nt][j & 1];
-                }
+                        for (int j = 0; j < 4; j++) o[ks][nt][j] *= f[nt][j & 1];
                 #pragma unroll
                 for (int half = 0; half < 2; half++)
                     #pragma unroll 1
@@ -845,16 +838,13 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    float (&to)[4] = P::RN ? add : o[ks][nt];
                     #pragma unroll
                     for (int part = 0; part < P::NP; part++)
                         #pragma unroll
                         for (int own = 0; own < (P::F32 ? 3 : 1); own++)
-                            if (own + part < 3) mma_16<typename P::TM>(to, v4[own], pb[nt][part][0], pb[nt][part][1]);
-                    if (P::RN) {
-                        #pragma unroll
-                        for (int j = 0; j < 4; j++) o[ks][nt][j] = fmaf(o[ks][nt][j], f[nt][j & 1], add[j]);
-                    }
+                            if (own + part < 3) mma_16<typename P::TM>(add, v4[own], pb[nt][part][0], pb[nt][part][1]);
+                    #pragma unroll
+                    for (int j = 0; j < 4; j += 2) fma2(o[ks][nt][j], o[ks][nt][j + 1], f[nt][0], f[nt][1], add[j], add[j + 1]);
                 }
             }
         }

@@ -559,3 +559,28 @@ def test_host_memory_is_refused(lg):
     with pytest.raises(ValueError):
         c.c.step(torch.zeros(1, dtype=torch.int32), _i32([0, 0]))
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("kv_heads,dim", [(8, 128), (4, 256), (2, 512)])
+def test_long_sums_of_one_sign_have_no_bias(lg, dtype, kv_heads, dim):
+    """16 requests that share one document of 131072 rows, V between 1 and 2.5: answers may differ from the rounded 64-bit ones both ways alike.  A warp adds up
+    at most 131072 / 16 / 2 slices; roundings to nearest of either sign, at most 2^-24 of the sum each, leave sqrt(4096) 2^-24 in the mean where all outputs
+    had them in common (they do not): four times that."""
+    import torch
+    dt, n, R, page, gqa = getattr(torch, dtype), 131072, 16, 64, 4
+    torch.manual_seed(dim)
+    k = torch.randn((n // page, page, kv_heads, dim), device="cuda").to(dt)
+    v = (1 + torch.rand((kv_heads, dim), device="cuda") + 0.5 * torch.rand((n // page, page, kv_heads, dim), device="cuda")).to(dt)
+    c = lg.PagedCache(k, v, _i32(np.tile(np.arange(n // page), (R, 1))), _i32([n] * R))
+    q = (0.3 * torch.randn((R, kv_heads * gqa, dim), device="cuda")).to(dt)
+    out = torch.empty_like(q)
+    c.attn(q, out, torch.empty(c.attn_work(R, 1, kv_heads * gqa), dtype=torch.uint8, device="cuda"))
+    off = []
+    for h in range(kv_heads):
+        p = torch.softmax(q[:, h * gqa:(h + 1) * gqa].double().reshape(-1, dim) @ k[:, :, h].reshape(n, dim).double().T * dim ** -0.5, -1)
+        want = p @ v[:, :, h].reshape(n, dim).double()
+        got = out[:, h * gqa:(h + 1) * gqa].reshape(-1, dim).double()
+        assert bool(((got - want).abs() <= (HALF_STEP[dtype] + 2.0 ** -14) * want).all())      # a tenth of half an f16 step beside the rounding
+        off.append(((got - want.to(dt).double()) / want).mean().item())
+    assert abs(np.mean(off)) <= 4 * 4096 ** 0.5 * 2.0 ** -24, off

@@ -780,10 +780,16 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             issue();
             at = ring_u32 + slot * P::UNIT;
             if (++slot == P::U) slot = 0;
-            // A row that some queries of the block see and others do not (the last rows of a block, the first of its windows): if its V holds inf or NaN, 0 times that
-            // would reach those that do not see it, so such a slice is multiplied key by key.
+            // Rows are here that some query of the request sees; one of this item need not (the last rows of a block, the first of its windows; an item may be
+            // one token of several).  If V of such a row holds inf or NaN, 0 times that would reach queries that do not see it, so the slice is multiplied
+            // key by key.
             bool plain = true;
-            if (!all && pos_lo != pos_hi) {
+            uint32_t every = 0xFFFFu;                                         // rows that every query of the item sees
+            if (!all) {
+                const int behind = k0 + 15 - pos_lo, before = a.window > 0 ? pos_hi - a.window + 1 - k0 : 0;
+                every = behind > 15 || before > 15 ? 0u : (0xFFFFu >> max(behind, 0)) & (0xFFFFu << max(before, 0));
+            }
+            if (ok & ~every) {
                 bool odd = false;
                 for (int i = lane; i < P::UNIT / 16; i += 32) odd |= not_finite<TC>(lds_u4(at + i * 16));
                 plain = !__any_sync(0xffffffffu, odd);

@@ -584,3 +584,32 @@ def test_long_sums_of_one_sign_have_no_bias(lg, dtype, kv_heads, dim):
         assert bool(((got - want).abs() <= (HALF_STEP[dtype] + 2.0 ** -14) * want).all())      # a tenth of half an f16 step beside the rounding
         off.append(((got - want.to(dt).double()) / want).mean().item())
     assert abs(np.mean(off)) <= 4 * 4096 ** 0.5 * 2.0 ** -24, off
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,new", [(8, 1, 512, 4), (7, 1, 512, 3), (8, 2, 512, 5), (16, 1, 256, 4), (8, 2, 256, 5), (32, 1, 128, 2), (64, 2, 64, 8), (40, 1, 80, 3)])
+@pytest.mark.parametrize("window", [0, 20])
+def test_a_bad_row_stays_with_the_tokens_that_see_it_where_a_block_is_several_groups(lg, dtype, cache, heads, kv_heads, dim, new, window):
+    """More query rows a KV head than one tile has: groups of one token and groups across tokens."""
+    import torch
+    lens, m = [100, 33, new + 2], [new] * 3
+    c, q, out, work = _attn_case(lg, 22, lens, m, heads, kv_heads, dim, 16, dtype, cache, window=window)
+    good, table = out.clone(), c.oracle.table
+    top = c.v.float().nan_to_num(0, 0, 0).abs().max()
+    first = [max(0, n - new - window + 1) for n in lens]
+    alone = [window > 0 and f + window <= n - new + 1 for f, n in zip(first, lens)]            # the first token alone sees that row
+    for r, n in enumerate(lens):
+        c.v[table[r, (n - 1) // 16], (n - 1) % 16] = float("nan")                 # the last token alone sees it
+        if alone[r]:
+            c.v[table[r, first[r] // 16], first[r] % 16] = float("inf")
+    c.c.attn(q, out, work, n_new=new, window=window)
+    for r in range(3):
+        for t in range(new):
+            got, want = out[r * new + t].float(), good[r * new + t].float()
+            if t == new - 1:
+                assert bool(got.isnan().all())
+            elif t == 0 and alone[r]:
+                assert not bool(got.isfinite().any())
+            else:
+                # another order of the same sums: f32 rounding of up to 104 terms, then the type's
+                assert bool(((got - want).abs() <= 2.0 ** -15 * top + 2 * HALF_STEP[dtype] * want.abs()).all()), (r, t)

@@ -71,7 +71,9 @@ int  lg_paged_append(const struct lg_paged_cache *c, const void *d_k, const void
  * as lg_paged_step wrote them, at most n_new of them (rows beyond are left as they are, with a status bit), and rows from d_start[n_req] on are left as
  * they are.  The last of a request's m rows is the query at position len - 1, row t the one at len - m + t; it sees the rows at its position and
  * before, with window > 0 the nearest `window` of them.  A query that sees nothing (a length of 0, pages that are not in the cache) gives
- * zeros.  scale 0: 1 / sqrt(head_dim).  What a query does not see does not reach it, inf and NaN included; K rows that it sees are finite.  Every sum has an order that the call's sizes and lengths
+ * zeros.  scale 0: 1 / sqrt(head_dim).  What a query does not see does not reach it, inf and NaN included.  V rows that it sees may hold any
+ * numbers: inf gives inf, inf of both signs or NaN give NaN, and a mean of large numbers is none larger; such calls take several times as long.  q and the
+ * K rows that it sees are finite, below 2^127 where they are f32.  Every sum has an order that the call's sizes and lengths
  * fix: the same call gives the same bits.
  * d_work: lg_paged_attn_work bytes, 16-byte aligned, this call's alone until the call's work has ended: calls and graphs that may
  * overlap have workspaces of their own. */

@@ -305,7 +305,7 @@ struct LgPagedAttnArgs {
     const int *start;
     int gqa, group_rows;               // query heads of a KV head, query rows of an item
     int whole;                         // pages are whole slices
-    float *part; float2 *part_ml;      // [CTA][2][query row of an item]: unnormalised output; maximum and sum
+    float *part; float2 *part_ml;      // [CTA][2][query row of an item]: output over the part's keys; maximum and sum
     int4 *jobs;                        // [CTA]: the item that it leaves unfinished (first row of the request, KV head, last CTA, first of its rows and their number), or -1
 };
 
@@ -328,7 +328,7 @@ __device__ __forceinline__ int paged_len(const LgPagedAttnArgs &a, int r) {
 
 // The work is a line of slices of 16 keys: request by request, KV head by KV head, group of 8 NT query rows by group (an item).  Every CTA of a
 // persistent grid takes a stretch of equal length of that line, so ragged lengths cost nothing; an item that one stretch holds is written at once,
-// of one that several stretches share each leaves (max, sum, unnormalised output), and lg_paged_merge_kernel adds those in their order.
+// of one that several stretches share each leaves (max, sum, output), and lg_paged_merge_kernel adds those in their order.
 // (Spans fixed by a request's own length: 876 us for 96 requests of 1.6K to 16K rows where this takes 539, the copy's bandwidth; short spans cost merges, and
 // about as many items as CTAs leave SMs idle: 153 us for two requests of 120000 rows where this takes 97.)
 //
@@ -371,25 +371,14 @@ template <> __device__ __forceinline__ uint32_t split2<__nv_bfloat16>(float &x, 
 }
 __device__ __forceinline__ float lds_f(uint32_t p) { float v; asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(p)); return v; }
 __device__ __forceinline__ float2 lds_f2(uint32_t p) { float2 v; asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(p)); return v; }
-__device__ __forceinline__ uint4 lds_u4(uint32_t p) { uint4 v; asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p)); return v; }
 __device__ __forceinline__ uint16_t lds_u16(uint32_t p) { uint16_t v; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(p)); return v; }
-// One of two packed 16-bit numbers; one element of a cache in shared memory; whether inf or NaN is among 16 bytes of a cache
-template <typename T> __device__ __forceinline__ float half16(uint32_t w, int high);
-template <> __device__ __forceinline__ float half16<__half>(uint32_t w, int high) { const __half2 h = *(const __half2 *)&w; return high ? __high2float(h) : __low2float(h); }
-template <> __device__ __forceinline__ float half16<__nv_bfloat16>(uint32_t w, int high) { return __uint_as_float(high ? w & 0xFFFF0000u : w << 16); }
+// One element of a cache in shared memory
 template <typename T> __device__ __forceinline__ float lds_elem(uint32_t p);
 template <> __device__ __forceinline__ float lds_elem<float>(uint32_t p) { return lds_f(p); }
 template <> __device__ __forceinline__ float lds_elem<__half>(uint32_t p) { return __half2float(__ushort_as_half(lds_u16(p))); }
 template <> __device__ __forceinline__ float lds_elem<__nv_bfloat16>(uint32_t p) { return __uint_as_float((uint32_t)lds_u16(p) << 16); }
-template <typename T> __device__ __forceinline__ bool not_finite(uint4 v) {
-    constexpr uint32_t e = sizeof(T) == 4 ? 0x7F800000u : std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
-    bool odd = false;
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    #pragma unroll
-    for (int i = 0; i < 4; i++)
-        odd |= sizeof(T) == 4 ? (w[i] & e) == e : (w[i] & e & 0xFFFF0000u) == (e & 0xFFFF0000u) || (w[i] & e & 0xFFFFu) == (e & 0xFFFFu);
-    return odd;
-}
+// A factor that is not 0, so that inf times it is inf; NaN stays
+__device__ __forceinline__ float above_zero(float x) { return x < 1.17549435e-38f ? 1.17549435e-38f : x; }
 // x = x f + a, y = y g + b in one instruction
 __device__ __forceinline__ void fma2(float &x, float &y, float f, float g, float a, float b) {
     asm("{\n.reg .b64 o, f, a;\nmov.b64 o, {%0, %1};\nmov.b64 f, {%2, %3};\nmov.b64 a, {%4, %5};\nfma.rn.f32x2 o, o, f, a;\nmov.b64 {%0, %1}, o;\n}"
@@ -478,8 +467,175 @@ template <typename TQ, typename TC, int HD, int NT> struct LgPagedTile {
     static_assert(U >= 2, "a unit in use and one on its way");
 };
 
+// 16 rows of K or V into a unit; lane i (and i + 16) knows where row i lies, in bytes, bit i of `there` whether it is read
+template <typename P> __device__ __forceinline__ void paged_copy_unit(const void *from, uint32_t dst, long long place, uint32_t there, int row_chunks, int lane) {
+    const unsigned char *base = (const unsigned char *)from;
+    #pragma unroll
+    for (int i = 0; i < P::CHUNKS / 2; i++) {                                 // 32 chunks of 16 bytes at a time
+        const int idx = i * 32 + lane, row = idx / P::CHUNKS, c = idx % P::CHUNKS;
+        const long long off = __shfl_sync(0xffffffffu, place, row);
+        const bool rd = (there >> row & 1) && c < row_chunks;
+        cp_async16_or_zero(dst + row * P::ROW + (P::place(row, c) << 4), rd ? base + off + c * 16 : base, rd);
+    }
+}
+// Scores of a slice whose K lies at `at`; query(i): fragment i of the queries
+template <typename P, int NT, typename Q> __device__ __forceinline__ void paged_scores(uint32_t at, int lane, Q &&query, float (&x)[NT][4]) {
+    const int g = lane >> 2, t4 = lane & 3;
+    float sc[NT][2][4];                                                       // two chains of products
+    #pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+        #pragma unroll
+        for (int j = 0; j < 4; j++) sc[nt][0][j] = sc[nt][1][j] = 0.0f;
+    float sum[P::LONG ? NT : 1][4];
+    if (P::LONG) {
+        #pragma unroll
+        for (int nt = 0; nt < NT; nt++) sum[nt][0] = sum[nt][1] = sum[nt][2] = sum[nt][3] = 0.0f;
+    }
+    #pragma unroll
+    for (int ks = 0; ks < P::KS; ks++) {
+        uint32_t k4[P::F32 ? 3 : 1][4];                                       // parts of 16 rows x 16 dims
+        if constexpr (P::F32) {
+            #pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int row = g + (e & 1) * 8;
+                float2 x = lds_f2(at + row * P::ROW + (P::place(row, 4 * ks + 2 * (e >> 1) + (t4 >> 1)) << 4) + (t4 & 1) * 8);
+                #pragma unroll
+                for (int part = 0; part < 3; part++) k4[part][e] = split2<typename P::TM>(x.x, x.y);
+            }
+        } else {
+            const int row = (lane & 7) + (lane & 8);
+            ldsm_x4_u32(k4[0], at + row * P::ROW + (P::place(row, 2 * ks + (lane >> 4)) << 4));
+        }
+        #pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+            #pragma unroll
+            for (int part = 0; part < P::NQ; part++) {
+                const uint2 v = query((nt * P::NQ + part) * P::KS + ks);
+                #pragma unroll
+                for (int own = 0; own < (P::F32 ? 3 : 1); own++)
+                    if (own + part < 3) mma_16<typename P::TM>(sc[nt][ks & 1], k4[own], v.x, v.y);
+            }
+        if (P::LONG && ks % 8 == 7 && ks != P::KS - 1) {
+            #pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+                #pragma unroll
+                for (int j = 0; j < 4; j++) { sum[nt][j] += sc[nt][0][j] + sc[nt][1][j]; sc[nt][0][j] = sc[nt][1][j] = 0.0f; }
+        }
+    }
+    #pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+        #pragma unroll
+        for (int j = 0; j < 4; j++) {
+            x[nt][j] = sc[nt][0][j] + sc[nt][1][j];
+            if (P::LONG) x[nt][j] += sum[nt][j];
+        }
+}
+// -inf for the scores of keys that a query (at position top) does not see
+__device__ __forceinline__ void paged_mask(float (&x)[4], const int (&top)[2], uint32_t ok, int k0, int window, int g) {
+    #pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int key = k0 + g + (j >> 1) * 8, pos = top[j & 1];
+        if (!(ok >> (g + (j >> 1) * 8) & 1) || key > pos || (window > 0 && key <= pos - window)) x[j] = -INFINITY;
+    }
+}
+// Scores of two columns into weights 2^(score - reference); the reference is the running maximum (and `lift`), f: what an old sum is multiplied by
+template <typename P> __device__ __forceinline__ void paged_weights(float (&x)[4], const float (&cs)[2], float (&mx)[2], float (&l)[2], float lift, float (&f)[2]) {
+    #pragma unroll
+    for (int j = 0; j < 2; j++) {
+        float m2 = fmaxf(x[j], x[j + 2]) * cs[j];
+        m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, 4));
+        m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, 8));
+        m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, 16));
+        m2 = fmaxf(lift != 0.0f ? m2 + lift : m2, mx[j]);
+        const float ref = m2 == -INFINITY ? 0.0f : m2;
+        f[j] = ex2(mx[j] - ref);
+        mx[j] = m2;
+        const float up = P::F16 ? 15.0f : 0.0f;
+        // score minus maximum in one rounding: small next to the maximum, where the weight is
+        x[j] = ex2(fmaf(x[j], cs[j], up - ref));
+        x[j + 2] = ex2(fmaf(x[j + 2], cs[j], up - ref));
+        l[j] = l[j] * f[j] + (x[j] + x[j + 2]);
+    }
+}
+
+// A warp's slices s, s + W .. of an item once more, where inf or NaN was among its outputs: the matrix instructions multiply every loaded row with all parts of a
+// weight, and 0 times inf is NaN -- for a query that does not see the row (the last rows of a block, the first of its windows), and for a part that is 0; f32
+// numbers above bf16's largest become inf in parts; and sums of numbers near the largest run over.  Here V is multiplied key by key, where a query
+// sees the key, with the whole weight, 2^-32 of what it is elsewhere (f16, which runs over nowhere: the same).  8 query rows at a time, so that it takes few
+// registers from the loop's; copies go to `unit` and are waited for.  res: [NT][KS + 1][4], 2 maxima and 2 sums, then the outputs.
 template <typename TQ, typename TC, int HD, int NT>
-__global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPagedTile<TQ, TC, HD, NT>::CTAS)) lg_paged_attn_kernel(LgPagedAttnArgs a) {
+__device__ __forceinline__ void paged_key_by_key(const LgPagedAttnArgs &a, const LgReq &q, int r, int head, int row0, int n_rows, int s0, int s_end, uint32_t unit,
+                                                 const uint32_t *sq, const float *cscale, float *res) {
+    typedef LgPagedTile<TQ, TC, HD, NT> P;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3, ps = a.c.page_size, row_chunks = a.c.hd * (int)sizeof(TC) / 16;
+    const int hi = q.len - q.held + q.m, lo = a.window > 0 ? q.len - q.held - a.window + 1 : 0;
+    #pragma unroll 1
+    for (int nt = 0; nt < NT; nt++) {
+        float cs[2], mx[2], l[2], o[P::KS][4];
+        int top[2];
+        #pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int n = nt * 8 + 2 * t4 + j;
+            cs[j] = cscale[n]; mx[j] = -INFINITY; l[j] = 0.0f;
+            top[j] = q.len - q.held + (row0 + min(n, n_rows - 1)) / a.gqa;
+        }
+        #pragma unroll
+        for (int ks = 0; ks < P::KS; ks++)
+            #pragma unroll
+            for (int j = 0; j < 4; j++) o[ks][j] = 0.0f;
+        #pragma unroll 1
+        for (int s = s0; s < s_end; s += P::W) {
+            const int key = s * 16 + (lane & 15), n = key / ps;
+            const long long place = key < hi && key >= lo ? paged_place(a.c, a.c.table[(size_t)r * a.c.table_stride + n], key - n * ps, head) : -1;
+            const uint32_t ok = __ballot_sync(0xffffffffu, place >= 0) & 0xFFFFu;
+            auto bring = [&](const void *from) {
+                __syncwarp();                                                 // what lies there has been read
+                paged_copy_unit<P>(from, unit, max(place, 0LL) * (int)sizeof(TC), ok, row_chunks, lane);
+                cp_async_commit();
+                cp_async_wait<0>();
+                __syncwarp();
+            };
+            float x[1][4], f[2];
+            bring(a.c.k);
+            paged_scores<P, 1>(unit, lane, [&](int i) { return *(const uint2 *)(sq + ((nt * P::NQ * P::KS + i) * 32 + lane) * 2); }, x);
+            paged_mask(x[0], top, ok, s * 16, a.window, g);
+            paged_weights<P>(x[0], cs, mx, l, P::F16 ? 0.0f : 32.0f, f);
+            bring(a.c.v);
+            #pragma unroll
+            for (int ks = 0; ks < P::KS; ks++)
+                #pragma unroll
+                for (int j = 0; j < 4; j++) o[ks][j] *= above_zero(f[j & 1]);
+            #pragma unroll 1
+            for (int row = 0; row < 16; row++) {
+                const int at = s * 16 + row;
+                #pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float p = __shfl_sync(0xffffffffu, row < 8 ? x[0][j] : x[0][2 + j], (row & 7) * 4 + t4);
+                    if (!(ok >> row & 1) || at > top[j] || (a.window > 0 && at <= top[j] - a.window)) continue;
+                    #pragma unroll
+                    for (int ks = 0; ks < P::KS; ks++)
+                        #pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int byte = (16 * ks + 8 * h + g) * (int)sizeof(TC);
+                            const float y = lds_elem<TC>(unit + row * P::ROW + (P::place(row, byte >> 4) << 4) + (byte & 15));
+                            o[ks][2 * h + j] += fabsf(y) < INFINITY ? p * y : y;               // (the smallest weights are 0 here)
+                        }
+                }
+            }
+        }
+        float *to = res + nt * 4 * (P::KS + 1);
+        #pragma unroll
+        for (int j = 0; j < 2; j++) { to[j] = mx[j]; to[2 + j] = l[j]; }
+        #pragma unroll
+        for (int ks = 0; ks < P::KS; ks++)
+            #pragma unroll
+            for (int j = 0; j < 4; j++) to[4 + ks * 4 + j] = o[ks][j];
+    }
+    __syncwarp();
+}
+
+template <typename TQ, typename TC, int HD, int NT>
+__global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPagedTile<TQ, TC, HD, NT>::CTAS)) lg_paged_attn_kernel(const __grid_constant__ LgPagedAttnArgs a) {
     typedef LgPagedTile<TQ, TC, HD, NT> P;
     extern __shared__ __align__(128) unsigned char lg_pa_sm[];
     unsigned char *ring = lg_pa_sm;
@@ -590,15 +746,7 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                 pok = a.whole ? pg >= 0 ? (0xFFFFu << first) & (0xFFFFu >> (16 - last)) : 0u : __ballot_sync(0xffffffffu, pg >= 0) & 0xFFFFu;
                 if (lane == 0) vmask[warp * 16 + ((n_issued >> 1) & 15)] = pok;
             }
-            const unsigned char *base = (const unsigned char *)(is_v ? a.c.v : a.c.k);
-            const uint32_t dst = ring_u32 + slot_in * P::UNIT;
-            #pragma unroll
-            for (int i = 0; i < P::CHUNKS / 2; i++) {                         // 32 chunks of 16 bytes at a time
-                const int idx = i * 32 + lane, row = idx / P::CHUNKS, c = idx % P::CHUNKS;
-                const long long off = __shfl_sync(0xffffffffu, poff, row);
-                const bool rd = (pok >> row & 1) && c < row_chunks;
-                cp_async16_or_zero(dst + row * P::ROW + (P::place(row, c) << 4), rd ? base + off + c * 16 : base, rd);
-            }
+            paged_copy_unit<P>(is_v ? a.c.v : a.c.k, ring_u32 + slot_in * P::UNIT, poff, pok, row_chunks, lane);
             if (is_v) {
                 ps += P::W;
                 nth++;
@@ -676,16 +824,18 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int n = nt * 8 + 2 * t4 + j;
-                cs[nt][j] = cscale[n]; mx[nt][j] = -INFINITY; l[nt][j] = 0.0f;
+                cs[nt][j] = cscale[n];
                 top[nt][j] = pos0 + (row0 + min(n, n_rows - 1)) / a.gqa;
             }
+        const int pos_lo = pos0 + row0 / a.gqa, pos_hi = pos0 + (row0 + n_rows - 1) / a.gqa;
+        #pragma unroll
+        for (int nt = 0; nt < NT; nt++) { mx[nt][0] = mx[nt][1] = -INFINITY; l[nt][0] = l[nt][1] = 0.0f; }
         #pragma unroll
         for (int ks = 0; ks < P::KS; ks++)
             #pragma unroll
             for (int nt = 0; nt < NT; nt++)
                 #pragma unroll
                 for (int j = 0; j < 4; j++) o[ks][nt][j] = 0.0f;
-        const int pos_lo = pos0 + row0 / a.gqa, pos_hi = pos0 + (row0 + n_rows - 1) / a.gqa;
         for (int s = s_begin + warp; s < s_end; s += P::W) {
             cp_async_wait<P::U - 2>();
             __syncwarp();
@@ -693,86 +843,21 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             const uint32_t ok = vmask[warp * 16 + ((n_used++) & 15)];
             uint32_t at = ring_u32 + slot * P::UNIT;
             if (++slot == P::U) slot = 0;
-            float sc[NT][2][4];                                               // two chains of products
-            #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-                #pragma unroll
-                for (int j = 0; j < 4; j++) sc[nt][0][j] = sc[nt][1][j] = 0.0f;
-            float sum[P::LONG ? NT : 1][4];
-            if (P::LONG) {
-                #pragma unroll
-                for (int nt = 0; nt < NT; nt++) sum[nt][0] = sum[nt][1] = sum[nt][2] = sum[nt][3] = 0.0f;
-            }
-            #pragma unroll
-            for (int ks = 0; ks < P::KS; ks++) {
-                uint32_t k4[P::F32 ? 3 : 1][4];                               // parts of 16 rows x 16 dims
-                if constexpr (P::F32) {
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int row = g + (e & 1) * 8;
-                        float2 x = lds_f2(at + row * P::ROW + (P::place(row, 4 * ks + 2 * (e >> 1) + (t4 >> 1)) << 4) + (t4 & 1) * 8);
-                        #pragma unroll
-                        for (int part = 0; part < 3; part++) k4[part][e] = split2<typename P::TM>(x.x, x.y);
-                    }
-                } else {
-                    const int row = (lane & 7) + (lane & 8);
-                    ldsm_x4_u32(k4[0], at + row * P::ROW + (P::place(row, 2 * ks + (lane >> 4)) << 4));
-                }
-                #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-                    #pragma unroll
-                    for (int part = 0; part < P::NQ; part++) {
-                        const int i = (nt * P::NQ + part) * P::KS + ks;
-                        uint2 v;
-                        if (P::QREG) v = make_uint2(qr[2 * i], qr[2 * i + 1]);
-                        else v = *(const uint2 *)(sq + (i * 32 + lane) * 2);
-                        #pragma unroll
-                        for (int own = 0; own < (P::F32 ? 3 : 1); own++)
-                            if (own + part < 3) mma_16<typename P::TM>(sc[nt][ks & 1], k4[own], v.x, v.y);
-                    }
-                if (P::LONG && ks % 8 == 7 && ks != P::KS - 1) {
-                    #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-                        #pragma unroll
-                        for (int j = 0; j < 4; j++) { sum[nt][j] += sc[nt][0][j] + sc[nt][1][j]; sc[nt][0][j] = sc[nt][1][j] = 0.0f; }
-                }
-            }
-            const int k0 = s * 16;
-            const bool all = ok == 0xFFFFu && k0 + 15 <= pos_lo && (a.window <= 0 || k0 > pos_hi - a.window);
+            float x[NT][4], f[NT][2];
+            paged_scores<P, NT>(at, lane, [&](int i) {
+                if (P::QREG) return make_uint2(qr[P::QREG ? 2 * i : 0], qr[P::QREG ? 2 * i + 1 : 0]);
+                return *(const uint2 *)(sq + (i * 32 + lane) * 2);
+            }, x);
+            const bool all = ok == 0xFFFFu && s * 16 + 15 <= pos_lo && (a.window <= 0 || s * 16 > pos_hi - a.window);
             uint32_t pb[NT][P::NP][2];
-            float f[NT][2];
             #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                float x[4];
-                #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    x[j] = sc[nt][0][j] + sc[nt][1][j];
-                    if (P::LONG) x[j] += sum[nt][j];
-                    if (!all) {
-                        const int key = k0 + g + (j >> 1) * 8, pos = top[nt][j & 1];
-                        if (!(ok >> (g + (j >> 1) * 8) & 1) || key > pos || (a.window > 0 && key <= pos - a.window)) x[j] = -INFINITY;
-                    }
-                }
-                #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    float m2 = fmaxf(x[j], x[j + 2]) * cs[nt][j];
-                    m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, 4));
-                    m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, 8));
-                    m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, 16));
-                    m2 = fmaxf(m2, mx[nt][j]);
-                    const float ref = m2 == -INFINITY ? 0.0f : m2;
-                    f[nt][j] = ex2(mx[nt][j] - ref);
-                    mx[nt][j] = m2;
-                    const float up = P::F16 ? 15.0f : 0.0f;
-                    // score minus maximum in one rounding: small next to the maximum, where the weight is
-                    x[j] = ex2(fmaf(x[j], cs[nt][j], up - ref));
-                    x[j + 2] = ex2(fmaf(x[j + 2], cs[nt][j], up - ref));
-                    l[nt][j] = l[nt][j] * f[nt][j] + (x[j] + x[j + 2]);
-                }
+                if (!all) paged_mask(x[nt], top[nt], ok, s * 16, a.window, g);
+                paged_weights<P>(x[nt], cs[nt], mx[nt], l[nt], 0.0f, f[nt]);
                 #pragma unroll
                 for (int part = 0; part < P::NP; part++) {
-                    pb[nt][part][0] = movm(split2<typename P::TM>(x[0], x[1]));
-                    pb[nt][part][1] = movm(split2<typename P::TM>(x[2], x[3]));
+                    pb[nt][part][0] = movm(split2<typename P::TM>(x[nt][0], x[nt][1]));
+                    pb[nt][part][1] = movm(split2<typename P::TM>(x[nt][2], x[nt][3]));
                 }
             }
             cp_async_wait<P::U - 2>();
@@ -780,51 +865,6 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             issue();
             at = ring_u32 + slot * P::UNIT;
             if (++slot == P::U) slot = 0;
-            // Rows are here that some query of the request sees; one of this item need not (the last rows of a block, the first of its windows; an item may be
-            // one token of several).  If V of such a row holds inf or NaN, 0 times that would reach queries that do not see it, so the slice is multiplied
-            // key by key.
-            bool plain = true;
-            uint32_t every = 0xFFFFu;                                         // rows that every query of the item sees
-            if (!all) {
-                const int behind = k0 + 15 - pos_lo, before = a.window > 0 ? pos_hi - a.window + 1 - k0 : 0;
-                every = behind > 15 || before > 15 ? 0u : (0xFFFFu >> max(behind, 0)) & (0xFFFFu << max(before, 0));
-            }
-            if (ok & ~every) {
-                bool odd = false;
-                for (int i = lane; i < P::UNIT / 16; i += 32) odd |= not_finite<TC>(lds_u4(at + i * 16));
-                plain = !__any_sync(0xffffffffu, odd);
-            }
-            if (!plain) {
-                #pragma unroll
-                for (int ks = 0; ks < P::KS; ks++)
-                    #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-                        #pragma unroll
-                        for (int j = 0; j < 4; j++) o[ks][nt][j] *= f[nt][j & 1];
-                #pragma unroll
-                for (int half = 0; half < 2; half++)
-                    #pragma unroll 1
-                    for (int k = 0; k < 8; k++) {
-                        const int row = half * 8 + k, key = k0 + row;
-                        #pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-                            #pragma unroll
-                            for (int j = 0; j < 2; j++) {
-                                float x = 0.0f;                               // the weight, from the lane that has it as an operand
-                                #pragma unroll
-                                for (int part = P::NP - 1; part >= 0; part--) x += half16<typename P::TM>(__shfl_sync(0xffffffffu, pb[nt][part][half], (2 * t4 + j) * 4 + (k >> 1)), k & 1);
-                                if (!(ok >> row & 1) || key > top[nt][j] || (a.window > 0 && key <= top[nt][j] - a.window)) continue;
-                                #pragma unroll
-                                for (int ks = 0; ks < P::KS; ks++)
-                                    #pragma unroll
-                                    for (int h = 0; h < 2; h++) {
-                                        const int d = 16 * ks + 8 * h + g, byte = d * (int)sizeof(TC);
-                                        o[ks][nt][2 * h + j] += x * lds_elem<TC>(at + row * P::ROW + (P::place(row, byte >> 4) << 4) + (byte & 15));
-                                    }
-                            }
-                    }
-                continue;
-            }
             #pragma unroll
             for (int ks = 0; ks < P::KS; ks++) {
                 uint32_t v4[P::F32 ? 3 : 1][4];                               // parts of 16 dims x 16 rows
@@ -854,6 +894,28 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                 }
             }
         }
+        __syncwarp();
+        float odd = 0.0f;                                                     // NaN where an output is inf or NaN
+        #pragma unroll
+        for (int ks = 0; ks < P::KS; ks++)
+            #pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+                #pragma unroll
+                for (int j = 0; j < 4; j++) odd = fmaf(o[ks][nt][j], 0.0f, odd);
+        if (__any_sync(0xffffffffu, odd != odd)) {
+            float res[NT * 4 * (P::KS + 1)];
+            paged_key_by_key<TQ, TC, HD, NT>(a, w.q, w.r, kvh, row0, n_rows, s_begin + warp, s_end, ring_u32 + slot_in * P::UNIT, sq, cscale, res);
+            #pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const float *from = res + nt * 4 * (P::KS + 1);
+                #pragma unroll
+                for (int j = 0; j < 2; j++) { mx[nt][j] = from[j]; l[nt][j] = from[2 + j]; }
+                #pragma unroll
+                for (int ks = 0; ks < P::KS; ks++)
+                    #pragma unroll
+                    for (int j = 0; j < 4; j++) o[ks][nt][j] = from[4 + ks * 4 + j];
+            }
+        }
         // the warps' results into one, in warp order
         #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -869,18 +931,24 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
         const bool head = w.at < 0, tail = w.at + w.q.n_sl > length;
         const long long part = ((long long)blockIdx.x * 2 + !head) * P::ROWS;
         if (!head && tail && tid == 0) a.jobs[blockIdx.x] = make_int4(w.q.first, kvh, (int)blockIdx.x + (w.at + w.q.n_sl - 1) / stretch, row0 << 8 | n_rows);
-        // row n of the item: its maximum, sum and the warps' factors, then (put) its numbers
-        auto finish = [&](int n, int first, int step, auto &&number) {
-            float m2 = -INFINITY, sum = 0.0f, fw[P::W];
+        // row n of the item: its maximum and sum, and what the warps' outputs are multiplied by -- together at most 1, so that their sum does not run over
+        auto factors = [&](int n, float &m2, float &sum, float (&fw)[P::W]) {
+            m2 = -INFINITY; sum = 0.0f;
             #pragma unroll
             for (int i = 0; i < P::W; i++) m2 = fmaxf(m2, stat[i * P::ROWS + n].x);
             #pragma unroll
             for (int i = 0; i < P::W; i++) { fw[i] = ex2(stat[i * P::ROWS + n].x - (m2 == -INFINITY ? 0.0f : m2)); sum += stat[i * P::ROWS + n].y * fw[i]; }
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            #pragma unroll
+            for (int i = 0; i < P::W; i++) fw[i] = above_zero(fw[i] * inv);
+        };
+        auto finish = [&](int n, int first, int step, auto &&number) {
+            float m2, sum, fw[P::W];
+            factors(n, m2, sum, fw);
             const int rho = row0 + n, t = rho / a.gqa, h = kvh * a.gqa + rho - t * a.gqa;
             if (!head && !tail) {
                 TQ *out = (TQ *)a.out + (long long)(w.q.first + t) * a.ld_out + (long long)h * a.c.hd;
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                for (int d = first; d < a.c.hd; d += step) out[d] = Elem<TQ>::put(number(d, fw) * inv);
+                for (int d = first; d < a.c.hd; d += step) out[d] = Elem<TQ>::put(number(d, fw));
             } else {
                 for (int d = first; d < a.c.hd; d += step) a.part[(part + n) * a.c.hd + d] = number(d, fw);
                 if (first == 0) a.part_ml[part + n] = make_float2(m2, sum);
@@ -917,10 +985,10 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
             for (int nt = 0; nt < NT; nt++)
                 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    float m2 = -INFINITY;
+                    float m2, sum, fw[P::W];
+                    factors(nt * 8 + 2 * t4 + j, m2, sum, fw);
                     #pragma unroll
-                    for (int i = 0; i < P::W; i++) m2 = fmaxf(m2, stat[i * P::ROWS + nt * 8 + 2 * t4 + j].x);
-                    f[nt][j] = ex2(mx[nt][j] - (m2 == -INFINITY ? 0.0f : m2));
+                    for (int i = 0; i < P::W; i++) if (i == warp) f[nt][j] = fw[i];
                 }
             for (int i = 0; i < P::W; i++) {
                 if (warp == i) {
@@ -971,8 +1039,8 @@ template <typename TQ> __global__ void __launch_bounds__(256) lg_paged_merge_ker
     for (int k = 0; k < 16; k++) y[k] = 0.0f;
     for (int i = warp; i < parts; i += 8) {
         const float2 ml = a.part_ml[place(i)];
-        const float f = ex2(ml.x - ref);
-        sum += ml.y * f;
+        const float f = above_zero(ex2(ml.x - ref) * (ml.y * 0x1p-46f));      // sums are at most 2^15 of 2^30 rows: outputs times this do not run over
+        sum += f;
         if (i != warp) load(i);
         #pragma unroll
         for (int k = 0; k < 4; k++)

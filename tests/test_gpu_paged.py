@@ -613,3 +613,79 @@ def test_a_bad_row_stays_with_the_tokens_that_see_it_where_a_block_is_several_gr
             else:
                 # another order of the same sums: f32 rounding of up to 104 terms, then the type's
                 assert bool(((got - want).abs() <= 2.0 ** -15 * top + 2 * HALF_STEP[dtype] * want.abs()).all()), (r, t)
+
+
+def _again(c, q, out, work, lens, m, kv_heads, window, dtype, cache, top=None):
+    """The call on changed V rows against the 64-bit form: inf, NaN and finite numbers in the same places, the finite ones within _tolerance()."""
+    c.c.attn(q, out, work, n_new=max(m), window=window)
+    got, qd, table, at = out.double().cpu().numpy(), q.double().cpu().numpy(), c.oracle.table, 0
+    for r, n in enumerate(lens):
+        k, v = ((x[table[r, : -(-n // 16)]].double().flatten(0, 1)[:n]).cpu().numpy() for x in (c.k, c.v))
+        positions = [n - m[r] + t for t in range(m[r])]
+        lowest = max(0, positions[0] - window + 1) if window else 0
+        k, v = k[lowest:], v[lowest:]
+        with np.errstate(invalid="ignore"):
+            want = attention(qd[at:at + m[r]], k, v, q.shape[-1] ** -0.5, [p - lowest for p in positions], window)
+        g = got[at:at + m[r]]
+        assert np.array_equal(np.isnan(g), np.isnan(want)), r
+        fine = np.isfinite(want)
+        assert np.array_equal(g[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)]), r
+        flat = np.nan_to_num(v, nan=0.0, posinf=0.0, neginf=0.0)
+        tol = _tolerance(np.where(fine, want, 0.0), qd[at:at + m[r]], k, flat, q.shape[-1] ** -0.5, dtype, cache)
+        assert (np.abs(g - want)[fine] <= tol[fine]).all(), r
+        at += m[r]
+    assert c.status.item() == 0
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,new,window", [(2, 1, 64, 1, 0), (8, 2, 128, 1, 100), (32, 1, 128, 2, 0), (16, 2, 256, 4, 20), (3, 1, 80, 3, 0), (8, 1, 512, 2, 0), (2, 2, 512, 1, 40)])
+def test_infinities_in_v_as_the_formula(lg, dtype, cache, heads, kv_heads, dim, new, window):
+    """inf times a weight, however small, is inf; two of either sign are NaN; the other dims are as ever."""
+    inf, lens, m = float("inf"), [300, 40, 17 + new, 6000], [new] * 4
+    c, q, out, work = _attn_case(lg, 41, lens, m, heads, kv_heads, dim, 16, dtype, cache, window=window)
+    table = c.oracle.table
+    for r, n in enumerate(lens):
+        for back, d, x in ((1, 3, inf), (9, 4, -inf), (10, 4, -inf), (11, 5, inf), (12, 5, -inf), (12, 6, float("nan")), (13, 7, inf)):
+            c.v[table[r, (n - back) // 16], (n - back) % 16, kv_heads - 1, d] = x
+        if not window:
+            c.v[table[r, 0], 0, 0, 1] = inf                    # far from the last row: other warps and CTAs join it
+    _again(c, q, out, work, lens, m, kv_heads, window, dtype, cache)
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_infinities_in_v_behind_weights_near_zero(lg, dtype, cache):
+    """Weights of 1e-43 to 1e-130 of the largest: 0 in 32 bits, not in the formula."""
+    lens = [100, 3000]
+    c, q, out, work = _attn_case(lg, 42, lens, [1, 1], 2, 1, 64, 16, dtype, cache)
+    table = c.oracle.table
+    for r, n in enumerate(lens):
+        # the last row leans towards head 0's query: its score is 100 to 300 above all others
+        c.k[table[r, (n - 1) // 16], (n - 1) % 16] = (q[r, 0].float() * (200.0 * 8 / q[r, 0].float().square().sum())).to(c.k.dtype)
+        for i in (0, 20, n - 2):
+            c.v[table[r, i // 16], i % 16, 0, i % 7] = float("-inf")
+    c.c.attn(q, out, work)
+    for r, n in enumerate(lens):
+        bad = {i % 7 for i in (0, 20, n - 2)}
+        got = out[r, 0]
+        assert all(got[d].item() == float("-inf") for d in bad), r
+        last = c.v[table[r, (n - 1) // 16], (n - 1) % 16, 0].float()
+        rest = [d for d in range(64) if d not in bad]
+        assert bool(((got[rest].float() - last[rest]).abs() <= 2.0 ** -16 * last.abs().max() + HALF_STEP[dtype] * last[rest].abs()).all()), r
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,new", [(2, 1, 64, 1), (16, 2, 128, 4), (4, 1, 256, 1), (8, 1, 512, 2)])
+def test_v_near_the_largest_number_of_its_type(lg, dtype, cache, heads, kv_heads, dim, new):
+    """A mean of numbers is none larger, wherever it is added up: in a warp, over warps, over CTAs."""
+    import torch
+    lens, m = [1 + new, 7, 90, 20011], [new] * 4
+    c, q, out, work = _attn_case(lg, 43, lens, m, heads, kv_heads, dim, 16, dtype, cache)
+    most = torch.finfo(c.v.dtype).max
+    for share in (1.0, 0.6):
+        c.v.fill_(most * share)
+        c.v[..., 1::2] = -most * share
+        c.c.attn(q, out, work, n_new=new)
+        want = c.v[0, 0, 0].double()                           # as the cache holds it
+        # equal numbers: the sum of the weights over itself, 16 f32 roundings, then the type's; at the very top one of them may go over it
+        near = (out.double() - want).abs() <= (2.0 ** -16 + HALF_STEP[dtype]) * most * share
+        assert bool((near | ((share == 1.0) & (out.double() == want.sign() * float("inf")))).all()) and not bool(out.isnan().any()), share

@@ -55,7 +55,8 @@ long long lg_debug_paged_place(const struct lg_paged_cache *c, int page, int row
  * each row its position, its slot (page * page_size + row in the page) and its request, in d_pos, d_slot, d_req [cap] (each may be
  * NULL), -1 in rows behind the last token.
  * Requests are served in order while pages and rows (cap) last: one that needs more than is left, or more than max_pages, stays as it is,
- * with no token in the step.  Values of d_keep above len count as len, negative ones as 0.  Tables and outputs do not overlap. */
+ * with no token in the step.  Values of d_keep above len count as len, negative ones as 0.  An entry of the table that is no page goes onto the
+ * stack as -1, and whoever takes that has rows without slots.  Tables and outputs do not overlap. */
 int  lg_paged_step(const struct lg_paged_cache *c, int n_req, const int *d_keep, const int *d_new, int cap, int *d_start, int *d_pos,
                    int *d_slot, int *d_req, void *stream);
 

@@ -193,8 +193,9 @@ template <int PER> __global__ void __launch_bounds__(LG_STEP_THREADS, 1) lg_page
     // those given up go onto the stack, over what was taken from it, the last one first; lengths
     const int base = n_free - (int)all[0];
     auto back = [&](int *e, long long to) {
-        if (to < a.c.n_pages && *e >= 0 && *e < a.c.n_pages) a.c.free_pages[to] = *e;
-        else paged_raise(a.c, LG_PAGED_BAD_PAGE);
+        const bool page = *e >= 0 && *e < a.c.n_pages;                        // what is none has a place on the stack all the same, and must not leave a page there
+        if (to < a.c.n_pages) a.c.free_pages[to] = page ? *e : -1;            // that another request took from it
+        if (!page || to >= a.c.n_pages) paged_raise(a.c, LG_PAGED_BAD_PAGE);
         *e = -1;
     };
     #pragma unroll

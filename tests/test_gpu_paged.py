@@ -689,3 +689,29 @@ def test_v_near_the_largest_number_of_its_type(lg, dtype, cache, heads, kv_heads
         # equal numbers: the sum of the weights over itself, 16 f32 roundings, then the type's; at the very top one of them may go over it
         near = (out.double() - want).abs() <= (2.0 ** -16 + HALF_STEP[dtype]) * most * share
         assert bool((near | ((share == 1.0) & (out.double() == want.sign() * float("inf")))).all()) and not bool(out.isnan().any()), share
+
+
+@pytest.mark.parametrize("n", [2, 2000])
+def test_an_entry_that_is_no_page_brings_none_back(lg, n):
+    """Released with a bad entry in its table: the stack must not show again what another request took from that place."""
+    rng = np.random.default_rng(n)
+    c = _Cache(lg, rng, [8, 4] + [5] * (n - 2), 4, 6, 3 + 2 * n)
+    c.step([8, 0] + [1] * (n - 2), 9 + n)                      # request 0 takes the two pages at the top
+    c.table[1, 0] = -5
+    c.table[n - 1, 0] = c.k.shape[0]
+    c.step([0] * n, 0, [1 << 30, 0] + [0] * (n - 2))
+    assert c.status.item() == Pages.BAD_PAGE
+
+    def pages():
+        table, lens, n_free = c.table.cpu().numpy(), c.len.cpu().numpy(), c.n_free.item()
+        held = [int(x) for r in range(n) for x in table[r, : -(-int(lens[r]) // 4)]] + [int(x) for x in c.free.cpu().numpy()[:n_free]]
+        return [p for p in held if 0 <= p < c.k.shape[0]]
+
+    assert len(set(pages())) == len(pages()) == c.k.shape[0] - (1 if n == 2 else 2)          # a bad entry's own page is lost
+    c.status.zero_()
+    start, _, slot, req = c.step([0] + [9] * (n - 1), 9 * n)
+    live = [int(s) for s in slot.tolist() if s >= 0]
+    assert len(set(pages())) == len(pages()) and len(set(live)) == len(live)
+    assert c.status.item() == Pages.BAD_PAGE and req.tolist().count(1) == 9 and slot.tolist().count(-1) > 9
+    taken = set(c.table.cpu().numpy()[0, :4].tolist())
+    assert not taken & {s // 4 for s in live}

@@ -53,7 +53,7 @@ long long lg_debug_paged_place(const struct lg_paged_cache *c, int page, int row
  * gives up go back in the opposite order, so that a step which rolls a step back leaves the stack as it was.  Updated: table
  * (-1 behind the last page given back), len, the stack.  Written: d_start [n_req + 1], first new token of each request in the step's token rows; for
  * each row its position, its slot (page * page_size + row in the page) and its request, in d_pos, d_slot, d_req [cap] (each may be
- * NULL), -1 in rows behind the last token.
+ * NULL; without any of them cap is only the limit below, up to 2^31 - 1), -1 in rows behind the last token.
  * Requests are served in order while pages and rows (cap) last: one that needs more than is left, or more than max_pages, stays as it is,
  * with no token in the step.  Values of d_keep above len count as len, negative ones as 0.  An entry of the table that is no page goes onto the
  * stack as -1, and whoever takes that has rows without slots.  Tables and outputs do not overlap. */

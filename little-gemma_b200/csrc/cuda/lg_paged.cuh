@@ -151,7 +151,9 @@ template <int PER> __global__ void __launch_bounds__(LG_STEP_THREADS, 1) lg_page
     if (tid == 0) { start[R] = (int)all[1]; if (rank == 0) a.start[R] = (int)all[1]; }
     __syncthreads();
     // tokens: the request whose rows hold row i, its place, and the page there -- from the table, or from the stack if this step takes it
-    for (int i = rank * LG_STEP_THREADS + tid; i < a.cap; i += ranks * LG_STEP_THREADS) {
+    const long long rows = a.pos || a.slot || a.req ? a.cap : all[1];         // (at most cap)
+    for (long long row = rank * LG_STEP_THREADS + tid; row < rows; row += (long long)ranks * LG_STEP_THREADS) {
+        const int i = (int)row;
         int pos = -1, slot = -1, req = -1;
         if (i < (int)all[1]) {
             int lo = 0, hi = R;                        // start[lo] <= i < start[hi]

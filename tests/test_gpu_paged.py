@@ -715,3 +715,17 @@ def test_an_entry_that_is_no_page_brings_none_back(lg, n):
     assert c.status.item() == Pages.BAD_PAGE and req.tolist().count(1) == 9 and slot.tolist().count(-1) > 9
     taken = set(c.table.cpu().numpy()[0, :4].tolist())
     assert not taken & {s // 4 for s in live}
+
+
+def test_a_step_without_outputs_for_tokens_has_no_limit_of_rows(lg):
+    """The largest cap there is, with pos, slot and req NULL: the loop over rows ends at the step's own."""
+    import ctypes
+    rng = np.random.default_rng(15)
+    c = _Cache(lg, rng, [5, 0, 16, 3000], 16, 200, 20)
+    for new, keep in (([3, 1, 0, 90], None), ([0, 0, 0, 0], [5, 0, 9, 3000]), ([1, 0, 1 << 30, 2], None)):
+        start, d_new, d_keep = _i32([-7] * 5), _i32(new), None if keep is None else _i32(keep)
+        assert lg.load().lg_paged_step(ctypes.byref(c.c.desc), 4, d_keep.data_ptr() if keep else None, d_new.data_ptr(), (1 << 31) - 1, start.data_ptr(), None, None, None, None) == 0
+        want = c.oracle.step(new, 200, keep)
+        assert start.tolist() == want[0] and c.status.item() == want[4]
+        assert c.len.tolist() == c.oracle.len.tolist() and np.array_equal(c.table.cpu().numpy(), c.oracle.table) and c.n_free.item() == c.oracle.n_free
+        c.status.zero_()

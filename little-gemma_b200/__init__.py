@@ -396,12 +396,15 @@ class PagedCache:
                               _array(status, "torch.int32", 1, "status"))
         self._ref = C.byref(self.desc)
 
-    def step(self, new, start, pos=None, slot=None, req=None, keep=None, stream: int = 0) -> None:
+    def step(self, new, start, pos=None, slot=None, req=None, keep=None, stream: int = 0, cap: int | None = None) -> None:
         """Requests 0 .. len(new)-1 keep their first `keep` rows (None: all) and get `new` rows more: pages, table, lengths and stack are
-        brought up to date; start [requests + 1] and, for each token of the step, pos, slot and req (-1 behind the last) are written."""
+        brought up to date; start [requests + 1] and, for each token of the step, pos, slot and req (-1 behind the last) are written.
+        cap: tokens that the step has room for; None: as many as the smallest of pos, slot and req holds -- without any of them 0, so that
+        only requests without new rows (a roll-back, a release) are served.  A request that is not served stays as it is, with a bit in `status`."""
         n = new.numel()
         rows = [t.numel() for t in (pos, slot, req) if t is not None]
-        cap = min(rows) if rows else 0
+        if cap is None:
+            cap = min(rows) if rows else 0
         i32 = "torch.int32"
         _ok(self.L.lg_paged_step(self._ref, n, _array(keep, i32, n, "keep"), _array(new, i32, n, "new"), cap, _array(start, i32, n + 1, "start"),
                                  _array(pos, i32, cap, "pos"), _array(slot, i32, cap, "slot"), _array(req, i32, cap, "req"), stream), "paged step")

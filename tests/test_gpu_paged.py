@@ -729,3 +729,16 @@ def test_a_step_without_outputs_for_tokens_has_no_limit_of_rows(lg):
         assert start.tolist() == want[0] and c.status.item() == want[4]
         assert c.len.tolist() == c.oracle.len.tolist() and np.array_equal(c.table.cpu().numpy(), c.oracle.table) and c.n_free.item() == c.oracle.n_free
         c.status.zero_()
+
+
+def test_a_step_without_outputs_serves_what_its_cap_allows(lg):
+    rng = np.random.default_rng(16)
+    c = _Cache(lg, rng, [5, 0, 16], 16, 8, 9)
+    start = _i32([-7] * 4)
+    c.c.step(_i32([3, 1, 0]), start)                           # no room given: nobody with new rows
+    assert start.tolist() == [0, 0, 0, 0] and c.len.tolist() == [5, 0, 16] and c.status.item() == Pages.NO_ROWS
+    c.status.zero_()
+    c.c.step(_i32([3, 1, 20]), start, cap=24)
+    want = c.oracle.step([3, 1, 20], 24)
+    assert start.tolist() == want[0] == [0, 3, 4, 24] and c.len.tolist() == [8, 1, 36] and c.status.item() == 0
+    assert np.array_equal(c.table.cpu().numpy(), c.oracle.table)

@@ -171,3 +171,26 @@ def test_plain_draw_on_hand_made_rows():
     # 1 / (2 + e + e^2) = 0.3995 < 0.4: the first of the order is not enough
     assert draw(x, 0.0, min_p=0.5) == (1, 0.5) and draw(x, 0.99, top_p=0.4)[0] == 3 and draw(x, 0.3, temperature=0.0) == (1, 1.0)
     assert draw([np.nan, -np.inf], 0.5) == (-1, 0.0) and draw([np.inf, 0.0, np.inf], 0.6) == (2, 0.5)
+
+
+def test_room_of_a_step(lg):
+    """cap: the smallest output's size, 0 without outputs, or what the caller says -- which the outputs have to hold."""
+    i = lambda n: _Tensor((n,), "int32")  # noqa: E731
+    kv = _Tensor((9, 16, 2, 64), "float16")
+    c = lg.PagedCache(kv, kv, _Tensor((4, 5), "int32"), i(4), i(9), i(1))
+    caps = []
+
+    class Lib:
+        @staticmethod
+        def lg_paged_step(ref, n, keep, new, cap, *rest):
+            caps.append(cap)
+            return 0
+
+    c.L = Lib
+    c.step(i(4), i(5))
+    c.step(i(4), i(5), i(7), i(6))
+    c.step(i(4), i(5), cap=100)
+    c.step(i(4), i(5), i(7), i(6), cap=5)
+    assert caps == [0, 6, 100, 5]
+    with pytest.raises(ValueError):
+        c.step(i(4), i(5), i(7), i(6), cap=7)

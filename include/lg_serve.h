@@ -54,8 +54,11 @@ long long lg_debug_paged_place(const struct lg_paged_cache *c, int page, int row
  * (-1 behind the last page given back), len, the stack.  Written: d_start [n_req + 1], first new token of each request in the step's token rows; for
  * each row its position, its slot (page * page_size + row in the page) and its request, in d_pos, d_slot, d_req [cap] (each may be
  * NULL; without any of them cap is only the limit below, up to 2^31 - 1), -1 in rows behind the last token.
- * Requests are served in order while pages and rows (cap) last: one that needs more than is left, or more than max_pages, stays as it is,
- * with no token in the step.  Values of d_keep above len count as len, negative ones as 0.  An entry of the table that is no page goes onto the
+ * Who is served is settled in this order.  One that would have more than max_pages pages is not.  Then pages, in the order of the requests: the first that
+ * needs more than are left is not served, and neither is a later one that needs any (pages given up in a step can be taken from the next on).  Then rows (cap), among those that have their pages: the first
+ * whose tokens do not fit is not, and neither is a later one with tokens; pages set aside for such a request stay on the stack and are not offered to
+ * another.  A request that is not served stays as it is, with no token in the step and a status bit; one that needs neither is always served.
+ * Values of d_keep above len count as len, negative ones as 0.  An entry of the table that is no page goes onto the
  * stack as -1, and whoever takes that has rows without slots.  Tables and outputs do not overlap. */
 int  lg_paged_step(const struct lg_paged_cache *c, int n_req, const int *d_keep, const int *d_new, int cap, int *d_start, int *d_pos,
                    int *d_slot, int *d_req, void *stream);

@@ -742,3 +742,12 @@ def test_a_step_without_outputs_serves_what_its_cap_allows(lg):
     want = c.oracle.step([3, 1, 20], 24)
     assert start.tolist() == want[0] == [0, 3, 4, 24] and c.len.tolist() == [8, 1, 36] and c.status.item() == 0
     assert np.array_equal(c.table.cpu().numpy(), c.oracle.table)
+
+
+def test_who_is_served_goes_by_the_declared_rule(lg):
+    from tests.test_serve_cpu import SERVED
+    for (lens, new, free, cap), (served, status) in SERVED:
+        c = _Cache(lg, np.random.default_rng(1), lens, 16, 4, free)
+        start, *_ = c.step(new, cap)
+        assert c.len.tolist() == [n + m * s for n, m, s in zip(lens, new, served)] and c.status.item() == status
+        assert start.tolist() == [sum(m * s for m, s in zip(new[:i], served[:i])) for i in range(len(new) + 1)]

@@ -194,3 +194,26 @@ def test_room_of_a_step(lg):
     assert caps == [0, 6, 100, 5]
     with pytest.raises(ValueError):
         c.step(i(4), i(5), i(7), i(6), cap=7)
+
+
+# (lengths, new tokens, free pages, cap): who is served, and the status -- pages of 16 rows, 4 columns, by the rules of include/lg_serve.h
+SERVED = [
+    (([16, 16], [17, 1], 2, 1), ([0, 0], Pages.NO_ROWS | Pages.NO_PAGES)),       # pages first: both are request 0's, which then has no rows; they are not offered again
+    (([16, 16, 16, 3], [17, 33, 1, 2], 3, 100), ([1, 0, 0, 1], Pages.NO_PAGES)),  # one page would do for request 2, behind one that had too few
+    (([1, 1, 1, 16], [5, 6, 2, 0], 0, 9), ([1, 0, 0, 1], Pages.NO_ROWS)),         # two rows would do for request 2, behind one that had too few
+    (([60, 16, 0], [5, 1, 0], 1, 9), ([0, 1, 1], Pages.TOO_LONG)),
+]
+
+
+@pytest.mark.parametrize("case,want", SERVED)
+def test_who_is_served(case, want):
+    lens, new, free, cap = case
+    table = np.full((len(lens), 4), -1)
+    at = free
+    for r, n in enumerate(lens):
+        k = -(-n // 16)
+        table[r, :k] = range(at, at + k)
+        at += k
+    p = Pages(table, lens, list(range(at)), free, 16)
+    *_, status = p.step(new, cap)
+    assert p.len.tolist() == [n + m * s for n, m, s in zip(lens, new, want[0])] and status == want[1]

@@ -430,6 +430,8 @@ class PagedCache:
         work: attn_work() bytes of device memory that no other call uses at the same time."""
         if len(q.shape) != 3 or q.shape != out.shape or q.dtype != out.dtype:
             raise ValueError("q and out: two tensors [rows, heads, head_dim] of one type are wanted")
+        if not work.is_contiguous():                           # its bytes are those from its address on
+            raise ValueError("work: a contiguous tensor is wanted")
         heads = q.shape[1]
         pq, tq, lq, rows = _rows(q, heads, self.dim, "q")
         po, _, lo, _ = _rows(out, heads, self.dim, "out")

@@ -217,3 +217,19 @@ def test_who_is_served(case, want):
     p = Pages(table, lens, list(range(at)), free, 16)
     *_, status = p.step(new, cap)
     assert p.len.tolist() == [n + m * s for n, m, s in zip(lens, new, want[0])] and status == want[1]
+
+
+def test_a_workspace_in_pieces_is_refused(lg):
+    """One element expanded to the size that is asked for is not that many bytes."""
+    kv, q = _Tensor((9, 16, 2, 64), "float16"), _Tensor((4, 4, 64), "float16")
+    c = lg.PagedCache(kv, kv, _Tensor((4, 5), "int32"), _Tensor((4,), "int32"))
+
+    class Lib:
+        @staticmethod
+        def lg_paged_attn(*args):
+            raise AssertionError("called")
+
+    c.L = Lib
+    for stride in ((0,), (2,)):
+        with pytest.raises(ValueError, match="work"):
+            c.attn(q, q, _Tensor((1 << 24,), "uint8", stride))

@@ -346,7 +346,8 @@ __device__ __forceinline__ int paged_len(const LgPagedAttnArgs &a, int r) {
 // power of two per row, 22 bits; bf16: 3, 24 bits), P as 2 parts (3 where the answer is f32 and the cache bf16; 2 of bf16 are 16 bits of a weight, off by 2^-18 of it
 // at most, for an answer of 8 bits); P carries a factor 2^15 in f16 so that
 // weights down to 2^-29 of the largest stay normal numbers.  Everything else is f32.  Rows of an f32 cache are split in registers into three bf16 parts
-// (24 bits); of the nine products of parts the six that reach the last bits of an f32 are computed.
+// (24 bits); of the nine products of parts the six that reach the last bits of an f32 are computed.  As an addition to a large sum cuts off, products of lower
+// parts are added up before the first ones or apart from them: f32 caches are then 1.3e-7 to 6e-7 (norm) off the 64-bit answer, with all in one sum 3e-7 to 1.8e-6.
 #define LG_PA_MAX_CTAS 296             // two per SM
 #define LG_PA_ITEM_COST 6              // of an item beside its slices, in slices: queries in, warps' results together, rows out
 #define LG_PA_MIN_STRETCH 8
@@ -443,10 +444,10 @@ template <int W> struct LgWalk {
 
 template <typename TQ, typename TC, int HD, int NT> struct LgPagedTile {
     typedef typename std::conditional<std::is_same<TC, __half>::value, __half, __nv_bfloat16>::type TM;      // the matrix instructions' type
-    static constexpr bool SAME = sizeof(TQ) == 2, F32 = sizeof(TC) == 4;
+    static constexpr bool SAME16 = sizeof(TQ) == 2, F32 = sizeof(TC) == 4;    // 16-bit queries; f32 cache
     static constexpr bool F16 = std::is_same<TC, __half>::value;
-    static constexpr int NQ = SAME ? 1 : F16 ? 2 : 3;                         // parts of a query
-    static constexpr int NP = SAME || F16 ? 2 : 3;                            // parts of a weight
+    static constexpr int NQ = SAME16 ? 1 : F16 ? 2 : 3;                       // parts of a query
+    static constexpr int NP = SAME16 || F16 ? 2 : 3;                          // parts of a weight
     static constexpr bool LONG = sizeof(TQ) == 4 && HD > 128;                 // f32 answers: scores added up with rounding to nearest too, every 128 dims
     static constexpr int KS = HD / 16;
     static constexpr int ROWS = 8 * NT;
@@ -484,11 +485,14 @@ template <typename P> __device__ __forceinline__ void paged_copy_unit(const void
 // Scores of a slice whose K lies at `at`; query(i): fragment i of the queries
 template <typename P, int NT, typename Q> __device__ __forceinline__ void paged_scores(uint32_t at, int lane, Q &&query, float (&x)[NT][4]) {
     const int g = lane >> 2, t4 = lane & 3;
-    float sc[NT][2][4];                                                       // two chains of products
+    // chains of products: those of the first parts in one, as each addition to a large sum cuts off, the others in one (f32 caches: two) of their own
+    constexpr int CH = P::F32 ? 3 : 2;
+    float sc[NT][CH][4];
     #pragma unroll
     for (int nt = 0; nt < NT; nt++)
         #pragma unroll
-        for (int j = 0; j < 4; j++) sc[nt][0][j] = sc[nt][1][j] = 0.0f;
+        for (int c = 0; c < CH; c++) sc[nt][c][0] = sc[nt][c][1] = sc[nt][c][2] = sc[nt][c][3] = 0.0f;
+    auto total = [&](int nt, int j) { return P::F32 ? sc[nt][0][j] + (sc[nt][1][j] + sc[nt][CH - 1][j]) : sc[nt][0][j] + sc[nt][1][j]; };
     float sum[P::LONG ? NT : 1][4];
     if (P::LONG) {
         #pragma unroll
@@ -516,20 +520,24 @@ template <typename P, int NT, typename Q> __device__ __forceinline__ void paged_
                 const uint2 v = query((nt * P::NQ + part) * P::KS + ks);
                 #pragma unroll
                 for (int own = 0; own < (P::F32 ? 3 : 1); own++)
-                    if (own + part < 3) mma_16<typename P::TM>(sc[nt][ks & 1], k4[own], v.x, v.y);
+                    if (own + part < 3) mma_16<typename P::TM>(sc[nt][P::SAME16 ? ks & 1 : !own && !part ? 0 : P::F32 ? 1 + (own + part + ks & 1) : 1], k4[own], v.x, v.y);
             }
         if (P::LONG && ks % 8 == 7 && ks != P::KS - 1) {
             #pragma unroll
             for (int nt = 0; nt < NT; nt++)
                 #pragma unroll
-                for (int j = 0; j < 4; j++) { sum[nt][j] += sc[nt][0][j] + sc[nt][1][j]; sc[nt][0][j] = sc[nt][1][j] = 0.0f; }
+                for (int j = 0; j < 4; j++) {
+                    sum[nt][j] += total(nt, j);
+                    #pragma unroll
+                    for (int c = 0; c < CH; c++) sc[nt][c][j] = 0.0f;
+                }
         }
     }
     #pragma unroll
     for (int nt = 0; nt < NT; nt++)
         #pragma unroll
         for (int j = 0; j < 4; j++) {
-            x[nt][j] = sc[nt][0][j] + sc[nt][1][j];
+            x[nt][j] = total(nt, j);
             if (P::LONG) x[nt][j] += sum[nt][j];
         }
 }
@@ -888,9 +896,9 @@ __global__ void __launch_bounds__((LgPagedTile<TQ, TC, HD, NT>::W * 32), (LgPage
                 for (int nt = 0; nt < NT; nt++) {
                     float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     #pragma unroll
-                    for (int part = 0; part < P::NP; part++)
+                    for (int part = P::NP - 1; part >= 0; part--)             // the smallest first: each addition to a large sum cuts off
                         #pragma unroll
-                        for (int own = 0; own < (P::F32 ? 3 : 1); own++)
+                        for (int own = P::F32 ? 2 : 0; own >= 0; own--)
                             if (own + part < 3) mma_16<typename P::TM>(add, v4[own], pb[nt][part][0], pb[nt][part][1]);
                     #pragma unroll
                     for (int j = 0; j < 4; j += 2) fma2(o[ks][nt][j], o[ks][nt][j + 1], f[nt][0], f[nt][1], add[j], add[j + 1]);

@@ -751,3 +751,21 @@ def test_who_is_served_goes_by_the_declared_rule(lg):
         start, *_ = c.step(new, cap)
         assert c.len.tolist() == [n + m * s for n, m, s in zip(lens, new, served)] and c.status.item() == status
         assert start.tolist() == [sum(m * s for m, s in zip(new[:i], served[:i])) for i in range(len(new) + 1)]
+
+
+@pytest.mark.parametrize("cache", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (6, 3, 128), (4, 2, 256), (8, 1, 512)])
+def test_f32_answers_are_as_exact_as_f32_sums(lg, cache, heads, kv_heads, dim):
+    """The error in the norm.  A score (1.5 on average) is a sum in 8 steps per 128 dims, each of which cuts off half of 2^-23 of a partial sum, half the score, on
+    average: 3 2^-23; as much for the sums over 128 dims, the lower parts, scale and maximum together; 2^-22 for the exponential: an error of a weight of
+    8 2^-23, which is the answer's."""
+    import torch
+    torch.manual_seed(dim)
+    n, page = 4000, 16
+    k, v = (torch.randn((n // page, page, kv_heads, dim), device="cuda").to(getattr(torch, cache)) for _ in range(2))
+    c = lg.PagedCache(k, v, _i32(np.arange(n // page)[None]), _i32([n]))
+    q = 1.5 * torch.randn((1, heads, dim), device="cuda")
+    out = torch.empty_like(q)
+    c.attn(q, out, torch.empty(c.attn_work(1, 1, heads), dtype=torch.uint8, device="cuda"))
+    want = attention(q.double().cpu().numpy(), k.flatten(0, 1).double().cpu().numpy(), v.flatten(0, 1).double().cpu().numpy(), dim ** -0.5, [n - 1])
+    assert np.linalg.norm(out.double().cpu().numpy() - want) <= 2.0 ** -20 * np.linalg.norm(want)

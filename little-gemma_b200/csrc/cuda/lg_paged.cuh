@@ -343,9 +343,8 @@ __device__ __forceinline__ int paged_len(const LgPagedAttnArgs &a, int r) {
 // to nearest and the factor of a moved maximum in the same operation: the instructions' own additions cut off, always towards zero, which over 131072 f16 rows of
 // one sign took 8.6e-5 from the result (0.18 of half a step) where this is 1.7e-6 off.  It costs nothing where copies are the bound (96 bf16 requests up to 16383
 // rows: 558 us either way), 17 % with 16-bit heads of 512, 5 to 11 % with 32 query rows a KV head.  Numerics: an f32 query enters as a sum of 16-bit parts (f16: 2 parts behind a
-// power of two per row, 22 bits; bf16: 3, 24 bits), P as 2 parts of f16, 22 bits, or 3 of bf16, 24 bits; bf16
-// answers with more than 8 query rows a KV head, or heads above 256, have 2 of bf16, 16 bits, as the third product would cost 5 to 10 % there and nothing
-// elsewhere (96 requests up to 16383 rows: differing roundings of the answers 7.3e-5 of the norm with 2, 4.7e-5 with 3, 7.8e-5 in 32-bit torch).  P carries a factor 2^15 in f16 so that
+// power of two per row, 22 bits; bf16: 3, 24 bits), P as 2 parts (3 where the answer is f32 and the cache bf16; 2 of bf16 are 16 bits of a weight, off by 2^-18 of it
+// at most, for an answer of 8 bits); P carries a factor 2^15 in f16 so that
 // weights down to 2^-29 of the largest stay normal numbers.  Everything else is f32.  Rows of an f32 cache are split in registers into three bf16 parts
 // (24 bits); of the nine products of parts the six that reach the last bits of an f32 are computed.  As an addition to a large sum cuts off, products of lower
 // parts are added up before the first ones or apart from them: f32 caches are then 1.3e-7 to 6e-7 (norm) off the 64-bit answer, with all in one sum 3e-7 to 1.8e-6.
@@ -448,7 +447,7 @@ template <typename TQ, typename TC, int HD, int NT> struct LgPagedTile {
     static constexpr bool SAME16 = sizeof(TQ) == 2, F32 = sizeof(TC) == 4;    // 16-bit queries; f32 cache
     static constexpr bool F16 = std::is_same<TC, __half>::value;
     static constexpr int NQ = SAME16 ? 1 : F16 ? 2 : 3;                       // parts of a query
-    static constexpr int NP = F16 || (SAME16 && (NT > 1 || HD > 256)) ? 2 : 3;      // parts of a weight
+    static constexpr int NP = SAME16 || F16 ? 2 : 3;                          // parts of a weight
     static constexpr bool LONG = sizeof(TQ) == 4 && HD > 128;                 // f32 answers: scores added up with rounding to nearest too, every 128 dims
     static constexpr int KS = HD / 16;
     static constexpr int ROWS = 8 * NT;

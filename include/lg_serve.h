@@ -77,8 +77,12 @@ int  lg_paged_append(const struct lg_paged_cache *c, const void *d_k, const void
  * before, with window > 0 the nearest `window` of them.  A query that sees nothing (a length of 0, pages that are not in the cache) gives
  * zeros.  scale 0: 1 / sqrt(head_dim).  What a query does not see does not reach it, inf and NaN included.  V rows that it sees may hold any
  * numbers: inf gives inf, inf of both signs or NaN give NaN, and a mean of large numbers is none larger; such calls take several times as long.  q and the
- * K rows that it sees are finite, below 2^127 where they are f32.  Every sum has an order that the call's sizes and lengths
- * fix: the same call gives the same bits.
+ * K rows that it sees are finite, below 2^127 where they are f32.
+ * Every sum is held in f32 and has an order that the call's sizes and lengths fix: the same call gives the same bits.  The work of a call is cut over all
+ * its requests, so a request's answer can have other last bits beside other requests, and a token in a block others than alone.  Products are of
+ * 16-bit numbers: an f32 query enters with 22 bits of its row's largest element over an f16 cache, with 24 over others; f32 K and V with 24; the weights with
+ * 22 bits over f16 and 24 over others, but 16 for bf16 answers.  f32 answers are 1e-7 to 7e-7 of their norm off 64-bit ones, as 32-bit sums are; 16-bit
+ * answers are off by their rounding.
  * d_work: lg_paged_attn_work bytes, 16-byte aligned, this call's alone until the call's work has ended: calls and graphs that may
  * overlap have workspaces of their own. */
 long long lg_paged_attn_work(const struct lg_paged_cache *c, int n_req, int n_new, int n_heads);

@@ -89,7 +89,7 @@ __device__ __forceinline__ void block_scan3(long long (&v)[3], long long (&total
 // taken, tokens, pages returned -- say where each request's things go, and every token and page then finds its place on its own.  Where
 // pages or rows do not suffice, two more sums decide who is served: a request that is not takes no pages, and neither does any later one
 // that needs some, so the pages taken are always the top of the stack in one piece.  Bound by latency: a step and its roll-back
-// take 9.4 us for 48 requests, 23 us for 2048 with 40576 tokens (one CTA, with the requests looked up again for every token: 274).
+// take 10.3 us for 48 requests, 23 us for 2048 with 40576 tokens (one CTA, with the requests looked up again for every token: 274).
 template <int PER> __global__ void __launch_bounds__(LG_STEP_THREADS, 1) lg_paged_step_kernel(LgStepArgs a) {
     extern __shared__ int sm[];
     __shared__ long long red[32][3];
@@ -263,8 +263,8 @@ template <typename T> struct Eight<T, T> {
 };
 
 // A thread moves 8 elements of a row at a time, two such pieces under way, K's and V's; a CTA has one row, or as many whole ones as its threads cover, and
-// goes on to the next.  Rows of one type are not looked at.  Bound by the bytes in and out: 8191 rows of 8 heads of 256 in bf16 take 18.6 to 25 us (134 MB; a division a piece and
-// conversion through f32 cost 30), 48 rows 1.9 us.
+// goes on to the next.  Rows of one type are not looked at.  Bound by the bytes in and out: 8191 rows of 8 heads of 256 in bf16 take 24 us (134 MB, three sets in turn; a division a piece and
+// conversion through f32 cost 30), 48 rows 2.1 us.
 template <typename TI, typename TC> __global__ void __launch_bounds__(LG_APPEND_THREADS) lg_paged_append_kernel(LgAppendArgs a) {
     const int per_head = a.c.hd >> 3, half = per_head * a.c.n_kv, units = 2 * half;
     const int here = units < LG_APPEND_THREADS ? (int)threadIdx.x / units : 0, rows = units < LG_APPEND_THREADS ? LG_APPEND_THREADS / units : 1;
@@ -332,22 +332,24 @@ __device__ __forceinline__ int paged_len(const LgPagedAttnArgs &a, int r) {
 // The work is a line of slices of 16 keys: request by request, KV head by KV head, group of 8 NT query rows by group (an item).  Every CTA of a
 // persistent grid takes a stretch of equal length of that line, so ragged lengths cost nothing; an item that one stretch holds is written at once,
 // of one that several stretches share each leaves (max, sum, output), and lg_paged_merge_kernel adds those in their order.
-// (Spans fixed by a request's own length: 876 us for 96 requests of 1.6K to 16K rows where this takes 539, the copy's bandwidth; short spans cost merges, and
-// about as many items as CTAs leave SMs idle: 153 us for two requests of 120000 rows where this takes 97.)
+// (Spans fixed by a request's own length took 876 us for 96 requests of 1.6K to 16K rows where this took 539, one set of inputs replayed: short spans cost
+// merges, and about as many items as CTAs leave SMs idle: 153 us for two requests of 120000 rows where this took 97.)
 //
 // Inside a CTA every warp works alone: it takes 16 keys (a slice) at a time, brings K and V in with 16-byte asynchronous copies through a ring
 // of U units of its own (a unit: 16 rows of K or of V; rows that no query may see are filled with zeros and never read), so the loop has no block barrier and
 // runs ahead across items.  Both products have the keys / head dims on the 16-row side and 8 queries as columns:
 //   S^T (16 keys x 8) = K Q^T, softmax with a running maximum per column in the accumulator's own lanes, O^T (16 dims x 8) += V^T P^T,
-// P^T turned from accumulator order into operand order by movmatrix.  A slice's products are added to the outputs outside of the matrix instructions, with rounding
-// to nearest and the factor of a moved maximum in the same operation: the instructions' own additions cut off, always towards zero, which over 131072 f16 rows of
-// one sign took 8.6e-5 from the result (0.18 of half a step) where this is 1.7e-6 off.  It costs nothing where copies are the bound (96 bf16 requests up to 16383
-// rows: 558 us either way), 17 % with 16-bit heads of 512, 5 to 11 % with 32 query rows a KV head.  Numerics: an f32 query enters as a sum of 16-bit parts (f16: 2 parts behind a
-// power of two per row, 22 bits; bf16: 3, 24 bits), P as 2 parts (3 where the answer is f32 and the cache bf16; 2 of bf16 are 16 bits of a weight, off by 2^-18 of it
-// at most, for an answer of 8 bits); P carries a factor 2^15 in f16 so that
-// weights down to 2^-29 of the largest stay normal numbers.  Everything else is f32.  Rows of an f32 cache are split in registers into three bf16 parts
-// (24 bits); of the nine products of parts the six that reach the last bits of an f32 are computed.  As an addition to a large sum cuts off, products of lower
-// parts are added up before the first ones or apart from them: f32 caches are then 1.3e-7 to 6e-7 (norm) off the 64-bit answer, with all in one sum 3e-7 to 1.8e-6.
+// P^T turned from accumulator order into operand order by movmatrix.
+//
+// Numerics.  An f32 query enters as a sum of 16-bit parts (f16: 2 parts behind a power of two per row, 22 bits; bf16: 3, 24 bits), P as 2 parts (3 where the
+// answer is f32 and the cache bf16; 2 of bf16 are 16 bits of a weight, off by 2^-18 of it at most, for an answer of 8 bits: the third takes 5 % more time
+// over many calls of 96 requests up to 16383 rows); P carries a factor 2^15 in f16 so that weights down to 2^-29 of the largest stay normal numbers.  Rows of an
+// f32 cache are split in registers into three bf16 parts (24 bits); of the nine products of parts the six that reach the last bits of an f32 are
+// computed.  The matrix instructions' additions cut off, always towards zero.  So a slice's products are added to the outputs outside of them, with rounding to
+// nearest and the factor of a moved maximum in the same operation: over 131072 f16 rows of one sign a sum inside took 8.6e-5 from the result (0.18 of half
+// a step), this 1.7e-6; it costs nothing where copies are the bound, 15 % with 16-bit heads of 512, 4 to 7 % with 16 query rows a KV head and more.  And products
+// of lower parts are added up before the first ones or apart from them: f32 caches are 1.3e-7 to 6e-7 (norm) off the 64-bit answer, with all in one sum
+// 3e-7 to 1.8e-6.  Everything else is f32.  Outputs that are not finite are computed again, see paged_key_by_key.
 #define LG_PA_MAX_CTAS 296             // two per SM
 #define LG_PA_ITEM_COST 6              // of an item beside its slices, in slices: queries in, warps' results together, rows out
 #define LG_PA_MIN_STRETCH 8

@@ -15,8 +15,10 @@
 //   fine    exact counts or weights over 1024 equal parts of that interval of keys (the logits as ordered integers), then of the part that holds the threshold,
 //           until a part is a single key: at most four rounds.  Where the lists hold the interval, every CTA fetches its tokens and does the rounds alone;
 //           otherwise (flat rows) the histograms of a round are added up over the cluster
-// Bound by the instructions of a pass over the row (about 30 a token and weight, 14 of them 64-bit arithmetic) and, for few rows, by the cluster barriers: one
-// row of 262144 with top-k and top-p 29 us, 48 rows with top-p and min-p 126 us, 512 rows of 32768 without filters 47 us.
+// Not at a limit of the device: 61 warp instructions per 32 tokens with temperature alone (29 of them a weight, 14 in 64 bits) and 170 with top-p and min-p fill
+// 57 and 43 % of the issue slots of two CTAs an SM (64 registers allow no third); the rest is waiting, for block and cluster barriers, results and the 64-bit
+// pipe, and a second round of CTAs where there are more than 296.  Few rows: cluster barriers, and code that is fetched for the first time.  One row of
+// 262144 with top-k and top-p 30 us, 48 rows with top-p and min-p 137 us, 512 rows of 32768 without filters 49 us.
 #pragma once
 #include "lg_device.cuh"
 #include <cuda_bf16.h>

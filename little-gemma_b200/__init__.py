@@ -405,6 +405,8 @@ class PagedCache:
         rows = [t.numel() for t in (pos, slot, req) if t is not None]
         if cap is None:
             cap = min(rows) if rows else 0
+        if not 0 <= cap < 1 << 31:
+            raise ValueError("cap: a number of tokens below 2^31 is wanted")
         i32 = "torch.int32"
         _ok(self.L.lg_paged_step(self._ref, n, _array(keep, i32, n, "keep"), _array(new, i32, n, "new"), cap, _array(start, i32, n + 1, "start"),
                                  _array(pos, i32, cap, "pos"), _array(slot, i32, cap, "slot"), _array(req, i32, cap, "req"), stream), "paged step")

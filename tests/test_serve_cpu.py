@@ -192,8 +192,9 @@ def test_room_of_a_step(lg):
     c.step(i(4), i(5), cap=100)
     c.step(i(4), i(5), i(7), i(6), cap=5)
     assert caps == [0, 6, 100, 5]
-    with pytest.raises(ValueError):
-        c.step(i(4), i(5), i(7), i(6), cap=7)
+    for args, cap in (((i(7), i(6)), 7), ((), -1), ((), 1 << 32)):
+        with pytest.raises(ValueError):
+            c.step(i(4), i(5), *args, cap=cap)
 
 
 # (lengths, new tokens, free pages, cap): who is served, and the status -- pages of 16 rows, 4 columns, by the rules of include/lg_serve.h
